@@ -195,10 +195,10 @@ def _lse(z):
 
 
 def _plain_quantize(x):
-    x = x.float()
-    scales = x.abs().amax(1) / 127.0
-    # a quotient next to a half decides by its 64-bit value
-    return (x.double() / scales.double()[:, None]).round().to(torch.int8), scales
+    # quotients in 64 bits: the scale is the fp32 number nearest to its own, and a code next to a half decides by its exact one
+    x = x.double()
+    scales = (x.abs().amax(1) / 127.0).float()
+    return (x / scales.double()[:, None]).round().to(torch.int8), scales
 
 
 def _plain_matmul(a, b, a_scales, b_scales, bias, dtype):
