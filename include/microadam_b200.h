@@ -37,6 +37,9 @@ extern "C" {
 #define MAB_D2K 1                 /* tools.py:12-14 CopyDirection.d2k */
 
 #define MAB_MAX_WINDOW 128        /* largest m (window rows) the update kernels accept */
+#define MAB_MAX_LIST 1024         /* largest k (entries of a row) mab_topk_logits and mab_distill_* accept */
+#define MAB_MAX_VOCAB 1048576     /* longest row of logits they accept */
+#define MAB_MAX_INNER 131071      /* largest inner size of mab_int8_matmul: 2^14 times it still fits 32 bits */
 
 /* Message of the last failure on the calling thread ("" if none). */
 const char* mab_last_error(void);
@@ -132,6 +135,50 @@ int mab_sparse_rows_dot(int64_t d, int64_t rows, int64_t k, int64_t d_block_size
 int mab_sparse_rows_combine(int64_t d, int64_t rows, int64_t k, int64_t d_block_size, int64_t k_block_size,
                             const float* M, const int16_t* I, const void* V, int v_dtype, void* out, int out_dtype,
                             void* stream);
+
+/* ---- distillation: a frozen teacher in 8 bits, its top logits, the student's loss ---------------------------
+ * No counterpart in the reference.  Rows lie `pitch` elements apart (at least their length) and may start anywhere their
+ * element type allows; they are not read or written beyond their length. */
+
+/* scales[r] = max |x[r, :]| / 127 (0 where that lies below 2^-126), codes[r, c] = the integer nearest x[r, c] / scales[r] (half to
+ * even, the exact quotient decides), 0 where the scale is 0.  A row with a NaN or an infinity: scale NaN, codes 0.  The operands of
+ * mab_int8_matmul: rows are tokens of activations or output channels of weights.  x is read once. */
+int mab_quantize_rows(int64_t rows, int64_t cols, const void* x, int x_dtype, int64_t x_pitch, int8_t* codes,
+                      int64_t codes_pitch, float* scales, void* stream);
+
+/* out[i, j] = (sum_c a[i, c] * b[j, c]) * a_scales[i] * b_scales[j] + bias[j], the sum exact in 32-bit integers, the rest in fp32,
+ * one rounding to out_dtype.  a: [m, k], b: [n, k], bias: [n] or NULL, out: [m, n].  a and b 16-byte aligned, their pitches multiples
+ * of 16; k <= MAB_MAX_INNER. */
+int mab_int8_matmul(int64_t m, int64_t n, int64_t k, const int8_t* a, int64_t a_pitch, const int8_t* b, int64_t b_pitch,
+                    const float* a_scales, const float* b_scales, const float* bias, void* out, int out_dtype, int64_t out_pitch,
+                    void* stream);
+
+/* Per row the k largest logits in descending order (ties: the lower index first; -0 equals +0; NaN below -inf) into values [rows, k]
+ * (the logits' type, unchanged) and indices [rows, k], and rest[r] = log sum exp(logit / temperature) over all others (-inf where
+ * there is nothing, NaN for a row with a NaN).  k <= MAB_MAX_LIST. */
+int mab_topk_logits(int64_t rows, int64_t vocab, int64_t k, const void* logits, int dtype, int64_t pitch, double temperature,
+                    void* values, int32_t* indices, float* rest, void* stream);
+
+/* loss[r] = weights[r] * KL(teacher || student) over the list's tokens and one class for all others, both distributions at
+ * `temperature`: the teacher's from its logits `values` [rows, k] at `indices` [rows, k] and rest[r], the logarithm of the mass of everything
+ * else as mab_topk_logits gives it (NULL: none; the teacher's distribution is that over its list), the student's from
+ * logits [rows, vocab].  An index outside [0, vocab) is an entry that is not there; an index that occurs again counts with the sum of its
+ * entries.  weights [rows] or NULL (all 1): a row with weight 0 is not read, its loss is 0.  A row without a teacher (no entry, no
+ * rest) has loss 0.  stats [rows, 2] and list_grad [rows, k] are what mab_distill_grad needs. */
+int mab_distill_loss(int64_t rows, int64_t vocab, int64_t k, const void* logits, int dtype, int64_t pitch, const int32_t* indices,
+                     const void* values, int v_dtype, const float* rest, const float* weights, double temperature, float* loss,
+                     float* stats, float* list_grad, void* stream);
+
+/* grad[r, v] = grad_loss[r * grad_loss_stride] * dloss[r] / dlogits[r, v], in the logits' type; zeros for a row with weight 0.  grad may be
+ * logits itself. */
+int mab_distill_grad(int64_t rows, int64_t vocab, int64_t k, const void* logits, int dtype, int64_t pitch, const int32_t* indices,
+                     const float* weights, double temperature, const float* stats, const float* list_grad, const float* grad_loss,
+                     int64_t grad_loss_stride, void* grad, int64_t grad_pitch, void* stream);
+
+/* Both in one call, with grad_loss = 1: a row is read from HBM once.  grad may be logits itself. */
+int mab_distill_step(int64_t rows, int64_t vocab, int64_t k, const void* logits, int dtype, int64_t pitch, const int32_t* indices,
+                     const void* values, int v_dtype, const float* rest, const float* weights, double temperature, float* loss,
+                     void* grad, int64_t grad_pitch, void* stream);
 
 /* ---- fused step over a list of tensors ------------------------------------------------------ */
 

@@ -129,5 +129,6 @@ int copy_timeout_f32_split(int* out, bool clear);   // ef_topk_quant_f32.cu
 int copy_timeout_bf16(int* out, bool clear);     // ef_topk_quant_bf16.cu
 int copy_timeout_bf16_warps(int* out, bool clear);  // ef_topk_quant_bf16_warps.cu
 int copy_timeout_window(int* out, bool clear);   // window_adam.cu
+int copy_timeout_int8_matmul(int* out, bool clear);   // int8_matmul.cu
 
 }  // namespace mab

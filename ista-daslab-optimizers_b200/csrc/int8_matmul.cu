@@ -1,0 +1,278 @@
+// out[i, j] = (sum_c a[i, c] b[j, c]) a_scale[i] b_scale[j] + bias[j]: 8-bit operands, exact 32-bit sums.
+//
+// The tensor cores' rows (128 lanes of tensor memory) are output channels (rows of b), their columns tokens (rows of a): a few tokens are a
+// narrow tile, not a nearly empty one, and a warp of the epilogue holds 32 neighbouring channels of one token, so its stores are whole sectors without a
+// detour through shared memory.  One warp issues tiled copies (128 bytes of the inner size, 128-byte swizzle, zeros beyond the edges) into a ring of
+// stages, one thread of another issues the products, four warps take the sums out of tensor memory.  Where there are fewer tiles than SMs the inner
+// size is split over the CTAs of a cluster, whose partial sums meet in distributed shared memory: integers, so in any order the same.
+// One to four tokens are no tile at all: a warp per pair of channels, four products an instruction, bound by the weights' bytes.
+#include "rows.cuh"
+#include "tcgen05.cuh"
+
+namespace mab {
+namespace int8mm {
+
+constexpr int BM = 128, BK = 128;                  // channels of a tile, bytes of the inner size of a stage
+constexpr int THREADS = 192;
+__device__ int g_timeout;
+
+struct Args {
+    const int8_t *a, *b;
+    int64_t a_pitch, b_pitch, out_pitch;
+    const float *a_scales, *b_scales, *bias;
+    void* out;
+    int m, n, k;
+    int token_tiles, split;
+};
+
+__device__ __forceinline__ float scaled(int sum, float token, float channel, float bias) { return fmaf((float)sum * token, channel, bias); }
+
+template <int BN> struct Ring {
+    static constexpr int STAGE = (BM + BN) * BK;
+    static constexpr int STAGES = BN == 256 ? 4 : BN == 128 ? 6 : 8;
+    static constexpr int BYTES = STAGE * STAGES + 1024;
+};
+
+template <typename T, int BN>
+__global__ void __launch_bounds__(THREADS) int8_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                                                              const __grid_constant__ Args g) {
+    using R = Ring<BN>;
+    extern __shared__ unsigned char dyn[];
+    unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~(uintptr_t)1023);
+    __shared__ uint64_t full[R::STAGES], empty[R::STAGES], done;
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_lost;
+    __shared__ float s_token[BN];
+    constexpr uint32_t COLUMNS = BN < 32 ? 32 : BN;
+    const int warp = warp_id(), lane = lane_id(), t = threadIdx.x;
+    const int rank = g.split > 1 ? (int)(blockIdx.x % g.split) : 0;
+    const int tile = blockIdx.x / g.split, token0 = tile % g.token_tiles * BN, channel0 = tile / g.token_tiles * BM;
+    const int steps = (g.k + BK - 1) / BK, k0 = (int)((int64_t)steps * rank / g.split), k1 = (int)((int64_t)steps * (rank + 1) / g.split);
+    if (t == 0) {
+        for (int i = 0; i < R::STAGES; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+        mbar_init(&done, 1);
+        s_lost = 0;
+    }
+    if (warp == 1) tmem_alloc(&s_tmem, COLUMNS);
+    for (int i = t; i < BN; i += THREADS) s_token[i] = token0 + i < g.m ? g.a_scales[token0 + i] : 0.0f;
+    tmem_fence_before();
+    __syncthreads();
+    tmem_fence_after();
+    const uint32_t acc = s_tmem;
+
+    if (warp == 0) {
+        if (lane == 0)
+            for (int i = k0; i < k1; ++i) {
+                const int s = (i - k0) % R::STAGES, round = (i - k0) / R::STAGES;
+                if (round > 0 && !mbar_wait(&empty[s], (round - 1) & 1)) { atomicExch(&s_lost, 1); break; }
+                unsigned char* stage = ring + s * R::STAGE;
+                mbar_arrive_expect_tx(&full[s], R::STAGE);
+                tile_g2s(stage, &map_b, i * BK, channel0, &full[s]);
+                tile_g2s(stage + BM * BK, &map_a, i * BK, token0, &full[s]);
+            }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            for (int i = k0; i < k1; ++i) {
+                const int s = (i - k0) % R::STAGES, round = (i - k0) / R::STAGES;
+                if (!mbar_wait(&full[s], round & 1)) {
+                    atomicExch(&s_lost, 1);         // the copies that may still be on their way: they must not outlive the CTA
+                    for (int n = i; n < k1 && n < i + R::STAGES; ++n) mbar_wait(&full[(n - k0) % R::STAGES], (n - k0) / R::STAGES & 1, 1 << 12);
+                    break;
+                }
+                tmem_fence_after();
+                const uint32_t stage = smem_addr(ring + s * R::STAGE);
+                const uint64_t wd = operand_desc(stage), td = operand_desc(stage + BM * BK);
+#pragma unroll
+                for (int j = 0; j < BK / 32; ++j) mma_i8(acc, wd + 2 * j, td + 2 * j, i8_instruction(BM, BN), i > k0 || j > 0);
+                mma_commit(&empty[s]);
+            }
+            mma_commit(&done);
+        }
+    }
+    __syncwarp();
+    if (!mbar_wait(&done, 0)) atomicExch(&s_lost, 1);
+    tmem_fence_after();
+    __syncthreads();
+    const bool lost = s_lost != 0;
+    if (lost && t == 0) atomicExch(&g_timeout, 1);
+    T* out = reinterpret_cast<T*>(g.out);
+
+    if (g.split == 1) {
+        if (warp >= 2 && !lost) {
+            const int quarter = warp & 3, channel = channel0 + 32 * quarter + lane;
+            const float cs = channel < g.n ? g.b_scales[channel] : 0.0f, bias = g.bias && channel < g.n ? g.bias[channel] : 0.0f;
+            for (int c = 0; c < BN && token0 + c < g.m; c += 16) {
+                int r[16];
+                tmem_load(acc + ((uint32_t)(32 * quarter) << 16) + c, r);
+                tmem_wait_load();
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (channel < g.n && token0 + c + i < g.m)
+                        Elem<T>::store(out, (int64_t)(token0 + c + i) * g.out_pitch + channel, scaled(r[i], s_token[c + i], cs, bias));
+            }
+        }
+    } else {
+        // the cluster's partial sums, [column][channel] in the ring, which every copy and product has left
+        int* part = reinterpret_cast<int*>(ring);
+        if (warp >= 2 && !lost) {
+            const int quarter = warp & 3;
+            for (int c = 0; c < BN; c += 16) {
+                int r[16];
+                tmem_load(acc + ((uint32_t)(32 * quarter) << 16) + c, r);
+                tmem_wait_load();
+#pragma unroll
+                for (int i = 0; i < 16; ++i) part[(c + i) * BM + 32 * quarter + lane] = r[i];
+            }
+        }
+        cluster_arrive_wait();
+        int c0 = BN * rank / g.split, c1 = BN * (rank + 1) / g.split;
+        bool any = false;
+        for (int s = 0; s < g.split; ++s) any |= cluster_load_u32(&s_lost, s) != 0;
+        if (!any)
+            for (int i = c0 * BM + t; i < c1 * BM; i += THREADS) {
+                const int token = token0 + i / BM, channel = channel0 + i % BM;
+                if (token >= g.m || channel >= g.n) continue;
+                int sum = 0;
+                for (int s = 0; s < g.split; ++s) sum += (int)cluster_load_u32(&part[i], s);
+                Elem<T>::store(out, (int64_t)token * g.out_pitch + channel, scaled(sum, s_token[i / BM], g.b_scales[channel], g.bias ? g.bias[channel] : 0.0f));
+            }
+        cluster_arrive_wait();
+    }
+    tmem_fence_before();
+    __syncthreads();
+    if (warp == 1) { tmem_fence_after(); tmem_free(acc, COLUMNS); }
+}
+
+// M tokens (m of them there): a warp for R channels, its lanes over the inner size.
+template <typename T, int M, int R>
+__global__ void __launch_bounds__(256) int8_rows_kernel(const __grid_constant__ Args g) {
+    const int lane = lane_id(), channel0 = (blockIdx.x * 8 + warp_id()) * R;
+    if (channel0 >= g.n) return;
+    int acc[M][R];
+#pragma unroll
+    for (int i = 0; i < M; ++i)
+#pragma unroll
+        for (int r = 0; r < R; ++r) acc[i][r] = 0;
+    const int8_t* b[R];
+    const int8_t* a[M];
+#pragma unroll
+    for (int r = 0; r < R; ++r) b[r] = g.b + (int64_t)min(channel0 + r, g.n - 1) * g.b_pitch;
+#pragma unroll
+    for (int i = 0; i < M; ++i) a[i] = g.a + (int64_t)min(i, g.m - 1) * g.a_pitch;
+    const int whole = g.k / 16;
+#pragma unroll 4
+    for (int v = lane; v < whole; v += 32) {
+        int4 w[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) w[r] = __ldg(reinterpret_cast<const int4*>(b[r]) + v);
+#pragma unroll
+        for (int i = 0; i < M; ++i) {
+            const int4 x = __ldg(reinterpret_cast<const int4*>(a[i]) + v);
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+                acc[i][r] = __dp4a(x.x, w[r].x, __dp4a(x.y, w[r].y, __dp4a(x.z, w[r].z, __dp4a(x.w, w[r].w, acc[i][r]))));
+        }
+    }
+    const int c = whole * 16 + lane;                // the last, partial vector by bytes
+    if (lane < 16 && c < g.k)
+#pragma unroll
+        for (int i = 0; i < M; ++i)
+#pragma unroll
+            for (int r = 0; r < R; ++r) acc[i][r] += (int)a[i][c] * (int)b[r][c];
+#pragma unroll
+    for (int i = 0; i < M; ++i)
+#pragma unroll
+        for (int r = 0; r < R; ++r) acc[i][r] = __reduce_add_sync(0xffffffffu, acc[i][r]);
+#pragma unroll
+    for (int i = 0; i < M; ++i)
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            if (lane == i * R + r && i < g.m && channel0 + r < g.n)
+                Elem<T>::store(reinterpret_cast<T*>(g.out), (int64_t)i * g.out_pitch + channel0 + r,
+                               scaled(acc[i][r], g.a_scales[i], g.b_scales[channel0 + r], g.bias ? g.bias[channel0 + r] : 0.0f));
+}
+
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static EncodeTiled encode_tiled() {
+    static const EncodeTiled fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+            found != cudaDriverEntryPointSuccess) p = nullptr;
+        return reinterpret_cast<EncodeTiled>(p);
+    }();
+    return fn;
+}
+
+// Rows of k bytes, `pitch` apart, in boxes of box_rows x 128 bytes.
+static int make_map(CUtensorMap* map, const int8_t* p, int64_t rows, int64_t k, int64_t pitch, int box_rows) {
+    const EncodeTiled fn = encode_tiled();
+    MAB_REQUIRE(fn, MAB_ERR_CUDA, "cuTensorMapEncodeTiled is not in this driver");
+    const cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)pitch};
+    const cuuint32_t box[2] = {BK, (cuuint32_t)box_rows}, ones[2] = {1, 1};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t*>(p), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    MAB_REQUIRE(r == CUDA_SUCCESS, MAB_ERR_CUDA, "cuTensorMapEncodeTiled failed with %d", (int)r);
+    return MAB_OK;
+}
+
+template <typename T, int BN> int launch_tiles(Args g, int sms, cudaStream_t s) {
+    CUtensorMap map_a, map_b;
+    if (int rc = make_map(&map_a, g.a, g.m, g.k, g.a_pitch, BN)) return rc;
+    if (int rc = make_map(&map_b, g.b, g.n, g.k, g.b_pitch, BM)) return rc;
+    g.token_tiles = (g.m + BN - 1) / BN;
+    const int64_t tiles = (int64_t)g.token_tiles * ((g.n + BM - 1) / BM);
+    const int steps = (g.k + BK - 1) / BK;
+    g.split = 1;
+    while (g.split < 8 && tiles * g.split * 2 <= sms && steps >= 4 * g.split) g.split *= 2;
+    return launch_rows(int8_matmul_kernel<T, BN>, "int8_matmul", tiles * g.split, THREADS, Ring<BN>::BYTES, g.split, s, map_a, map_b, g);
+}
+
+template <typename T> int launch(const Args& g, cudaStream_t s) {
+    const int sms = device_sm_count();
+    if (sms < 0) return MAB_ERR_CUDA;
+    if (g.m <= 4) {
+        const int64_t ctas = ceil_div64(g.n, 16);
+        if (g.m == 1) return launch_rows(int8_rows_kernel<T, 1, 2>, "int8_matmul", ctas, 256, 0, 1, s, g);
+        if (g.m == 2) return launch_rows(int8_rows_kernel<T, 2, 2>, "int8_matmul", ctas, 256, 0, 1, s, g);
+        return launch_rows(int8_rows_kernel<T, 4, 2>, "int8_matmul", ctas, 256, 0, 1, s, g);
+    }
+    if (g.m <= 16) return launch_tiles<T, 16>(g, sms, s);
+    if (g.m <= 32) return launch_tiles<T, 32>(g, sms, s);
+    if (g.m <= 64) return launch_tiles<T, 64>(g, sms, s);
+    if (g.m <= 128) return launch_tiles<T, 128>(g, sms, s);
+    return launch_tiles<T, 256>(g, sms, s);
+}
+
+}  // namespace int8mm
+
+int copy_timeout_int8_matmul(int* out, bool clear) {
+    cudaError_t e = cudaMemcpyFromSymbol(out, int8mm::g_timeout, sizeof(int));
+    if (e == cudaSuccess && clear) { const int z = 0; e = cudaMemcpyToSymbol(int8mm::g_timeout, &z, sizeof(int)); }
+    return e == cudaSuccess ? MAB_OK : cuda_fail(e, "int8_matmul wait flag");
+}
+
+}  // namespace mab
+
+using namespace mab;
+
+extern "C" int mab_int8_matmul(int64_t m, int64_t n, int64_t k, const int8_t* a, int64_t a_pitch, const int8_t* b, int64_t b_pitch,
+                               const float* a_scales, const float* b_scales, const float* bias, void* out, int out_dtype, int64_t out_pitch,
+                               void* stream) {
+    MAB_REQUIRE(m >= 0 && n >= 0 && k >= 1, MAB_ERR_BAD_ARG, "mab_int8_matmul: m=%lld, n=%lld, k=%lld", (long long)m, (long long)n, (long long)k);
+    MAB_REQUIRE(out_dtype == MAB_F32 || out_dtype == MAB_BF16, MAB_ERR_UNSUPPORTED, "mab_int8_matmul: element type %d", out_dtype);
+    MAB_REQUIRE(m < (1 << 30) && n < (1 << 30) && k <= MAB_MAX_INNER && ceil_div64(m, 16) * ceil_div64(n, 128) < (1 << 28), MAB_ERR_LIMIT,
+                "mab_int8_matmul: m=%lld, n=%lld, k=%lld (at most %d)", (long long)m, (long long)n, (long long)k, MAB_MAX_INNER);
+    if (m == 0 || n == 0) return MAB_OK;
+    MAB_REQUIRE(a && b && a_scales && b_scales && out, MAB_ERR_BAD_ARG, "mab_int8_matmul: null pointer");
+    MAB_REQUIRE(a_pitch >= k && b_pitch >= k && out_pitch >= n, MAB_ERR_BAD_ARG, "mab_int8_matmul: rows lie %lld, %lld, %lld apart", (long long)a_pitch,
+                (long long)b_pitch, (long long)out_pitch);
+    MAB_REQUIRE(aligned_to(a, 16) && aligned_to(b, 16) && a_pitch % 16 == 0 && b_pitch % 16 == 0, MAB_ERR_BAD_ARG,
+                "mab_int8_matmul: codes have to start on 16 bytes, their rows a multiple of 16 apart (%lld, %lld)", (long long)a_pitch, (long long)b_pitch);
+    MAB_REQUIRE(aligned_to(a_scales, 4) && aligned_to(b_scales, 4) && aligned_to(bias, 4) && aligned_to(out, out_dtype == MAB_F32 ? 4 : 2),
+                MAB_ERR_BAD_ARG, "mab_int8_matmul: misaligned buffer");
+    int8mm::Args g = {a, b, a_pitch, b_pitch, out_pitch, a_scales, b_scales, bias, out, (int)m, (int)n, (int)k, 1, 1};
+    return out_dtype == MAB_F32 ? int8mm::launch<float>(g, (cudaStream_t)stream) : int8mm::launch<uint16_t>(g, (cudaStream_t)stream);
+}

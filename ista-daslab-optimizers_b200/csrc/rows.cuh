@@ -1,0 +1,121 @@
+// Rows of a dense matrix (logits, activations) read 16 bytes a lane, wherever a row starts, and what the kernels that take a cluster
+// of CTAs per row share.
+#pragma once
+#include "common.cuh"
+#include "fused.cuh"
+
+namespace mab {
+
+// A row of n values as a grid of 16-byte vectors: vector v holds the elements [v N - lead, v N - lead + N).  The first and the last one
+// can be partial; no load reaches outside the row.
+template <typename T> struct RowGrid {
+    static constexpr int N = 16 / (int)sizeof(T);
+    const T* p;
+    int n, lead, count;                      // elements, elements of vector 0 before the row, vectors
+    __device__ __forceinline__ RowGrid(const T* row, int elements) : p(row), n(elements) {
+        lead = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+        count = (elements + lead + N - 1) / N;
+    }
+    __device__ __forceinline__ int first(int v) const { return v * N - lead; }
+    __device__ __forceinline__ bool whole(int v) const { return first(v) >= 0 && first(v) + N <= n; }
+    // the whole vectors among [v0, v1)
+    __device__ __forceinline__ int whole_from(int v0) const { return v0 == 0 && lead ? 1 : v0; }
+    __device__ __forceinline__ int whole_to(int v1) const { return v1 == count && (n + lead) % N ? v1 - 1 : v1; }
+    __device__ __forceinline__ uint4 load(int v) const { return *reinterpret_cast<const uint4*>(p + first(v)); }
+    // a partial vector, by elements; what lies outside the row reads as `none`
+    __device__ __forceinline__ void load_part(int v, float (&x)[N], float none) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int e = first(v) + i;
+            x[i] = e >= 0 && e < n ? Elem<T>::load(p, e) : none;
+        }
+    }
+};
+
+__device__ __forceinline__ void unpack(uint4 r, float (&x)[4], const float*) {
+    x[0] = __uint_as_float(r.x); x[1] = __uint_as_float(r.y); x[2] = __uint_as_float(r.z); x[3] = __uint_as_float(r.w);
+}
+__device__ __forceinline__ void unpack(uint4 r, float (&x)[8], const uint16_t*) {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u); }
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ uint4 pack(const float (&x)[4], const float*) {
+    return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+}
+__device__ __forceinline__ uint4 pack(const float (&x)[8], const uint16_t*) {
+    return make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// The value next below that of an order key (ord_key); the two zeros have one key, that of +0.
+__device__ __forceinline__ float below_key(uint32_t key) { return ord_value(key == 0x80000000u ? 0x7FFFFFFEu : key - 1u); }
+
+constexpr float INF_F = __builtin_huge_valf();
+constexpr uint32_t KEY_NEG_INF = 0x007FFFFFu;       // ord_key(-inf); every number lies above it
+// Order key of a value with NaN (0) below -inf and one key for the two zeros.
+__device__ __forceinline__ uint32_t row_key(float x) { return x == x ? ord_key(x + 0.0f) : 0u; }
+
+// ----------------------------------------------------------------------------- clusters of CTAs, one per row
+__device__ __forceinline__ void cluster_arrive_wait() {
+    asm volatile("barrier.cluster.arrive;\n\tbarrier.cluster.wait;" ::: "memory");
+}
+// Address of `p` (in this CTA's shared memory) in that of CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t cluster_addr(const void* p, int rank) {
+    uint32_t a;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ double cluster_load_f64(const double* p, int rank) {
+    double v;
+    asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(cluster_addr(p, rank)) : "memory");
+    return v;
+}
+__device__ __forceinline__ float cluster_load_f32(const float* p, int rank) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr(p, rank)) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t cluster_load_u32(const void* p, int rank) {
+    uint32_t v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(cluster_addr(p, rank)) : "memory");
+    return v;
+}
+__device__ __forceinline__ unsigned long long cluster_load_u64(const void* p, int rank) {
+    unsigned long long v;
+    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(cluster_addr(p, rank)) : "memory");
+    return v;
+}
+
+// Launches `kernel` with clusters of `cluster` CTAs (1: without) and counts it.
+template <typename... P, typename... A>
+static int launch_rows(void (*kernel)(P...), const char* what, int64_t ctas, int threads, size_t smem, int cluster, cudaStream_t s, A... args) {
+    if (smem > 48 * 1024) MAB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)ctas);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 1 : 0;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+    if (e != cudaSuccess) return cuda_fail(e, what);
+    count_launch();
+    return MAB_OK;
+}
+
+}  // namespace mab

@@ -21,6 +21,7 @@ MAB_F32, MAB_BF16 = 0, 1
 MAB_K2D, MAB_D2K = 0, 1
 MAB_MAX_WINDOW = 128
 MAB_STATIC_MAX_TENSORS = 1024
+MAB_MAX_LIST, MAB_MAX_VOCAB, MAB_MAX_INNER = 1024, 1 << 20, 131071
 MAB_PROBE_NORM_G, MAB_PROBE_NORM_U, MAB_PROBE_NORM_E, MAB_PROBE_ZEROS_U, MAB_PROBE_NORM_QE, MAB_PROBE_ZEROS_QE = range(6)
 MAB_PROBE_SLOTS = 8
 
@@ -77,6 +78,16 @@ SIGNATURES = {
     'mab_quant_stats': (c_int, [c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_void_p]),
     'mab_sparse_rows_dot': (c_int, [c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p]),
     'mab_sparse_rows_combine': (c_int, [c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p]),
+    'mab_quantize_rows': (c_int, [c_int64, c_int64, c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p, c_void_p]),
+    'mab_int8_matmul': (c_int, [c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
+                                c_int64, c_void_p]),
+    'mab_topk_logits': (c_int, [c_int64, c_int64, c_int64, c_void_p, c_int, c_int64, c_double, c_void_p, c_void_p, c_void_p, c_void_p]),
+    'mab_distill_loss': (c_int, [c_int64, c_int64, c_int64, c_void_p, c_int, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_double,
+                                 c_void_p, c_void_p, c_void_p, c_void_p]),
+    'mab_distill_grad': (c_int, [c_int64, c_int64, c_int64, c_void_p, c_int, c_int64, c_void_p, c_void_p, c_double, c_void_p, c_void_p, c_void_p,
+                                 c_int64, c_void_p, c_int64, c_void_p]),
+    'mab_distill_step': (c_int, [c_int64, c_int64, c_int64, c_void_p, c_int, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_double,
+                                 c_void_p, c_void_p, c_int64, c_void_p]),
     'mab_fused_step_workspace_bytes': (c_int64, [c_int]),
     'mab_fused_step_workspace_bytes_for': (c_int64, [POINTER(MabTensor), c_int, POINTER(MabStepArgs)]),
     'mab_fused_supported': (c_int, [POINTER(MabTensor), POINTER(MabStepArgs)]),

@@ -1,0 +1,422 @@
+"""The distillation operators against plain forms in 64 bits (distill_cases.py, which derives the tolerances): types, odd sizes, offsets, distances of
+rows, masks, ties, infinities and NaN, and a run of them together in front of the optimizer's step."""
+import math
+
+import pytest
+import torch
+
+import distill_cases as D
+
+pytestmark = pytest.mark.gpu
+F32, BF16 = torch.float32, torch.bfloat16
+INF = math.inf
+
+
+def _gen(seed):
+    return torch.Generator('cuda').manual_seed(seed)
+
+
+def _normal(gen, *shape, scale=1.0):
+    return torch.randn(*shape, generator=gen, device='cuda') * scale
+
+
+def _placed(x, dtype, skip=0, gap=0):
+    """x in rows `gap` further apart than they are long, starting `skip` elements into a buffer; what lies between is NaN (or 77)."""
+    rows, cols = x.shape
+    buf = torch.full((skip + rows * (cols + gap) + 16,), 77 if dtype == torch.int8 else math.nan, dtype=dtype, device='cuda')
+    out = buf[skip:skip + rows * (cols + gap)].view(rows, cols + gap)[:, :cols]
+    out.copy_(x)
+    return out
+
+
+# ------------------------------------------------------------------------------------------------ quantize_rows
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('rows,cols,skip,gap', [(1, 1, 0, 0), (3, 5, 1, 0), (1, 4096, 0, 0), (7, 257, 3, 2), (130, 64, 0, 8), (5, 767, 0, 0), (33, 8191, 0, 0),
+                                                (2, 16384, 0, 0), (2, 40001, 1, 3), (3, 70000, 0, 0)])
+def test_quantize_rows(dtype, rows, cols, skip, gap):
+    from ista_daslab_optimizers_b200 import quantize_rows
+    g = _gen(rows * 1000 + cols)
+    x = _normal(g, rows, cols) * (0.01 + 100 * torch.rand(rows, 1, generator=g, device='cuda'))
+    x = _placed(x.to(dtype), dtype, skip, gap)
+    codes, scales = quantize_rows(x)
+    want, want_scales = D.quantize(x)
+    assert torch.equal(scales, want_scales)
+    assert torch.equal(codes, want)
+    assert codes.stride(0) % 16 == 0 or rows == 1
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+def test_quantize_rows_values_next_to_a_half(dtype):
+    """Rows whose scale is a power of two times 1 or an odd mantissa, with every half-integer multiple of it and its neighbours."""
+    from ista_daslab_optimizers_b200 import quantize_rows
+    rows = []
+    for s in (1.0, 2.0 ** -20, 0.7, 1.9999999, 3.0e-38, 1.1754944e-38, 1e36, 0.33333334):
+        s = torch.tensor(s, dtype=F32)
+        half = (torch.arange(-127, 127).float() + 0.5) * s
+        near = torch.cat([half, torch.nextafter(half, half * 2), torch.nextafter(half, half * 0), torch.arange(-126, 127).float() * s])
+        near = near.clamp(-127 * s, 127 * s)
+        rows.append(torch.cat([127 * s[None], near]))
+    x = torch.stack(rows).cuda().to(dtype)
+    x = torch.cat([x, torch.zeros_like(x[:1]), torch.full_like(x[:1], 1e-40)])
+    codes, scales = quantize_rows(x)
+    want, want_scales = D.quantize(x)
+    assert torch.equal(scales, want_scales)
+    assert torch.equal(codes, want)
+
+
+def test_quantize_rows_non_finite_and_given_outputs():
+    from ista_daslab_optimizers_b200 import quantize_rows
+    x = _normal(_gen(5), 6, 300)
+    x[1, 7], x[2, 299], x[3, 0], x[4, :] = INF, math.nan, -INF, 0.0
+    buf = torch.full((8, 304), 55, dtype=torch.int8, device='cuda')
+    scales = torch.full((8,), 5.0, device='cuda')
+    quantize_rows(x, buf[1:7, 2:302], scales[1:7])
+    want, want_scales = D.quantize(x)
+    assert torch.equal(scales[1:7].nan_to_num(9.0), want_scales.nan_to_num(9.0)) and torch.equal(buf[1:7, 2:302], want)
+    assert (buf[0] == 55).all() and (buf[7] == 55).all() and (buf[:, :2] == 55).all() and (buf[:, 302:] == 55).all()
+    assert scales[0] == 5.0 and scales[7] == 5.0
+
+
+# ------------------------------------------------------------------------------------------------ int8_matmul
+
+def _codes(g, rows, cols, extreme=False):
+    c = torch.zeros(rows, (cols + 15) // 16 * 16, dtype=torch.int8, device='cuda')[:, :cols]
+    c.copy_(torch.full((rows, cols), -128, device='cuda') if extreme else torch.randint(-128, 128, (rows, cols), generator=g, device='cuda'))
+    return c
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('m,n,k,bias', [
+    (1, 1, 1, False), (1, 130, 16, True), (2, 77, 767, False), (3, 1000, 129, True), (4, 4096, 4096, False), (5, 128, 128, True), (5, 130, 100, False),
+    (16, 300, 1000, False), (17, 129, 31, True), (31, 1024, 4096, False), (41, 257, 2049, True), (64, 128, 8192, False), (65, 300, 640, True),
+    (128, 256, 255, False), (129, 511, 513, True), (256, 384, 1024, False), (257, 1025, 767, True), (300, 2048, 512, False), (777, 515, 129, False)])
+def test_int8_matmul(dtype, m, n, k, bias):
+    from ista_daslab_optimizers_b200 import int8_matmul
+    g = _gen(m * 7 + n * 3 + k)
+    a, b = _codes(g, m, k), _codes(g, n, k)
+    sa, sb = torch.rand(m, generator=g, device='cuda') + 0.01, torch.rand(n, generator=g, device='cuda') * 0.01
+    bs = _normal(g, n, scale=50.0) if bias else None
+    buf = torch.full((m + 2, n + 3), 7.0, dtype=dtype, device='cuda')
+    out = int8_matmul(a, b, sa, sb, bs, out=buf[1:m + 1, 1:n + 1])
+    want, tol = D.matmul(a, b, sa, sb, bs)
+    D.assert_near(out, want, tol + (0 if dtype == F32 else D.half_step(dtype) * want.abs()), 'product')
+    assert (buf[0] == 7).all() and (buf[m + 1] == 7).all() and (buf[:, 0] == 7).all() and (buf[:, n + 1:] == 7).all()
+    assert torch.equal(int8_matmul(a, b, sa, sb, bs, dtype=dtype), out)
+
+
+@pytest.mark.parametrize('m', [1, 7, 200])
+def test_int8_matmul_longest_sum_and_special_scales(m):
+    from ista_daslab_optimizers_b200 import int8_matmul, _native as N
+    k = N.MAB_MAX_INNER
+    a, b = _codes(None, m, k, extreme=True), _codes(None, 150, k, extreme=True)
+    sa, sb = torch.ones(m, device='cuda'), torch.ones(150, device='cuda')
+    sb[3], sb[4] = math.nan, 0.0
+    out = int8_matmul(a, b, sa, sb, dtype=F32)
+    want = torch.full((m, 150), float(k * 16384), device='cuda')
+    want[:, 4] = 0.0
+    assert out[:, 3].isnan().all()
+    keep = [i for i in range(150) if i != 3]
+    assert torch.equal(out[:, keep], want[:, keep])          # 131071 * 2^14 is exact in fp32
+
+
+# ------------------------------------------------------------------------------------------------ topk_logits
+
+def _check_topk(z, k, tau):
+    from ista_daslab_optimizers_b200 import topk_logits
+    values, indices, rest = topk_logits(z, k, tau)
+    w_values, w_indices, w_rest = D.topk(z, k, tau)
+    assert torch.equal(indices, w_indices)
+    assert torch.equal(values.nan_to_num(123.0), w_values.nan_to_num(123.0)) and torch.equal(values.isnan(), w_values.isnan())
+    assert values.dtype == z.dtype
+    D.assert_near(rest, w_rest, D.sum_error(z.shape[1]) + 2 * D.U * w_rest.abs().nan_to_num(0.0, posinf=0.0, neginf=0.0), 'rest')
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('rows,vocab,k,tau,skip,gap', [
+    (1, 1, 1, 1.0, 0, 0), (3, 2, 1, 1.0, 1, 0), (2, 7, 7, 2.0, 1, 2), (4, 1000, 1, 0.7, 0, 0), (5, 50257, 20, 1.0, 0, 0), (3, 50257, 257, 2.0, 1, 6),
+    (1, 128256, 64, 1.0, 0, 0), (2, 151936, 1000, 1.0, 3, 0), (150, 4097, 33, 1.0, 0, 0), (300, 2048, 1024, 1.0, 0, 0), (300, 30000, 512, 1.3, 1, 1),
+    (160, 128256, 64, 2.0, 0, 0), (2, 1 << 20, 1024, 1.0, 0, 0), (200, 1024, 1024, 1.0, 0, 0), (149, 16384, 100, 1.0, 0, 0), (149, 16391, 1024, 1.0, 5, 0)])
+def test_topk_logits(dtype, rows, vocab, k, tau, skip, gap):
+    g = _gen(rows + vocab + k)
+    z = _normal(g, rows, vocab, scale=3.0)
+    _check_topk(_placed(z.to(dtype), dtype, skip, gap), k, tau)
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('rows', [2, 301])
+@pytest.mark.parametrize('kind', ['equal', 'zeros', 'two', 'ascending', 'descending', 'late', 'masked', 'lowest', 'few', 'none', 'inf', 'many_inf', 'nan',
+                                  'all_nan', 'gap', 'large', 'blocks'])
+def test_topk_logits_kinds(dtype, rows, kind):
+    vocab, k = 40001, 65
+    g = _gen(rows)
+    z = _normal(g, rows, vocab, scale=2.0)
+    low = torch.finfo(dtype).min
+    if kind == 'equal':
+        z[:] = 1.5
+    elif kind == 'zeros':
+        z = torch.where(z > 0, 0.0, -0.0)
+    elif kind == 'two':
+        z = torch.where(z > 2.0, 1.0, 0.5)
+    elif kind == 'ascending':
+        z = torch.arange(vocab, device='cuda').float().div(64.0).expand(rows, vocab).clone()
+    elif kind == 'descending':
+        z = torch.arange(vocab, 0, -1, device='cuda').float().div(64.0).expand(rows, vocab).clone()
+    elif kind == 'late':                             # the first half is masked
+        z[:, :vocab // 2] = -1e4
+    elif kind == 'masked':
+        z[torch.rand(rows, vocab, generator=g, device='cuda') < 0.7] = -INF
+    elif kind == 'lowest':                           # fewer numbers than k, the rest the type's lowest
+        z[:, 40:] = low
+    elif kind == 'few':
+        z[:, 40:] = -INF
+    elif kind == 'none':
+        z[:] = -INF
+    elif kind == 'inf':
+        z[:, 17::5000] = INF
+    elif kind == 'many_inf':
+        z[:, 17::100] = INF
+    elif kind == 'nan':
+        z[0, 5::1000] = math.nan
+        z[-1, 39000] = math.nan
+    elif kind == 'all_nan':
+        z[:, 30:] = math.nan
+    elif kind == 'gap':                              # the rest is far below the list
+        z[:, 500::600] += 400.0
+        z[:, 500 + 600 * k:] = -7.0
+    elif kind == 'large':
+        z *= 1e30
+    elif kind == 'blocks':                           # one value per stretch, rising late
+        z = (torch.arange(vocab, device='cuda') // 9000).float().expand(rows, vocab).clone()
+    _check_topk(z.to(dtype), k, 1.0)
+
+
+# ------------------------------------------------------------------------------------------------ distillation
+
+def _problem(rows, vocab, k, dtype, v_dtype, tau, rest, masked, ragged, skip=0, gap=0, seed=0):
+    g = _gen(seed + rows + vocab + k)
+    teacher = _normal(g, rows, vocab, scale=2.0)
+    z = _placed((teacher * 0.7 + _normal(g, rows, vocab)).to(dtype), dtype, skip, gap)
+    val, idx = torch.topk(teacher, k)
+    idx = idx.int()
+    r = torch.logsumexp(teacher.scatter(1, idx.long(), -INF) / tau, 1) if rest else None
+    if ragged:
+        idx[torch.rand(rows, k, generator=g, device='cuda') < 0.4] = -1
+    w = None
+    if masked:
+        w = torch.rand(rows, generator=g, device='cuda') * 3 - 1
+        w[::3] = 0.0
+    return z, idx, val.to(v_dtype), r, w
+
+
+def _check_distill(z, idx, val, rest, w, tau, what=''):
+    from ista_daslab_optimizers_b200 import distill_loss, distill_step
+    want = D.distill(z, idx, val, rest, w, tau)
+    loss, grad = distill_step(z, idx, val, rest, w, tau)
+    D.assert_distill(loss, grad, want, z.shape[1], 'step ' + what)
+    leaf = z.detach().clone().requires_grad_() if z.is_contiguous() else z.detach().requires_grad_()
+    out = distill_loss(leaf, idx, val, rest, w, tau)
+    g, = torch.autograd.grad(out.sum(), leaf)
+    D.assert_distill(out.detach(), g, want, z.shape[1], 'loss ' + what)
+    z.requires_grad_(False)
+    return loss, grad
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('rows,vocab,k,v_dtype,tau,rest,masked,ragged,skip,gap', [
+    (1, 1, 1, F32, 1.0, False, False, False, 0, 0), (2, 2, 1, F32, 1.0, True, False, False, 1, 0), (3, 9, 9, BF16, 2.0, False, False, False, 1, 3),
+    (4, 1000, 5, F32, 0.7, True, True, False, 0, 0), (60, 50257, 32, F32, 1.0, False, False, True, 0, 0), (5, 50257, 257, BF16, 1.5, True, False, False, 1, 6),
+    (1, 128256, 64, F32, 2.0, True, False, False, 0, 0), (2, 151936, 1000, F32, 1.0, True, False, True, 3, 0), (150, 4097, 33, BF16, 1.0, True, True, True, 0, 0),
+    (300, 2048, 1024, F32, 1.0, True, False, False, 0, 0), (300, 30001, 512, F32, 1.3, False, True, True, 1, 1), (2, 1 << 20, 1024, F32, 1.0, True, False, False, 0, 0),
+    (310, 5003, 7, F32, 4.0, True, True, False, 0, 5)])
+def test_distill(dtype, rows, vocab, k, v_dtype, tau, rest, masked, ragged, skip, gap):
+    _check_distill(*_problem(rows, vocab, k, dtype, v_dtype, tau, rest, masked, ragged, skip, gap), tau)
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('rows', [3, 320])
+def test_distill_masks_and_indices(dtype, rows):
+    """Entries that are absent, out of range, repeated; a row without a teacher; vocabularies masked by -inf and by the type's lowest value."""
+    vocab, k, tau = 20011, 40, 1.0
+    z, idx, val, rest, _ = _problem(rows, vocab, k, dtype, F32, tau, True, False, False)
+    idx[0] = -1
+    idx[1, 3:] = vocab
+    idx[1, 7], idx[1, 8] = 2 ** 31 - 1, -2 ** 31
+    _check_distill(z, idx, val, rest, None, tau, 'absent')
+    idx[2, 10:30] = idx[2, 5].item()
+    idx[2, 39] = idx[2, 0].item()
+    _check_distill(z, idx, val, rest, None, tau, 'repeated')
+    loss, grad = _check_distill(z, idx, val, None, None, tau, 'no rest')
+    assert loss[0] == 0 and (grad[0] == 0).all()
+    r2 = rest.clone()
+    r2[0] = -INF                                     # neither entries nor a rest
+    loss, grad = _check_distill(z, idx, val, r2, None, tau, 'no teacher')
+    assert loss[0] == 0 and (grad[0] == 0).all()
+    for low in (-INF, torch.finfo(dtype).min):
+        y = z.clone()
+        y[:, vocab - 100:] = low
+        keep = idx.clone()
+        keep[keep >= vocab - 100] = -1
+        _check_distill(y, keep, val, rest, None, tau, f'columns {low}')
+        y[:] = low                                   # only the list is left
+        y.scatter_(1, keep.clamp(0, vocab - 1).long(), 1.0)
+        _check_distill(y, keep, val, None, None, tau, f'list only {low}')
+    v2 = val.clone()
+    v2[:, 20:] = -INF                                # listed, with nothing
+    _check_distill(z, idx, v2, rest, None, tau, 'empty entries')
+
+
+def test_distill_skipped_rows_are_not_looked_at():
+    from ista_daslab_optimizers_b200 import distill_loss, distill_step
+    z, idx, val, rest, w = _problem(9, 3001, 8, F32, F32, 1.0, True, True, False)
+    z[::3] = math.nan
+    loss, grad = distill_step(z, idx, val, rest, w)
+    assert (loss[::3] == 0).all() and (grad[::3] == 0).all() and torch.isfinite(loss).all() and torch.isfinite(grad).all()
+    leaf = z.clone().requires_grad_()
+    out = distill_loss(leaf, idx, val, rest, w)
+    out.backward(torch.full_like(out, INF).where(w == 0, torch.ones_like(out)))
+    assert (leaf.grad[::3] == 0).all() and torch.isfinite(leaf.grad).all()
+    bad, bad_grad = distill_step(z, idx, val, rest, None)
+    assert bad[::3].isnan().all() and bad_grad[::3].isnan().all() and torch.isfinite(bad[1::3]).all()
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('skip,gap', [(0, 0), (1, 3)])
+def test_distill_step_in_place_and_elsewhere(dtype, skip, gap):
+    from ista_daslab_optimizers_b200 import distill_step
+    z, idx, val, rest, w = _problem(20, 9001, 50, dtype, F32, 1.0, True, True, True, skip, gap)
+    loss, grad = distill_step(z, idx, val, rest, w)
+    other = _placed(torch.zeros_like(z), dtype, 2, 5)      # another offset than the logits'
+    loss2, g2 = distill_step(z, idx, val, rest, w, grad=other)
+    assert g2.data_ptr() == other.data_ptr() and torch.equal(g2, grad) and torch.equal(loss, loss2)
+    loss3, g3 = distill_step(z, idx, val, rest, w, grad=z)
+    assert torch.equal(z, grad) and torch.equal(loss3, loss)
+    gaps = z.as_strided((20, 9001 + gap), (9001 + gap, 1), z.storage_offset())[:, 9001:]
+    assert gap == 0 or gaps.isnan().all()
+
+
+def test_distill_gradient_against_differences():
+    """Central differences of the loss kernel itself: f(z + h) - f(z - h) = 2 h f' + O(h^3 f'''), with |f'''| <= 2 / tau^3 for a mixture of log-sum-exps, and the
+    loss's own error on both sides."""
+    from ista_daslab_optimizers_b200 import distill_loss
+    tau, vocab, k, h = 1.5, 200, 10, 0.05
+    z, idx, val, rest, _ = _problem(1, vocab, k, F32, F32, tau, True, False, False)
+    leaf = z.clone().requires_grad_()
+    grad, = torch.autograd.grad(distill_loss(leaf, idx, val, rest, None, tau).sum(), leaf)
+    step = h * torch.eye(vocab, device='cuda')
+    rows = lambda t: t.expand(vocab, *t.shape[1:]).contiguous()      # noqa: E731
+    up, down = z + step, z - step
+    wide = (up.diagonal() - down.diagonal()).double()
+    f = [distill_loss(x, rows(idx), rows(val), rows(rest), None, tau).double() for x in (up, down)]
+    slope = (f[0] - f[1]) / wide
+    tol = h * h / 6 * 2 / tau ** 3 + 2 * (D.sum_error(vocab) + 2 * D.U * 5) / (2 * h)
+    D.assert_near(grad[0], slope, tol, 'slope')
+
+
+def test_distill_broadcast_upstream_gradient():
+    from ista_daslab_optimizers_b200 import distill_loss
+    z, idx, val, rest, _ = _problem(6, 3000, 16, F32, F32, 1.0, True, False, False)
+    leaf = z.clone().requires_grad_()
+    g = torch.autograd.grad(distill_loss(leaf, idx, val, rest).mean(), leaf)[0]          # a gradient of distance 0
+    up = torch.arange(12, device='cuda').float()
+    every, = torch.autograd.grad(distill_loss(leaf, idx, val, rest), leaf, up[::2])       # ... and of distance 2
+    one = D.distill(z, idx, val, rest, None, 1.0)
+    tol = (D.sum_error(3000) + 72 * D.U) * one[2] + 2 * D.U * one[1].abs() + 2.0 ** -126
+    D.assert_near(g, one[1] / 6, tol / 6, 'mean')
+    D.assert_near(every, one[1] * up[::2, None].double(), tol * up[::2, None], 'rows')
+
+
+def test_distill_saved_logits_cannot_change_unnoticed():
+    from ista_daslab_optimizers_b200 import distill_loss
+    z, idx, val, rest, _ = _problem(2, 500, 4, F32, F32, 1.0, True, False, False)
+    leaf = z.clone().requires_grad_()
+    y = leaf * 1.0
+    loss = distill_loss(y, idx, val, rest)
+    y.detach().mul_(2.0)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        loss.sum().backward()
+
+
+# ------------------------------------------------------------------------------------------------ together
+
+def test_teacher_to_optimizer_step():
+    """A frozen linear teacher in 8 bits, its top logits, the student's loss and gradient, the optimizer's step: each against the 64-bit form on the inputs
+    it had, and the same step by autograd."""
+    from ista_daslab_optimizers_b200 import MicroAdam, distill_loss, distill_step, int8_matmul, quantize_rows, topk_logits
+    g = _gen(1)
+    tokens, width, vocab, k, tau = 130, 256, 5003, 16, 2.0
+    hidden = _normal(g, tokens, width).to(BF16)
+    codes, scales = quantize_rows(_normal(g, vocab, width, scale=0.2).to(BF16))
+    x, x_scales = quantize_rows(hidden)
+    teacher = int8_matmul(x, codes, x_scales, scales)
+    want, tol = D.matmul(x, codes, x_scales, scales, None)
+    D.assert_near(teacher, want, tol + D.half_step(BF16) * want.abs(), 'teacher')
+    values, indices, rest = topk_logits(teacher, k, tau)
+    assert torch.equal(indices, D.topk(teacher, k, tau)[1])
+    steps = []
+    for by_autograd in (False, True):
+        weight = torch.nn.Parameter(_normal(_gen(2), vocab, width, scale=0.1).to(BF16))
+        opt = MicroAdam([weight], m=4, lr=1e-3, quant_block_size=64)
+        for _ in range(2):
+            student = hidden @ weight.T
+            if by_autograd:
+                distill_loss(student, indices, values, rest, None, tau).sum().backward()
+            else:
+                loss, grad = distill_step(student.detach(), indices, values, rest, None, tau)
+                D.assert_distill(loss, grad, D.distill(student.detach(), indices, values, rest, None, tau), vocab, 'student')
+                student.backward(grad)
+            opt.step()
+            opt.zero_grad()
+        assert torch.isfinite(weight).all()
+        steps.append(weight.detach().clone())
+    assert (steps[0].float() - steps[1].float()).abs().max() < 4e-3     # two steps of lr 1e-3 each differ by at most twice as much
+    assert not torch.equal(steps[0], _normal(_gen(2), vocab, width, scale=0.1).to(BF16))
+
+
+def test_captured_and_replayed_with_other_streams():
+    """The chain captured into a graph and replayed on new inputs gives what eager calls on another stream give, bit for bit."""
+    from ista_daslab_optimizers_b200 import distill_step, int8_matmul, quantize_rows, topk_logits, _native as N
+    g = _gen(3)
+    codes, scales = quantize_rows(_normal(g, 3001, 512, scale=0.2))
+    hidden, student = _normal(g, 70, 512).to(BF16), _normal(g, 70, 3001).to(BF16)
+
+    def chain(h, s):
+        x, xs = quantize_rows(h)
+        t = int8_matmul(x, codes, xs, scales)
+        v, i, r = topk_logits(t, 20)
+        return (t, v, i, r) + distill_step(s, i, v, r)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        chain(hidden, student)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = chain(hidden, student)
+    for seed in (4, 5):
+        h, s = _normal(_gen(seed), 70, 512).to(BF16), _normal(_gen(seed + 10), 70, 3001).to(BF16)
+        hidden.copy_(h)
+        student.copy_(s)
+        graph.replay()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            eager = chain(h, s)
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        for a, b in zip(out, eager):
+            assert torch.equal(a, b)
+    assert N.device_error() == 0
+
+
+def test_repeated_calls_give_the_same_bits():
+    from ista_daslab_optimizers_b200 import distill_step, topk_logits
+    for rows in (3, 400):
+        z, idx, val, rest, w = _problem(rows, 30011, 100, BF16, F32, 1.0, True, True, True)
+        first = distill_step(z, idx, val, rest, w) + topk_logits(z, 100)
+        for _ in range(5):
+            again = distill_step(z, idx, val, rest, w) + topk_logits(z, 100)
+            for i, (a, b) in enumerate(zip(first, again)):
+                if i != 4:                           # (`rest` sums what candidates leave in the order in which they came: to its tolerance)
+                    assert torch.equal(a, b)
+            D.assert_near(again[4], first[4], 2 * D.sum_error(30011), 'rest')
