@@ -52,6 +52,43 @@ __device__ __forceinline__ uint4 pack(const float (&x)[8], const uint16_t*) {
     return make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
 }
 
+// Pairs of floats in 64 bits, for the packed instructions.
+__device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void split(uint64_t p, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(p)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ void unpack_pairs(uint4 r, uint64_t (&x)[2], const float*) {
+    x[0] = (uint64_t)r.y << 32 | r.x; x[1] = (uint64_t)r.w << 32 | r.z;
+}
+__device__ __forceinline__ void unpack_pairs(uint4 r, uint64_t (&x)[4], const uint16_t*) {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = (uint64_t)(w[i] & 0xFFFF0000u) << 32 | (uint64_t)(w[i] << 16);
+}
+// Largest of a vector's values that are not NaN (NaN where there is none).
+__device__ __forceinline__ float vector_max(uint4 r, const float*) {
+    return fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)), fmaxf(__uint_as_float(r.z), __uint_as_float(r.w)));
+}
+__device__ __forceinline__ float vector_max(uint4 r, const uint16_t*) {
+    uint32_t a, b;
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(r.x), "r"(r.y));
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(b) : "r"(r.z), "r"(r.w));
+    asm("max.bf16x2 %0, %0, %1;" : "+r"(a) : "r"(b));
+    return fmaxf(__uint_as_float(a << 16), __uint_as_float(a & 0xFFFF0000u));
+}
+
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

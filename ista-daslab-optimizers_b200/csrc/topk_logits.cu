@@ -1,10 +1,10 @@
 // The k largest logits of every row, in descending order (ties: the lower index first), and rest = log sum exp(z / tau) over all others.
 //
-// One pass over the row.  The first chunk gives a bound: the k-th largest of its vectors' maxima, which at least k values reach.  From then on
-// a value above the bound becomes a candidate in shared memory (some k ln(row / chunk) of a row do), every other one goes into the sum at once,
-// relative to the bound, so the sum over the rest is its own and not a difference of two large ones.  When the candidates outgrow half of their room, the k
-// largest of them stay, the others go into the sum, and the bound rises to the k-th; a chunk whose candidates do not fit (ascending rows, a
-// chunk of one value) is selected from exactly, in registers.  At the end every candidate counts those before it, which is its place.
+// One pass over the row.  A sample (the maxima of vectors spread over the row) gives a bound that at least k values reach: the k-th largest of the maxima.  Then the row
+// streams by: a value above the bound becomes a candidate in shared memory, every other one goes into the sum at once, relative to the bound, so the
+// sum over the rest is its own and not a difference of two large ones.  Of the candidates the k-th is found by bisection on their keys; those below it join the
+// sum, the others are put in order.  No barrier and no decision of the block falls into the stream: where more candidates come than there is room for (equal values,
+// a row that is not like its sample), the row is gone through again, chunk by chunk, each selected from exactly in registers.
 //
 // The order is that of 64-bit keys, value above 2^32 - 1 - index: distinct, so "larger" contains the tie rule.  NaN lies below -inf and makes
 // the rest NaN.  A row belongs to a cluster of one to eight CTAs; the first of them merges the candidates of all.
@@ -14,13 +14,14 @@ namespace mab {
 namespace toplogits {
 
 constexpr int NT = 512, WARPS = NT / 32;
-constexpr int UNROLL = 4;                          // vectors a thread holds of a chunk
-constexpr int CAP = 4096;                          // candidates
-constexpr int ROOM = CAP / 2;                      // pruned to k when more are there after a chunk
+constexpr int UNROLL = 4;                          // vectors a thread has in flight
+constexpr int SLOW_UNROLL = 2;                     // vectors a thread holds of a chunk that is selected from exactly
+constexpr int CAP = 3072;                          // candidates
+constexpr int LIST = 3072, REACH = 1536;           // vectors that hold one by the first bound, and by the second
 constexpr int MAX_K = 1024;
 constexpr int ITEMS = CAP / NT;
-constexpr int LAST = MAX_K / NT;                    // candidates a thread has in the end
-static_assert(ROOM + MAX_K <= CAP && 8 * MAX_K / 2 <= CAP, "a chunk's exact selection and a merge have room");
+constexpr int SAMPLE = 16;                         // most vectors a thread samples
+static_assert(2 * MAX_K <= CAP, "what is held and what a chunk adds have room");
 
 struct Args {
     const void* logits;
@@ -30,35 +31,77 @@ struct Args {
     float* rest;
     double tau;
     float scale;
-    int vocab, k, cluster;
+    int vocab, k, cluster, sample;
 };
 
 struct Shared {
     unsigned long long cand[CAP];
+    int list[LIST];                                 // vectors with a value above the bound ...
+    uint32_t list_key[LIST];                        // ... and the keys of their largest
+    int reach[REACH];                               // those that reach the second bound
+    int n_list, n_reach;
     double red[WARPS];
     double sum;                                     // this CTA's sum over the rest, and its reference
     float ref;
-    int n;                                          // candidates (can count beyond CAP while a chunk overflows)
+    int far;
+    int n;                                          // candidates (counts beyond CAP where they do not fit)
     int count[64];                                  // counters of a bisection, one per step
     uint32_t warp_max[WARPS];
     int scan[40];
-    unsigned long long kth;
-};
+    double terms[WARPS];                            // of candidates that go into the rest
+};                                                  //   a sum of integers does not depend on it
 
-// A thread's sum over the rest, relative to exp(ref).
+// Order keys of as many bits as the type has; NaN (0) below -inf, one key for the two zeros.
+template <typename T> struct Key {
+    static constexpr int SHIFT = 32 - 8 * (int)sizeof(T);
+    static constexpr uint32_t NEG_INF = KEY_NEG_INF >> SHIFT, MOST = 0xFFFFFFFFu >> SHIFT;
+    __device__ __forceinline__ static uint32_t of(float x) { return row_key(x) >> SHIFT; }
+    __device__ __forceinline__ static float value(uint32_t key) {
+        return SHIFT ? ord_value(key << SHIFT | (key & 0x8000u ? 0u : 0xFFFFu)) : ord_value(key);
+    }
+    __device__ __forceinline__ static float below(uint32_t key) {              // the next value below; the key under that of +0 is the unused one of -0
+        return value(key == (0x80000000u >> SHIFT) ? key - 2 : key - 1);
+    }
+    __device__ __forceinline__ static float bound(uint32_t key) { return key > NEG_INF ? value(key) : -INF_F; }
+    __device__ __forceinline__ static unsigned long long composite(float x, int e) { return (unsigned long long)of(x) << 32 | (0xFFFFFFFFu - (uint32_t)e); }
+    __device__ __forceinline__ static float value_of(unsigned long long c) { return value((uint32_t)(c >> 32)); }
+};
+__device__ __forceinline__ int index_of(unsigned long long c) { return (int)(0xFFFFFFFFu - (uint32_t)c); }
+
+// A thread's sum over the rest, relative to exp2(ref), ref a reference times `scale`: exp2(x scale - ref) is one operation and the instruction, and the
+// rounding of ref cancels in the end.  `far`: a reference so large was in use that its rounding is no longer small against 1: the sum does not count.
+constexpr float FAR = 1048576.0f;
 struct Rest {
     float s, ref, scale;
-    __device__ __forceinline__ void add(float x) { s += ex2((x - ref) * scale); }
-    __device__ __forceinline__ void move(float to) {                                 // references only rise (from none: 0)
-        if (to == -INF_F) to = 0.0f;
-        if (!(s == 0.0f)) s *= ex2((ref - to) * scale);
+    bool far;
+    __device__ __forceinline__ void add(float x) { s += ex2(fmaf(x, scale, -ref)); }
+    __device__ __forceinline__ void move(float to_value) {
+        const float to = to_value == -INF_F ? 0.0f : fminf(fmaxf(to_value * scale, -3e38f), 3e38f);
+        far |= !(fabsf(to) < FAR);
+        if (!(s == 0.0f)) s *= ex2(ref - to);
         ref = to;
     }
 };
 
-__device__ __forceinline__ unsigned long long composite(float x, int e) { return (unsigned long long)row_key(x) << 32 | (0xFFFFFFFFu - (uint32_t)e); }
-__device__ __forceinline__ int index_of(unsigned long long c) { return (int)(0xFFFFFFFFu - (uint32_t)c); }
-__device__ __forceinline__ float value_of(unsigned long long c) { return ord_value((uint32_t)(c >> 32)); }
+// A candidate's term in the rest, rounded to a multiple of 2^-38: candidates come in any order and to any thread, and doubles on one grid
+// have the same sum in every order (32768 of them, each at most 1 but for a rounding, stay exact).
+__device__ __forceinline__ double grid_term(const Rest& rest, float x) {
+    const double d = (double)ex2(fmaf(x, rest.scale, -rest.ref));
+    return __dadd_rn(__dadd_rn(d, 24576.0), -24576.0);
+}
+// Adds the block's terms to the rest, in the first thread.
+__device__ __forceinline__ void add_terms(double* parts, double mine, Rest& rest) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    if (lane_id() == 0) parts[warp_id()] = mine;
+    __syncthreads();
+    if (warp_id() == 0) {
+        double all = lane_id() < WARPS ? parts[lane_id()] : 0.0;
+#pragma unroll
+        for (int o = WARPS / 2; o; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+        if (lane_id() == 0) rest.s += (float)all;
+    }
+}
 
 // Sum of one int per thread, step `i` of a bisection: counters are cleared by `clear_counts`, each is used once.
 __device__ __forceinline__ int block_count(Shared& sh, int c, int i) {
@@ -73,181 +116,173 @@ __device__ __forceinline__ void clear_counts(Shared& sh) {
     __syncthreads();
 }
 
-// Largest key T with count(>= T) >= k, `counted(mid)` being the calling thread's number of keys >= mid.  Needs count(>= lo) >= k.
-template <typename F> __device__ __forceinline__ uint32_t kth_key(Shared& sh, uint32_t lo, uint32_t hi, int k, F counted) {
+// Largest key T in [lo, hi] with count(>= T) >= k, or any with count(>= T) in [k, most], `counted(mid)` being the calling thread's number of keys >= mid.
+// Needs count(>= lo) >= k, count(> hi) < k.  `reached`: count(>= T).
+template <typename F> __device__ __forceinline__ uint32_t kth_key(Shared& sh, uint32_t lo, uint32_t hi, int k, int most, int& reached, F counted) {
     clear_counts(sh);
-    for (int i = 0; lo < hi; ++i) {                 // invariant: count(>= lo) >= k, count(>= hi + 1) < k
+    reached = 0x7FFFFFFF;
+    for (int i = 0; lo < hi; ++i) {
         const uint32_t mid = lo + (hi - lo) / 2 + 1;
-        if (block_count(sh, counted(mid), i) >= k) lo = mid;
-        else hi = mid - 1;
+        const int c = block_count(sh, counted(mid), i);
+        if (c < k) { hi = mid - 1; continue; }
+        lo = mid;
+        reached = c;
+        if (c <= most) break;
     }
     return lo;
 }
 
-// The k largest of the n > k candidates stay; the others go into the rest.  Returns the k-th key.
-__device__ __noinline__ uint32_t prune(Shared& sh, int k, Rest& rest) {
-    const int t = threadIdx.x, n = sh.n;
-    unsigned long long c[ITEMS];
-#pragma unroll
-    for (int i = 0; i < ITEMS; ++i) c[i] = t + i * NT < n ? sh.cand[t + i * NT] : 0ull;
-    auto there = [&](int i) { return t + i * NT < n; };
-    const uint32_t T = kth_key(sh, 0u, 0xFFFFFFFFu, k, [&](uint32_t mid) {
-        int r = 0;
-#pragma unroll
-        for (int i = 0; i < ITEMS; ++i) r += there(i) && (uint32_t)(c[i] >> 32) >= mid;
-        return r;
-    });
-    clear_counts(sh);
-    int above = 0;
-#pragma unroll
-    for (int i = 0; i < ITEMS; ++i) above += there(i) && (uint32_t)(c[i] >> 32) > T;
-    above = block_count(sh, above, 0);
-    const uint32_t L = kth_key(sh, 0u, 0xFFFFFFFFu, k - above, [&](uint32_t mid) {      // among the equals: the largest low words (lowest indices)
-        int r = 0;
-#pragma unroll
-        for (int i = 0; i < ITEMS; ++i) r += there(i) && (uint32_t)(c[i] >> 32) == T && (uint32_t)c[i] >= mid;
-        return r;
-    });
-    const unsigned long long last = (unsigned long long)T << 32 | L;
-    __syncthreads();
-    if (t == 0) sh.n = 0;
-    __syncthreads();
-    rest.move(T > KEY_NEG_INF ? ord_value(T) : -INF_F);
-#pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-        if (!there(i)) continue;
-        if (c[i] >= last) sh.cand[atomicAdd(&sh.n, 1)] = c[i];
-        else rest.add(value_of(c[i]));
+// The same for one key per thread, from either end: the range is first narrowed in growing steps from where the answer is expected.
+template <typename T, bool FROM_TOP> __device__ __forceinline__ uint32_t kth_of_threads(bool there, uint32_t mine, uint32_t lo, uint32_t hi, int k, int most) {
+    uint32_t step = 128u << (16 - Key<T>::SHIFT);                  // an octave
+    bool narrowing = true;
+    while (lo < hi) {
+        uint32_t mid = lo + (hi - lo) / 2 + 1;
+        if (narrowing && (hi - lo) / 2 > step) mid = FROM_TOP ? hi - step : lo + step;
+        else narrowing = false;
+        step *= 2;
+        const int r = __syncthreads_count(there && mine >= mid);
+        if (r < k) { hi = mid - 1; narrowing &= FROM_TOP; continue; }
+        lo = mid;
+        narrowing &= !FROM_TOP;
+        if (r <= most) break;
     }
-    __syncthreads();
-    return T;
+    return lo;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(NT, 2) topk_logits_kernel(Args a) {
-    constexpr int N = RowGrid<T>::N;
-    extern __shared__ __align__(16) unsigned char dyn[];
-    Shared& sh = *reinterpret_cast<Shared*>(dyn);
-    const int C = a.cluster, rank = C > 1 ? (int)(blockIdx.x % C) : 0, t = threadIdx.x, k = a.k;
-    const int64_t row = blockIdx.x / C;
-    const RowGrid<T> g(reinterpret_cast<const T*>(a.logits) + row * a.pitch, a.vocab);
-    const int per = (g.count + C - 1) / C, v0 = min(rank * per, g.count), v1 = min(v0 + per, g.count);
+// The key of the k-th largest of n >= k keys, or one between that and the (k + slack)-th; all lie in [lo, hi], n <= LIST.
+template <typename T> __device__ __noinline__ uint32_t kth_of_list(Shared& sh, int n, int k, int slack, uint32_t lo, uint32_t hi) {
+    const int t = threadIdx.x;
+    if (n <= NT) return kth_of_threads<T, false>(t < n, t < n ? sh.list_key[t] : 0u, lo, hi, k, k + slack);
+    int reached;
+    return kth_key(sh, lo, hi, k, k + slack, reached, [&](uint32_t mid) {
+        int r = 0;
+        for (int i = t; i < n; i += NT) r += sh.list_key[i] >= mid;
+        return r;
+    });
+}
+
+// A key that at least k values of the whole vectors [w0, w1) reach, near the k-th largest: of the maxima of vectors spread evenly over them.
+// NEG_INF where there are not enough.
+template <typename T> __device__ __noinline__ uint32_t bound_of_sample(Shared& sh, const RowGrid<T>& g, int w0, int w1, int k, int sample) {
+    using K = Key<T>;
+    const int every = (max(w1 - w0, 0) + 31) / 32, groups = min(sample * WARPS, every), apart = groups ? every / groups * 32 : 0;
+    auto maximum = [&](int u) {                     // of the u-th vector of this thread
+        const int j = u * WARPS + warp_id(), v = w0 + j * apart + lane_id();
+        return u < sample && j < groups && v < w1 ? vector_max(g.load(v), (const T*)nullptr) : -INF_F;
+    };
+    auto largest = [&](uint32_t top) {
+        top = __reduce_max_sync(0xffffffffu, top);
+        if (lane_id() == 0) sh.warp_max[warp_id()] = top;
+        __syncthreads();
+        return max(__reduce_max_sync(0xffffffffu, sh.warp_max[lane_id() & (WARPS - 1)]), K::NEG_INF);
+    };
+    if (k <= NT / 4) {                              // the threads' maxima are enough of them
+        float m[4], top = -INF_F;
+        for (int b = 0; b < sample; b += 4) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) m[u] = maximum(b + u);
+            top = fmaxf(top, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])));
+        }
+        const uint32_t mine = K::of(top);
+        return kth_of_threads<T, true>(true, mine, K::NEG_INF, largest(mine), k, k + k / 8);
+    }
+    uint32_t key[SAMPLE], top = 0;
+#pragma unroll
+    for (int u = 0; u < SAMPLE; ++u) { key[u] = K::of(maximum(u)); top = max(top, key[u]); }
+    int reached;
+    return kth_key(sh, K::NEG_INF, largest(top), k, k + k / 8, reached, [&](uint32_t mid) {
+        int r = 0;
+#pragma unroll
+        for (int u = 0; u < SAMPLE; ++u) r += key[u] >= mid;
+        return r;
+    });
+}
+
+// Of the n > k candidates (n <= CAP) those from the k-th on stay, in no order, k to k + slack of them; the others go into the rest, relative to a bound below
+// the former.  Returns the bound's key; [lo, hi] holds all keys.
+template <typename T> __device__ __noinline__ uint32_t prune(Shared& sh, int k, int slack, uint32_t lo, uint32_t hi, Rest& rest) {
+    const int t = threadIdx.x, n = sh.n;
+    unsigned long long c[ITEMS];
+    int reached;
+    uint32_t key;
+    c[0] = t < n ? sh.cand[t] : 0ull;
+    if (n <= NT) {
+        const uint32_t mine = t < n ? (uint32_t)(c[0] >> 32) : 0u;
+        key = kth_of_threads<T, false>(t < n, mine, lo, hi, k, k + slack);
+        reached = __syncthreads_count(t < n && mine >= key);
+    } else {
+#pragma unroll
+        for (int i = 1; i < ITEMS; ++i) c[i] = t + i * NT < n ? sh.cand[t + i * NT] : 0ull;
+        key = kth_key(sh, lo, hi, k, k + slack, reached, [&](uint32_t mid) {
+            int r = 0;
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) r += t + i * NT < n && (uint32_t)(c[i] >> 32) >= mid;
+            return r;
+        });
+    }
+    unsigned long long last = (unsigned long long)key << 32;
+    if (reached > k + slack) {                      // more equals of the k-th than places: the lowest indices
+        if (n <= NT)
+#pragma unroll
+            for (int i = 1; i < ITEMS; ++i) c[i] = 0ull;
+        clear_counts(sh);
+        int above = 0;
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) above += t + i * NT < n && (uint32_t)(c[i] >> 32) > key;
+        above = block_count(sh, above, 0);
+        last |= kth_key(sh, 0xFFFFFFFFu - (uint32_t)MAB_MAX_VOCAB, 0xFFFFFFFFu, k - above, k - above, reached, [&](uint32_t mid) {
+            int r = 0;
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) r += t + i * NT < n && (uint32_t)(c[i] >> 32) == key && (uint32_t)c[i] >= mid;
+            return r;
+        });
+    }
+    __syncthreads();
     if (t == 0) sh.n = 0;
     __syncthreads();
-    Rest rest = {0.0f, 0.0f, a.scale};
-    float bound = -INF_F;                           // values above it are candidates
-    bool all = true;                                // no bound yet: everything is one, NaN too
-
-    for (int base = v0; base < v1; base += NT * UNROLL) {
-        // a chunk: the vectors base + u NT + t.  The partial vectors are among the first and the last; what lies outside the row has no place.
-        uint4 raw[UNROLL];
-        int e_first[UNROLL];
-        uint32_t valid[UNROLL];                     // bits of the elements that are there
+    rest.move(Key<T>::bound(key));
+    double terms = 0.0;
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
+    for (int i = 0; i < ITEMS; ++i) {
+        if (t + i * NT >= n) break;
+        if (c[i] >= last) sh.cand[atomicAdd(&sh.n, 1)] = c[i];
+        else terms += grid_term(rest, Key<T>::value_of(c[i]));
+    }
+    add_terms(sh.terms, terms, rest);
+    return key;
+}
+
+// The candidates and the rest of the vectors [v0, v1), whatever they hold: every chunk's k largest that lie above the bound are found exactly, in
+// registers; the bound is the k-th of the chunk before, and of all candidates whenever those outgrow their room.
+template <typename T> __device__ __noinline__ void select_slowly(Shared& sh, const RowGrid<T>& g, int v0, int v1, int k, Rest& rest) {
+    constexpr int N = RowGrid<T>::N;
+    using K = Key<T>;
+    const int t = threadIdx.x;
+    __syncthreads();
+    if (t == 0) sh.n = 0;
+    rest.s = rest.ref = 0.0f;
+    uint32_t floor_key = 0;                         // smaller keys cannot be among the k largest any more
+    for (int base = v0; base < v1; base += NT * SLOW_UNROLL) {
+        float x[SLOW_UNROLL][N];
+        uint32_t valid[SLOW_UNROLL];                // bits of the elements that are there
+#pragma unroll
+        for (int u = 0; u < SLOW_UNROLL; ++u) {
             const int v = base + u * NT + t;
             valid[u] = 0;
-            raw[u] = make_uint4(0, 0, 0, 0);
-            e_first[u] = g.first(v);
             if (v < v1) {
-                if (g.whole(v)) { raw[u] = g.load(v); valid[u] = (1u << N) - 1u; }
-                else {
-                    float x[N];
-                    g.load_part(v, x, 0.0f);
-                    raw[u] = pack(x, (const T*)nullptr);
+                if (g.whole(v)) unpack(g.load(v), x[u], (const T*)nullptr);
+                else g.load_part(v, x[u], 0.0f);
 #pragma unroll
-                    for (int i = 0; i < N; ++i) if (e_first[u] + i >= 0 && e_first[u] + i < g.n) valid[u] |= 1u << i;
-                }
+                for (int i = 0; i < N; ++i) if (g.first(v) + i >= 0 && g.first(v) + i < g.n) valid[u] |= 1u << i;
             }
         }
-        const int n0 = sh.n;
-        const float s0 = rest.s;
-        bool exact = false;
-        if (all && min(v1 - base, NT * UNROLL) * N > ROOM) {
-            // a bound that at least k values of this chunk reach: the k-th largest of the vectors' maxima
-            uint32_t key[UNROLL];
-            uint32_t top = 0;
-#pragma unroll
-            for (int u = 0; u < UNROLL; ++u) {
-                float x[N], m = -INF_F;
-                unpack(raw[u], x, (const T*)nullptr);
-#pragma unroll
-                for (int i = 0; i < N; ++i) if (valid[u] >> i & 1u) m = fmaxf(m, x[i]);
-                key[u] = valid[u] ? row_key(m) : 0u;
-                top = max(top, key[u]);
-            }
-            top = __reduce_max_sync(0xffffffffu, top);
-            if (lane_id() == 0) sh.warp_max[warp_id()] = top;
-            clear_counts(sh);
-            for (int i = 0; i < WARPS; ++i) top = max(top, sh.warp_max[i]);
-            auto counted = [&](uint32_t mid) {
-                int r = 0;
-#pragma unroll
-                for (int u = 0; u < UNROLL; ++u) r += key[u] >= mid;
-                return r;
-            };
-            uint32_t lo = KEY_NEG_INF + 1, hi = top;
-            if (hi > lo && block_count(sh, counted(lo), 0) >= k) {
-                for (int i = 1; lo < hi; ++i) {
-                    const uint32_t mid = lo + (hi - lo) / 2 + 1;
-                    const int c = block_count(sh, counted(mid), i);
-                    if (c >= k) { lo = mid; if (c <= k + k / 4) break; }
-                    else hi = mid - 1;
-                }
-                bound = below_key(lo);
-                all = false;
-                rest.move(bound);
-            } else {
-                exact = true;                       // fewer than k numbers among the maxima
-            }
-        }
-        __syncthreads();                            // n0 is read
-        if (!exact) {
-            bool over = false;
-#pragma unroll
-            for (int u = 0; u < UNROLL; ++u) {
-                float x[N];
-                unpack(raw[u], x, (const T*)nullptr);
-                float m = x[0];
-#pragma unroll
-                for (int i = 1; i < N; ++i) m = fmaxf(m, x[i]);
-                if (all || m > bound || valid[u] != (1u << N) - 1u) {
-#pragma unroll
-                    for (int i = 0; i < N; ++i) {
-                        if (!(valid[u] >> i & 1u)) { x[i] = -INF_F; continue; }
-                        if (all || x[i] > bound) {
-                            const int at = atomicAdd(&sh.n, 1);
-                            if (at < CAP) sh.cand[at] = composite(x[i], e_first[u] + i);
-                            over |= at >= ROOM;
-                            x[i] = -INF_F;
-                        }
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < N; ++i) rest.add(x[i]);
-            }
-            if (!__syncthreads_or(over)) continue;
-            if (sh.n <= CAP) {
-                const uint32_t T_ = prune(sh, k, rest);
-                bound = T_ > KEY_NEG_INF ? ord_value(T_) : -INF_F;
-                all = false;
-                continue;
-            }
-        }
-        // exact selection from the chunk: its k largest eligible elements (all, where there are fewer) are candidates, the others go into the rest
-        __syncthreads();
-        if (t == 0) sh.n = n0;
-        rest.s = s0;
-        const uint32_t floor_key = all ? 0u : (bound == -INF_F ? KEY_NEG_INF : row_key(bound)) + 1u;     // eligible: key >= floor_key
         auto counted = [&](uint32_t mid) {
             int r = 0;
 #pragma unroll
-            for (int u = 0; u < UNROLL; ++u) {
-                float x[N];
-                unpack(raw[u], x, (const T*)nullptr);
+            for (int u = 0; u < SLOW_UNROLL; ++u)
 #pragma unroll
-                for (int i = 0; i < N; ++i) r += (valid[u] >> i & 1u) && row_key(x[i]) >= mid;
-            }
+                for (int i = 0; i < N; ++i) r += (valid[u] >> i & 1u) && K::of(x[u][i]) >= mid;
             return r;
         };
         clear_counts(sh);
@@ -255,43 +290,160 @@ __global__ void __launch_bounds__(NT, 2) topk_logits_kernel(Args a) {
         uint32_t kth = floor_key;
         int need = 0x7FFFFFFF;                      // equals of the k-th that are taken, in the order of their indices
         if (eligible > k) {
-            kth = kth_key(sh, floor_key, 0xFFFFFFFFu, k, counted);
+            int reached;
+            kth = kth_key(sh, floor_key, K::MOST, k, 0, reached, counted);
             clear_counts(sh);
-            need = k - block_count(sh, kth == 0xFFFFFFFFu ? 0 : counted(kth + 1u), 0);
-            rest.move(kth > KEY_NEG_INF ? ord_value(kth) : -INF_F);
+            need = k - block_count(sh, counted(kth + 1u), 0);
+            rest.move(K::bound(kth));
         }
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
-            float x[N];
-            unpack(raw[u], x, (const T*)nullptr);
-            int equal = 0;
+        for (int u = 0; u < SLOW_UNROLL; ++u) {
+            int equal = 0, total = 0, before = 0;
 #pragma unroll
-            for (int i = 0; i < N; ++i) equal += (valid[u] >> i & 1u) && row_key(x[i]) == kth;
-            int total = 0;
-            int before = need == 0x7FFFFFFF ? 0 : block_exclusive_scan(equal, sh.scan, total);
+            for (int i = 0; i < N; ++i) equal += (valid[u] >> i & 1u) && K::of(x[u][i]) == kth;
+            if (need != 0x7FFFFFFF) before = block_exclusive_scan(equal, sh.scan, total);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 if (!(valid[u] >> i & 1u)) continue;
-                const uint32_t key = row_key(x[i]);
-                const bool take = key > kth || (key == kth && (need == 0x7FFFFFFF || before++ < need));
-                if (take) sh.cand[atomicAdd(&sh.n, 1)] = composite(x[i], e_first[u] + i);
-                else rest.add(x[i]);
+                const uint32_t key = K::of(x[u][i]);
+                if (key > kth || (key == kth && (need == 0x7FFFFFFF || before++ < need)))
+                    sh.cand[atomicAdd(&sh.n, 1)] = K::composite(x[u][i], g.first(base + u * NT + t) + i);
+                else rest.add(x[u][i]);
             }
             if (need != 0x7FFFFFFF) need = max(0, need - total);
             __syncthreads();
         }
-        if (eligible > k) { bound = kth > KEY_NEG_INF ? ord_value(kth) : -INF_F; all = false; }
-        __syncthreads();
-        if (sh.n > ROOM) {                          // (n0 + k can be beyond it: the next chunk needs the room)
-            const uint32_t T_ = prune(sh, k, rest);
-            bound = T_ > KEY_NEG_INF ? ord_value(T_) : -INF_F;
-            all = false;
+        if (eligible > k) floor_key = kth + 1u;     // k values from the k-th on are held, with lower indices than all that follow
+        if (sh.n > CAP - k) floor_key = prune<T>(sh, k, 0, 0u, K::MOST, rest) + 1u;
+    }
+    __syncthreads();
+}
+
+template <typename T>
+__global__ void __launch_bounds__(NT, 3) topk_logits_kernel(Args a) {
+    constexpr int N = RowGrid<T>::N;
+    using K = Key<T>;
+    extern __shared__ __align__(16) unsigned char dyn[];
+    Shared& sh = *reinterpret_cast<Shared*>(dyn);
+    const int C = a.cluster, rank = C > 1 ? (int)(blockIdx.x % C) : 0, t = threadIdx.x, k = a.k;
+    const int64_t row = blockIdx.x / C;
+    const RowGrid<T> g(reinterpret_cast<const T*>(a.logits) + row * a.pitch, a.vocab);
+    const int per = (g.count + C - 1) / C, v0 = min(rank * per, g.count), v1 = min(v0 + per, g.count);
+    const int w0 = g.whole_from(v0), w1 = g.whole_to(v1);
+    if (t == 0) sh.n = sh.n_list = sh.n_reach = 0;
+    Rest rest = {0.0f, 0.0f, a.scale, false};
+    float bound = -INF_F;                           // values above it are candidates
+    uint32_t lo_key = 0, top_key = K::MOST;         // no candidate's key lies outside
+    bool slow = false;
+    const bool all = (v1 - v0) * N <= CAP;          // everything is a candidate
+
+    if (!all) {
+        const uint32_t at = bound_of_sample<T>(sh, g, w0, w1, k, a.sample);
+        slow = at == K::NEG_INF;                    // fewer than k numbers among the maxima
+        if (!slow) {
+            bound = K::below(at);
+            lo_key = at;
+            rest.move(bound);
         }
     }
     __syncthreads();
-    if (C > 1 && sh.n > k) prune(sh, k, rest);
+    if (!slow) {
+        uint64_t sum = 0;                           // two floats
+        const uint64_t scale2 = pair_of(a.scale, a.scale), ref2 = pair_of(-rest.ref, -rest.ref);
+        auto see = [&](uint4 r, int v) {
+            const float m = vector_max(r, (const T*)nullptr);
+            if (m > bound) {
+                const int at = atomicAdd(&sh.n_list, 1);
+                if (at < LIST) { sh.list[at] = v; sh.list_key[at] = K::of(m); }
+            } else {
+                uint64_t x[N / 2];
+                unpack_pairs(r, x, (const T*)nullptr);
+#pragma unroll
+                for (int i = 0; i < N / 2; ++i) {
+                    float lo, hi;
+                    split(fma2(x[i], scale2, ref2), lo, hi);
+                    sum = add2(sum, pair_of(ex2(lo), ex2(hi)));
+                }
+            }
+        };
+        auto push = [&](float x, int e) {
+            const int at = atomicAdd(&sh.n, 1);
+            if (at < CAP) sh.cand[at] = K::composite(x, e);
+        };
+        if (!all) {
+            int v = w0 + t;
+            for (; v + (UNROLL - 1) * NT < w1; v += UNROLL * NT) {
+                uint4 r[UNROLL];
+#pragma unroll
+                for (int u = 0; u < UNROLL; ++u) r[u] = g.load(v + u * NT);
+#pragma unroll
+                for (int u = 0; u < UNROLL; ++u) see(r[u], v + u * NT);
+            }
+            for (; v < w1; v += NT) see(g.load(v), v);
+        }
+        float lo, hi;
+        split(sum, lo, hi);
+        rest.s += lo + hi;
+        __syncthreads();
+        // the vectors of the list (or all), element by element.  As many vectors as k reach the k-th of their largest: a bound nearer to the k-th value
+        const int listed = all ? w1 - w0 : sh.n_list;
+        slow = listed > LIST;
+        if (!slow && !all) {
+            lo_key = kth_of_list<T>(sh, listed, k, k / 8, lo_key, top_key);
+            bound = K::below(lo_key);
+            rest.move(bound);
+        }
+        double terms = 0.0;
+        if (all) {
+            for (int i = t; i < listed * N; i += NT) push(Elem<T>::load(g.p, g.first(w0) + i), g.first(w0) + i);
+        } else if (!slow) {
+            // vectors below the new bound go into the sum; of the others, which are some k, a thread has an element at a time
+            for (int j = t; j < listed; j += NT) {
+                const int v = sh.list[j];
+                if (sh.list_key[j] >= lo_key) {
+                    const int at = atomicAdd(&sh.n_reach, 1);
+                    if (at < REACH) sh.reach[at] = v;
+                    continue;
+                }
+                float x[N];
+                unpack(g.load(v), x, (const T*)nullptr);
+#pragma unroll
+                for (int i = 0; i < N; ++i) terms += grid_term(rest, x[i]);
+            }
+            __syncthreads();
+            const int reaching = sh.n_reach;
+            slow = reaching > REACH;
+            if (!slow)
+                for (int i = t; i < reaching * N; i += NT) {
+                    const int e = g.first(sh.reach[i / N]) + i % N;
+                    const float x = Elem<T>::load(g.p, e);
+                    if (x > bound) push(x, e);
+                    else terms += grid_term(rest, x);
+                }
+        }
+        if (t < 2) {                                // the partial vectors
+            const int pv = t == 0 ? 0 : g.count - 1;
+            if (pv >= v0 && pv < v1 && !g.whole(pv) && (t == 0 || g.count > 1)) {
+                for (int i = 0; i < N; ++i) {
+                    const int e = g.first(pv) + i;
+                    if (e < 0 || e >= g.n) continue;
+                    const float x = Elem<T>::load(g.p, e);
+                    if (all || x > bound) push(x, e);
+                    else rest.add(x);
+                }
+            }
+        }
+        add_terms(sh.terms, terms, rest);
+        slow |= sh.n > CAP;
+    }
+    if (slow) {
+        select_slowly<T>(sh, g, v0, v1, k, rest);
+        lo_key = 0;
+    }
 
     if (C > 1) {                                    // the first CTA takes over the others' candidates and sums
+        if (sh.n > k) prune<T>(sh, k, 0, lo_key, K::MOST, rest);
+        lo_key = 0;                                 // (the others' bounds are others)
         float s = rest.s;
 #pragma unroll
         for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -302,65 +454,74 @@ __global__ void __launch_bounds__(NT, 2) topk_logits_kernel(Args a) {
             for (int i = 0; i < WARPS; ++i) sum += sh.red[i];
             sh.sum = sum;
             sh.ref = rest.ref;
+            sh.far = rest.far;
         }
         cluster_arrive_wait();
         if (rank == 0) {
-            const int mine = sh.n;
-            int at = mine;
+            int at = sh.n;
             for (int c = 1; c < C; ++c) {
                 const int n = (int)cluster_load_u32(&sh.n, c);
                 for (int i = t; i < n; i += NT) sh.cand[at + i] = cluster_load_u64(&sh.cand[i], c);
                 at += n;
             }
-            __syncthreads();
-            if (t == 0) sh.n = at;
+            for (int c = 1; c < C; ++c) rest.far |= cluster_load_u32(&sh.far, c) != 0u;
             float ref = -INF_F;                     // the largest reference of those that have a sum
             for (int c = 0; c < C; ++c)
                 if (!(cluster_load_f64(&sh.sum, c) == 0.0)) ref = fmaxf(ref, cluster_load_f32(&sh.ref, c));
-            rest.move(ref);
-            if (t == 0)
-                for (int c = 1; c < C; ++c) {
-                    const double sum = cluster_load_f64(&sh.sum, c);
-                    if (!(sum == 0.0)) rest.s += (float)(sum * exp(((double)cluster_load_f32(&sh.ref, c) - (double)rest.ref) / a.tau));
-                }
+            if (ref != -INF_F) {
+                if (!(rest.s == 0.0f)) rest.s *= ex2(rest.ref - ref);
+                rest.ref = ref;
+                if (t == 0)
+                    for (int c = 1; c < C; ++c) {
+                        const double sum = cluster_load_f64(&sh.sum, c);
+                        if (!(sum == 0.0)) rest.s += (float)(sum * exp2((double)cluster_load_f32(&sh.ref, c) - (double)ref));
+                    }
+            }
+            __syncthreads();
+            if (t == 0) sh.n = at;
             __syncthreads();
         }
         cluster_arrive_wait();
         if (rank != 0) return;
     }
-    if (sh.n > k && sh.n > NT) prune(sh, k, rest);
-
-    // places: the number of larger candidates
-    const int n = sh.n;
-    unsigned long long mine[LAST];
-    int place[LAST];
-#pragma unroll
-    for (int i = 0; i < LAST; ++i) {
-        mine[i] = t + i * NT < n ? sh.cand[t + i * NT] : 0ull;
-        place[i] = 0;
+    // those from the k-th on, in order: a few by the number of larger ones, many by a sorting network
+    const bool few = k <= 128;
+    if (sh.n > (few ? 192 : k)) prune<T>(sh, k, few ? 64 : 0, lo_key, K::MOST, rest);
+    unsigned long long* cand = sh.cand;
+    const int kept = sh.n;                          // k, or up to 192 where few
+    if (few) {
+        const unsigned long long mine = t < kept ? cand[t] : 0ull;
+        int place = 0;
+        if (t < kept)
+            for (int j = 0; j < kept; ++j) place += cand[j] > mine;
+        __syncthreads();
+        if (t < kept && place < k) cand[place] = mine;
+        __syncthreads();
+        if (kept > k) {
+            rest.move(K::bound((uint32_t)(cand[k - 1] >> 32)));
+            add_terms(sh.terms, t < kept && place >= k ? grid_term(rest, K::value_of(mine)) : 0.0, rest);
+        }
+    } else {
+        int size = 256;
+        while (size < k) size *= 2;
+        for (int i = k + t; i < size; i += NT) cand[i] = 0ull;
+        for (int block = 2; block <= size; block *= 2)
+            for (int d = block / 2; d; d /= 2) {
+                __syncthreads();
+                for (int i = t; i < size / 2; i += NT) {
+                    const int p = 2 * i - (i & (d - 1)), q = p + d;
+                    const unsigned long long x = cand[p], y = cand[q];
+                    if ((x < y) == ((p & block) == 0)) { cand[p] = y; cand[q] = x; }
+                }
+            }
+        __syncthreads();
     }
-    for (int j = 0; j < n; ++j) {
-        const unsigned long long other = sh.cand[j];
-#pragma unroll
-        for (int i = 0; i < LAST; ++i) place[i] += other > mine[i];
-    }
-#pragma unroll
-    for (int i = 0; i < LAST; ++i) {
-        if (t + i * NT >= n || place[i] >= k) continue;
-        const int e = index_of(mine[i]);
-        a.indices[row * k + place[i]] = e;
-        reinterpret_cast<T*>(a.values)[row * k + place[i]] = g.p[e];
-        if (place[i] == k - 1) sh.kth = mine[i];
-    }
-    __syncthreads();
-    const uint32_t kth = (uint32_t)(sh.kth >> 32);
-    rest.move(kth > KEY_NEG_INF ? ord_value(kth) : -INF_F);
-#pragma unroll
-    for (int i = 0; i < LAST; ++i) {
-        if (t + i * NT >= n) continue;
-        const float x = value_of(mine[i]);
-        if (place[i] >= k) rest.add(x);
-        else if (x != x) rest.s = x;                // a NaN in the list: the rest is NaN
+    for (int i = t; i < k; i += NT) {
+        const unsigned long long c = cand[i];
+        const int e = index_of(c);
+        a.indices[row * k + i] = e;
+        reinterpret_cast<T*>(a.values)[row * k + i] = g.p[e];
+        if ((uint32_t)(c >> 32) == 0u) rest.s = K::value_of(c);             // a NaN in the list: the rest is NaN
     }
     float s = rest.s;
 #pragma unroll
@@ -369,25 +530,26 @@ __global__ void __launch_bounds__(NT, 2) topk_logits_kernel(Args a) {
     __syncthreads();
     double sum = 0.0;
     for (int i = 0; i < WARPS; ++i) sum += sh.red[i];
-    double ref = (double)rest.ref;
-    if (sum == sum ? (!(sum >= 1e-20) && a.vocab > k) : rest.ref == INF_F) {
+    double ref = (double)rest.ref * 0.69314718055994531;
+    const unsigned long long last = cand[k - 1];
+    if (a.vocab > k && (rest.far || (sum == sum && !(sum >= 1e-3)))) {
         // nothing to speak of relative to the bound (masked logits, a gap), or infinities: again, relative to the largest of the rest
-        const unsigned long long last = sh.kth;
         float m = -INF_F, bad = 0.0f;
         for (int e = t; e < a.vocab; e += NT) {
             const float x = Elem<T>::load(g.p, e);
             if (x != x) bad = x;
-            else if (composite(x, e) < last) m = fmaxf(m, x);
+            else if (K::composite(x, e) < last) m = fmaxf(m, x);
         }
-        m = ord_value(__reduce_max_sync(0xffffffffu, ord_key(m)));
-        if (lane_id() == 0) sh.warp_max[warp_id()] = ord_key(m);
+        const uint32_t top = __reduce_max_sync(0xffffffffu, ord_key(m));
+        if (lane_id() == 0) sh.warp_max[warp_id()] = top;
         __syncthreads();
+        m = -INF_F;
         for (int i = 0; i < WARPS; ++i) m = fmaxf(m, ord_value(sh.warp_max[i]));
         double part = (double)bad;
         if (m != -INF_F && m != INF_F)
             for (int e = t; e < a.vocab; e += NT) {
                 const float x = Elem<T>::load(g.p, e);
-                if (x == x && composite(x, e) < last) part += (double)ex2((x - m) * a.scale);
+                if (x == x && K::composite(x, e) < last) part += (double)ex2((x - m) * a.scale);
             }
 #pragma unroll
         for (int o = 16; o; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
@@ -396,11 +558,10 @@ __global__ void __launch_bounds__(NT, 2) topk_logits_kernel(Args a) {
         __syncthreads();
         sum = 0.0;
         for (int i = 0; i < WARPS; ++i) sum += sh.red[i];
-        ref = (double)m;
-        if (m == INF_F && sum == sum) { sum = 1.0; }
-        if (m == -INF_F) ref = 0.0;
+        ref = m == -INF_F ? 0.0 : (double)m / a.tau;
+        if (m == INF_F && sum == sum) sum = 1.0;
     }
-    if (t == 0) a.rest[row] = sum == 0.0 ? -INF_F : (float)(ref / a.tau + log(sum));
+    if (t == 0) a.rest[row] = sum == 0.0 ? -INF_F : (float)(ref + log(sum));
 }
 
 template <typename T> int launch(Args a, int64_t rows, cudaStream_t s) {
@@ -409,6 +570,9 @@ template <typename T> int launch(Args a, int64_t rows, cudaStream_t s) {
     // CTAs of a row: until every SM has one, no part below 4 KB, and the merged lists fit the candidates' room
     a.cluster = 1;
     while (a.cluster < 8 && rows * a.cluster * 2 <= sms && (int64_t)a.vocab * sizeof(T) / (2 * a.cluster) >= 4096 && 2 * a.cluster * a.k <= CAP) a.cluster *= 2;
+    // vectors a thread samples: so many that some k (part / sample) candidates fit, a quarter of the room for what the sample does not show
+    const int64_t part = ((int64_t)a.vocab / RowGrid<T>::N + a.cluster) / a.cluster;
+    a.sample = (int)std::min<int64_t>(SAMPLE, std::max<int64_t>(4, ceil_div64(part * a.k, (int64_t)NT * CAP * 3 / 4)));
     return launch_rows(topk_logits_kernel<T>, "topk_logits", rows * a.cluster, NT, sizeof(Shared), a.cluster, s, a);
 }
 
