@@ -143,6 +143,116 @@ __global__ void __launch_bounds__(THREADS) int8_matmul_kernel(const __grid_const
     if (warp == 1) { tmem_fence_after(); tmem_free(acc, COLUMNS); }
 }
 
+// The form for many tokens: two CTAs share a tile of 256 channels and up to 256 tokens, so a stage of the ring is 16 KB of weights and up to 16 KB of tokens
+// a CTA for twice the products, and they stay on their SMs: while eight warps take the sums of one tile out of tensor memory, the next tile's go into its other
+// half.  Tiles of the same channels follow one another: the weights come from HBM once.
+constexpr int PAIR_THREADS = 320, PAIR_STAGES = 6, PAIR_STAGE = 2 * BM * BK, PAIR_LIMIT = 1 << 18;
+constexpr int PAIR_BYTES = PAIR_STAGE * PAIR_STAGES + 1024;
+
+template <typename T>
+__global__ void __launch_bounds__(PAIR_THREADS) int8_matmul_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                                                                        const __grid_constant__ Args g, int tokens, int tiles) {
+    extern __shared__ unsigned char dyn[];
+    unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~(uintptr_t)1023);
+    __shared__ uint64_t full[PAIR_STAGES], empty[PAIR_STAGES], ready[2], taken[2];
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_lost;
+    const int warp = warp_id(), lane = lane_id(), t = threadIdx.x, rank = (int)(blockIdx.x & 1), pair = (int)(blockIdx.x >> 1), pairs = (int)(gridDim.x >> 1);
+    const int steps = (g.k + BK - 1) / BK;
+    if (t == 0) {
+        for (int i = 0; i < PAIR_STAGES; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&ready[i], 1); mbar_init(&taken[i], 16); }
+        s_lost = 0;
+    }
+    if (warp == 1) tmem_alloc_pair(&s_tmem, 512);
+    tmem_fence_before();
+    __syncthreads();
+    cluster_arrive_wait();                          // the other CTA's barriers are there
+    tmem_fence_after();
+    const uint32_t acc = s_tmem;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int n = 0;                              // stages filled so far
+            bool ok = true;
+            for (int tile = pair; ok && tile < tiles; tile += pairs) {
+                const int token0 = tile % g.token_tiles * tokens + rank * (tokens / 2), channel0 = tile / g.token_tiles * 2 * BM + rank * BM;
+                for (int i = 0; i < steps; ++i, ++n) {
+                    const int s = n % PAIR_STAGES, round = n / PAIR_STAGES;
+                    if (round > 0 && !mbar_wait_cluster(&empty[s], (round - 1) & 1, PAIR_LIMIT)) { ok = false; break; }
+                    unsigned char* stage = ring + s * PAIR_STAGE;
+                    const uint32_t bar = cluster_addr(&full[s], 0);
+                    if (rank == 0) mbar_arrive_expect_tx(&full[s], (uint32_t)(2 * BM + tokens) * BK);     // both CTAs' bytes
+                    tile_g2s_pair(stage, &map_b, i * BK, channel0, bar);
+                    tile_g2s_pair(stage + BM * BK, &map_a, i * BK, token0, bar);
+                }
+            }
+            if (!ok) atomicExch(&s_lost, 1);
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            const uint32_t instruction = i8_instruction(2 * BM, tokens);
+            int n = 0, done = 0;                    // stages, tiles
+            bool ok = true;
+            for (int tile = pair; ok && tile < tiles; tile += pairs, ++done) {
+                const uint32_t d = acc + (done & 1) * 256;
+                if (done >= 2 && !mbar_wait_cluster(&taken[done & 1], (done / 2 - 1) & 1, PAIR_LIMIT)) { ok = false; break; }
+                tmem_fence_after();
+                for (int i = 0; i < steps; ++i, ++n) {
+                    const int s = n % PAIR_STAGES, round = n / PAIR_STAGES;
+                    if (!mbar_wait_cluster(&full[s], round & 1, PAIR_LIMIT)) { ok = false; break; }
+                    tmem_fence_after();
+                    const uint32_t stage = smem_addr(ring + s * PAIR_STAGE);
+                    const uint64_t wd = operand_desc(stage), td = operand_desc(stage + BM * BK);
+#pragma unroll
+                    for (int j = 0; j < BK / 32; ++j) mma_i8_pair(d, wd + 2 * j, td + 2 * j, instruction, i > 0 || j > 0);
+                    mma_commit_pair(&empty[s]);
+                }
+                if (ok) mma_commit_pair(&ready[done & 1]);
+            }
+            if (!ok) {                              // copies that may still be on their way must not outlive the CTAs
+                atomicExch(&s_lost, 1);
+                for (int i = 0; i < PAIR_STAGES; ++i, ++n) mbar_wait_cluster(&full[n % PAIR_STAGES], n / PAIR_STAGES & 1, 1 << 10);
+            }
+        }
+    } else {
+        const int quarter = warp & 3, half = (warp - 2) >> 2;               // 32 channels, half of the tokens
+        const int c0 = half ? (tokens / 2 + 15) / 16 * 16 : 0, c1 = half ? tokens : (tokens / 2 + 15) / 16 * 16;
+        int done = 0;
+        for (int tile = pair; tile < tiles; tile += pairs, ++done) {
+            const int token0 = tile % g.token_tiles * tokens, channel = tile / g.token_tiles * 2 * BM + rank * BM + 32 * quarter + lane;
+            const bool there = channel < g.n;
+            const float cs = there ? g.b_scales[channel] : 0.0f, bias = g.bias && there ? g.bias[channel] : 0.0f;
+            if (!mbar_wait_cluster(&ready[done & 1], done / 2 & 1, PAIR_LIMIT)) { if (lane == 0) atomicExch(&s_lost, 1); break; }
+            tmem_fence_after();
+            const uint32_t from = acc + ((uint32_t)(32 * quarter) << 16) + (done & 1) * 256;
+            T* out = reinterpret_cast<T*>(g.out) + (int64_t)token0 * g.out_pitch + channel;
+            for (int c = c0; c < c1; c += 16) {
+                int r[16];
+                tmem_load(from + c, r);
+                const float scale = token0 + c + (lane & 15) < g.m ? g.a_scales[token0 + c + (lane & 15)] : 0.0f;
+                tmem_wait_load();
+                if (c + 16 >= c1) {                 // the sums of the tile are in registers: its half of tensor memory is free
+                    tmem_fence_before();
+                    if (lane == 0) mbar_arrive_cluster(cluster_addr(&taken[done & 1], 0));
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float s = __shfl_sync(0xffffffffu, scale, i);
+                    if (there && token0 + c + i < g.m) Elem<T>::store(out, (int64_t)(c + i) * g.out_pitch, scaled(r[i], s, cs, bias));
+                }
+            }
+        }
+    }
+    __syncwarp();
+    tmem_fence_before();
+    __syncthreads();
+    if (s_lost && t == 0) atomicExch(&g_timeout, 1);
+    cluster_arrive_wait();                          // nobody reports to a CTA that is gone
+    tmem_fence_after();
+    if (warp == 1) tmem_free_pair(acc, 512);
+}
+
 // M tokens (m of them there): a warp for R channels, its lanes over the inner size.
 template <typename T, int M, int R>
 __global__ void __launch_bounds__(256) int8_rows_kernel(const __grid_constant__ Args g) {
@@ -230,6 +340,18 @@ template <typename T, int BN> int launch_tiles(Args g, int sms, cudaStream_t s) 
     return launch_rows(int8_matmul_kernel<T, BN>, "int8_matmul", tiles * g.split, THREADS, Ring<BN>::BYTES, g.split, s, map_a, map_b, g);
 }
 
+// Tiles of 256 channels and as few tokens as cover them all evenly (a multiple of 32).
+template <typename T> int launch_pairs(Args g, int sms, cudaStream_t s) {
+    const int parts = (g.m + 255) / 256, tokens = ((g.m + parts - 1) / parts + 31) / 32 * 32;
+    CUtensorMap map_a, map_b;
+    if (int rc = make_map(&map_a, g.a, g.m, g.k, g.a_pitch, tokens / 2)) return rc;
+    if (int rc = make_map(&map_b, g.b, g.n, g.k, g.b_pitch, BM)) return rc;
+    g.token_tiles = (g.m + tokens - 1) / tokens;
+    const int64_t tiles = (int64_t)g.token_tiles * ((g.n + 2 * BM - 1) / (2 * BM));
+    const int64_t pairs = std::min<int64_t>(tiles, sms / 2);
+    return launch_rows(int8_matmul_pair_kernel<T>, "int8_matmul", pairs * 2, PAIR_THREADS, PAIR_BYTES, 2, s, map_a, map_b, g, tokens, (int)tiles);
+}
+
 template <typename T> int launch(const Args& g, cudaStream_t s) {
     const int sms = device_sm_count();
     if (sms < 0) return MAB_ERR_CUDA;
@@ -239,6 +361,7 @@ template <typename T> int launch(const Args& g, cudaStream_t s) {
         if (g.m == 2) return launch_rows(int8_rows_kernel<T, 2, 2>, "int8_matmul", ctas, 256, 0, 1, s, g);
         return launch_rows(int8_rows_kernel<T, 4, 2>, "int8_matmul", ctas, 256, 0, 1, s, g);
     }
+    if (g.m > 64 && ceil_div64(g.m, 256) * ceil_div64(g.n, 2 * BM) * 4 >= sms) return launch_pairs<T>(g, sms, s);
     if (g.m <= 16) return launch_tiles<T, 16>(g, sms, s);
     if (g.m <= 32) return launch_tiles<T, 32>(g, sms, s);
     if (g.m <= 64) return launch_tiles<T, 64>(g, sms, s);
