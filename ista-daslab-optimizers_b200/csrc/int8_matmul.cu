@@ -216,30 +216,46 @@ __global__ void __launch_bounds__(PAIR_THREADS) int8_matmul_pair_kernel(const __
             }
         }
     } else {
-        const int quarter = warp & 3, half = (warp - 2) >> 2;               // 32 channels, half of the tokens
-        const int c0 = half ? (tokens / 2 + 15) / 16 * 16 : 0, c1 = half ? tokens : (tokens / 2 + 15) / 16 * 16;
+        // 32 channels and every other group of 32 tokens a warp
+        const int quarter = warp & 3, half = (warp - 2) >> 2, groups = tokens / 32;
         int done = 0;
         for (int tile = pair; tile < tiles; tile += pairs, ++done) {
             const int token0 = tile % g.token_tiles * tokens, channel = tile / g.token_tiles * 2 * BM + rank * BM + 32 * quarter + lane;
             const bool there = channel < g.n;
             const float cs = there ? g.b_scales[channel] : 0.0f, bias = g.bias && there ? g.bias[channel] : 0.0f;
+            float scale[4];                         // of the tokens of this warp's groups, one a lane
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int token = token0 + (2 * j + half) * 32 + lane;
+                scale[j] = 2 * j + half < groups && token < g.m ? g.a_scales[token] : 0.0f;
+            }
             if (!mbar_wait_cluster(&ready[done & 1], done / 2 & 1, PAIR_LIMIT)) { if (lane == 0) atomicExch(&s_lost, 1); break; }
             tmem_fence_after();
             const uint32_t from = acc + ((uint32_t)(32 * quarter) << 16) + (done & 1) * 256;
-            T* out = reinterpret_cast<T*>(g.out) + (int64_t)token0 * g.out_pitch + channel;
-            for (int c = c0; c < c1; c += 16) {
-                int r[16];
-                tmem_load(from + c, r);
-                const float scale = token0 + c + (lane & 15) < g.m ? g.a_scales[token0 + c + (lane & 15)] : 0.0f;
+            if (half >= groups && lane == 0) mbar_arrive_cluster(cluster_addr(&taken[done & 1], 0));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int group = 2 * j + half;
+                if (group >= groups) break;
+                int r[32];
+                tmem_load(from + 32 * group, r);
                 tmem_wait_load();
-                if (c + 16 >= c1) {                 // the sums of the tile are in registers: its half of tensor memory is free
+                if (group + 2 >= groups) {          // the warp's sums of the tile are in registers
                     tmem_fence_before();
                     if (lane == 0) mbar_arrive_cluster(cluster_addr(&taken[done & 1], 0));
                 }
+                const int first = token0 + 32 * group, there_tokens = g.m - first;
+                T* out = reinterpret_cast<T*>(g.out) + (int64_t)first * g.out_pitch + channel;
+                if (there_tokens >= 32 && __all_sync(0xffffffffu, there)) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float s = __shfl_sync(0xffffffffu, scale, i);
-                    if (there && token0 + c + i < g.m) Elem<T>::store(out, (int64_t)(c + i) * g.out_pitch, scaled(r[i], s, cs, bias));
+                    for (int i = 0; i < 32; ++i, out += g.out_pitch)
+                        Elem<T>::store(out, 0, scaled(r[i], __shfl_sync(0xffffffffu, scale[j], i), cs, bias));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i, out += g.out_pitch) {
+                        const float s = __shfl_sync(0xffffffffu, scale[j], i);
+                        if (there && i < there_tokens) Elem<T>::store(out, 0, scaled(r[i], s, cs, bias));
+                    }
                 }
             }
         }
