@@ -22,71 +22,81 @@ struct Args {
     const float *a_scales, *b_scales, *bias;
     void* out;
     int m, n, k;
-    int token_tiles, split;
+    int token_tiles, split, stages, height;        // tiles of `height` channels (a multiple of 8, at most 128)
 };
 
 __device__ __forceinline__ float scaled(int sum, float token, float channel, float bias) { return fmaf((float)sum * token, channel, bias); }
 
-template <int BN> struct Ring {
-    static constexpr int STAGE = (BM + BN) * BK;
-    static constexpr int STAGES = BN == 256 ? 4 : BN == 128 ? 6 : 8;
-    static constexpr int BYTES = STAGE * STAGES + 1024;
-};
+constexpr int MOST_STAGES = 9, RING_ONE = 200 * 1024, RING_TWO = 108 * 1024;      // the ring of one CTA, or of each of two, on an SM
 
 template <typename T, int BN>
 __global__ void __launch_bounds__(THREADS) int8_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                                                               const __grid_constant__ Args g) {
-    using R = Ring<BN>;
+    constexpr int STAGE = (BM + BN) * BK;
     extern __shared__ unsigned char dyn[];
     unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~(uintptr_t)1023);
-    __shared__ uint64_t full[R::STAGES], empty[R::STAGES], done;
+    __shared__ uint64_t full[MOST_STAGES], empty[MOST_STAGES], done;
     __shared__ uint32_t s_tmem;
     __shared__ int s_lost;
     __shared__ float s_token[BN];
+    __shared__ float2 s_channel[BM];
     constexpr uint32_t COLUMNS = BN < 32 ? 32 : BN;
     const int warp = warp_id(), lane = lane_id(), t = threadIdx.x;
     const int rank = g.split > 1 ? (int)(blockIdx.x % g.split) : 0;
-    const int tile = blockIdx.x / g.split, token0 = tile % g.token_tiles * BN, channel0 = tile / g.token_tiles * BM;
+    const int tile = blockIdx.x / g.split, token0 = tile % g.token_tiles * BN, channel0 = tile / g.token_tiles * g.height;
     const int steps = (g.k + BK - 1) / BK, k0 = (int)((int64_t)steps * rank / g.split), k1 = (int)((int64_t)steps * (rank + 1) / g.split);
+    const int stages = g.stages;
+    auto load = [&](int i, int s) {                 // step i into stage s
+        unsigned char* stage = ring + s * STAGE;
+        mbar_arrive_expect_tx(&full[s], (uint32_t)(g.height + BN) * BK);
+        tile_g2s(stage, &map_b, i * BK, channel0, &full[s]);
+        tile_g2s(stage + BM * BK, &map_a, i * BK, token0, &full[s]);
+    };
     if (t == 0) {
-        for (int i = 0; i < R::STAGES; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+        for (int i = 0; i < stages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
         mbar_init(&done, 1);
         s_lost = 0;
+        for (int i = k0; i < k1 && i < k0 + stages; ++i) load(i, i - k0);         // (only this thread and the copy engine know of the barriers yet)
     }
     if (warp == 1) tmem_alloc(&s_tmem, COLUMNS);
     for (int i = t; i < BN; i += THREADS) s_token[i] = token0 + i < g.m ? g.a_scales[token0 + i] : 0.0f;
+    if (t < BM) {
+        const int channel = channel0 + t;
+        s_channel[t] = t < g.height && channel < g.n ? make_float2(g.b_scales[channel], g.bias ? g.bias[channel] : 0.0f) : make_float2(0.0f, 0.0f);
+    }
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
     const uint32_t acc = s_tmem;
 
-    if (warp == 0) {
-        if (lane == 0)
-            for (int i = k0; i < k1; ++i) {
-                const int s = (i - k0) % R::STAGES, round = (i - k0) / R::STAGES;
-                if (round > 0 && !mbar_wait(&empty[s], (round - 1) & 1)) { atomicExch(&s_lost, 1); break; }
-                unsigned char* stage = ring + s * R::STAGE;
-                mbar_arrive_expect_tx(&full[s], R::STAGE);
-                tile_g2s(stage, &map_b, i * BK, channel0, &full[s]);
-                tile_g2s(stage + BM * BK, &map_a, i * BK, token0, &full[s]);
+    if (warp < 2) {
+        const bool issuing = elect_one();
+        int s = 0;
+        uint32_t parity = 0;
+        auto next = [&] { if (++s == stages) { s = 0; parity ^= 1; } };
+        if (warp == 0) {
+            for (int i = k0 + stages; i < k1; ++i, next()) {
+                if (!mbar_wait(&empty[s], parity)) { s_lost = 1; break; }
+                if (issuing) load(i, s);
+                __syncwarp();
             }
-    } else if (warp == 1) {
-        if (lane == 0) {
-            for (int i = k0; i < k1; ++i) {
-                const int s = (i - k0) % R::STAGES, round = (i - k0) / R::STAGES;
-                if (!mbar_wait(&full[s], round & 1)) {
-                    atomicExch(&s_lost, 1);         // the copies that may still be on their way: they must not outlive the CTA
-                    for (int n = i; n < k1 && n < i + R::STAGES; ++n) mbar_wait(&full[(n - k0) % R::STAGES], (n - k0) / R::STAGES & 1, 1 << 12);
-                    break;
-                }
+        } else {
+            const uint32_t ring0 = smem_addr(ring);
+            int i = k0;
+            for (; i < k1; ++i, next()) {
+                if (!mbar_wait(&full[s], parity)) { s_lost = 1; break; }
                 tmem_fence_after();
-                const uint32_t stage = smem_addr(ring + s * R::STAGE);
+                const uint32_t stage = ring0 + s * STAGE;
                 const uint64_t wd = operand_desc(stage), td = operand_desc(stage + BM * BK);
+                if (issuing) {
 #pragma unroll
-                for (int j = 0; j < BK / 32; ++j) mma_i8(acc, wd + 2 * j, td + 2 * j, i8_instruction(BM, BN), i > k0 || j > 0);
-                mma_commit(&empty[s]);
+                    for (int j = 0; j < BK / 32; ++j) mma_i8(acc, wd + 2 * j, td + 2 * j, i8_instruction(BM, BN), i > k0 || j > 0);
+                    mma_commit(&empty[s]);
+                }
+                __syncwarp();
             }
-            mma_commit(&done);
+            for (int n = 0; i < k1 && n < stages; ++i, ++n, next()) mbar_wait(&full[s], parity, 1 << 12);      // lost: copies still on their way must not outlive the CTA
+            if (issuing) mma_commit(&done);
         }
     }
     __syncwarp();
@@ -99,15 +109,16 @@ __global__ void __launch_bounds__(THREADS) int8_matmul_kernel(const __grid_const
 
     if (g.split == 1) {
         if (warp >= 2 && !lost) {
-            const int quarter = warp & 3, channel = channel0 + 32 * quarter + lane;
-            const float cs = channel < g.n ? g.b_scales[channel] : 0.0f, bias = g.bias && channel < g.n ? g.bias[channel] : 0.0f;
+            const int quarter = warp & 3, at = 32 * quarter + lane, channel = channel0 + at;
+            const bool there = at < g.height && channel < g.n;
+            const float cs = s_channel[at].x, bias = s_channel[at].y;
             for (int c = 0; c < BN && token0 + c < g.m; c += 16) {
                 int r[16];
                 tmem_load(acc + ((uint32_t)(32 * quarter) << 16) + c, r);
-                tmem_wait_load();
+                tmem_wait_load(r);
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    if (channel < g.n && token0 + c + i < g.m)
+                    if (there && token0 + c + i < g.m)
                         Elem<T>::store(out, (int64_t)(token0 + c + i) * g.out_pitch + channel, scaled(r[i], s_token[c + i], cs, bias));
             }
         }
@@ -119,22 +130,29 @@ __global__ void __launch_bounds__(THREADS) int8_matmul_kernel(const __grid_const
             for (int c = 0; c < BN; c += 16) {
                 int r[16];
                 tmem_load(acc + ((uint32_t)(32 * quarter) << 16) + c, r);
-                tmem_wait_load();
+                tmem_wait_load(r);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) part[(c + i) * BM + 32 * quarter + lane] = r[i];
             }
         }
         cluster_arrive_wait();
-        int c0 = BN * rank / g.split, c1 = BN * (rank + 1) / g.split;
+        const int there = min(BN, g.m - token0), c0 = there * rank / g.split, c1 = there * (rank + 1) / g.split;      // this CTA's columns
         bool any = false;
         for (int s = 0; s < g.split; ++s) any |= cluster_load_u32(&s_lost, s) != 0;
         if (!any)
-            for (int i = c0 * BM + t; i < c1 * BM; i += THREADS) {
-                const int token = token0 + i / BM, channel = channel0 + i % BM;
-                if (token >= g.m || channel >= g.n) continue;
-                int sum = 0;
-                for (int s = 0; s < g.split; ++s) sum += (int)cluster_load_u32(&part[i], s);
-                Elem<T>::store(out, (int64_t)token * g.out_pitch + channel, scaled(sum, s_token[i / BM], g.b_scales[channel], g.bias ? g.bias[channel] : 0.0f));
+            for (int i = c0 * (BM / 4) + t; i < c1 * (BM / 4); i += THREADS) {
+                const int column = i / (BM / 4), at = i % (BM / 4) * 4, channel = channel0 + at;
+                int4 p[8], sum = make_int4(0, 0, 0, 0);
+#pragma unroll
+                for (int s = 0; s < 8; ++s) if (s < g.split) p[s] = cluster_load_int4(&part[4 * i], s);
+#pragma unroll
+                for (int s = 0; s < 8; ++s) if (s < g.split) { sum.x += p[s].x; sum.y += p[s].y; sum.z += p[s].z; sum.w += p[s].w; }
+                const int sums[4] = {sum.x, sum.y, sum.z, sum.w};
+                T* o = out + (int64_t)(token0 + column) * g.out_pitch + channel;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (at + j < g.height && channel + j < g.n)
+                        Elem<T>::store(o, j, scaled(sums[j], s_token[column], s_channel[at + j].x, s_channel[at + j].y));
             }
         cluster_arrive_wait();
     }
@@ -144,9 +162,10 @@ __global__ void __launch_bounds__(THREADS) int8_matmul_kernel(const __grid_const
 }
 
 // The form for many tokens: two CTAs share a tile of 256 channels and up to 256 tokens, so a stage of the ring is 16 KB of weights and up to 16 KB of tokens
-// a CTA for twice the products, and they stay on their SMs: while eight warps take the sums of one tile out of tensor memory, the next tile's go into its other
+// a CTA for twice the products, and they stay on their SMs: while other warps take the sums of one tile out of tensor memory, the next tile's go into its other
 // half.  Tiles of the same channels follow one another: the weights come from HBM once.
-constexpr int PAIR_THREADS = 320, PAIR_STAGES = 6, PAIR_STAGE = 2 * BM * BK, PAIR_LIMIT = 1 << 18;
+constexpr int PAIR_SLICES = 2, PAIR_WARPS = 4 * PAIR_SLICES, PAIR_THREADS = 32 * (2 + PAIR_WARPS);
+constexpr int PAIR_STAGES = 6, PAIR_STAGE = 2 * BM * BK, PAIR_LIMIT = 1 << 18;
 constexpr int PAIR_BYTES = PAIR_STAGE * PAIR_STAGES + 1024;
 
 template <typename T>
@@ -161,7 +180,7 @@ __global__ void __launch_bounds__(PAIR_THREADS) int8_matmul_pair_kernel(const __
     const int steps = (g.k + BK - 1) / BK;
     if (t == 0) {
         for (int i = 0; i < PAIR_STAGES; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(&ready[i], 1); mbar_init(&taken[i], 16); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&ready[i], 1); mbar_init(&taken[i], 2 * PAIR_WARPS); }
         s_lost = 0;
     }
     if (warp == 1) tmem_alloc_pair(&s_tmem, 512);
@@ -171,76 +190,86 @@ __global__ void __launch_bounds__(PAIR_THREADS) int8_matmul_pair_kernel(const __
     tmem_fence_after();
     const uint32_t acc = s_tmem;
 
-    if (warp == 0) {
-        if (lane == 0) {
-            int n = 0;                              // stages filled so far
-            bool ok = true;
+    if (warp < 2) {
+        const bool issuing = elect_one();
+        int s = 0;
+        uint32_t parity = 0;
+        auto next = [&] { if (++s == PAIR_STAGES) { s = 0; parity ^= 1; } };
+        bool ok = true;
+        if (warp == 0) {
+            const uint32_t full0 = cluster_addr(&full[0], 0), bytes = (uint32_t)(2 * BM + tokens) * BK;       // both CTAs' bytes
+            int filled = 0;
             for (int tile = pair; ok && tile < tiles; tile += pairs) {
                 const int token0 = tile % g.token_tiles * tokens + rank * (tokens / 2), channel0 = tile / g.token_tiles * 2 * BM + rank * BM;
-                for (int i = 0; i < steps; ++i, ++n) {
-                    const int s = n % PAIR_STAGES, round = n / PAIR_STAGES;
-                    if (round > 0 && !mbar_wait_cluster(&empty[s], (round - 1) & 1, PAIR_LIMIT)) { ok = false; break; }
-                    unsigned char* stage = ring + s * PAIR_STAGE;
-                    const uint32_t bar = cluster_addr(&full[s], 0);
-                    if (rank == 0) mbar_arrive_expect_tx(&full[s], (uint32_t)(2 * BM + tokens) * BK);     // both CTAs' bytes
-                    tile_g2s_pair(stage, &map_b, i * BK, channel0, bar);
-                    tile_g2s_pair(stage + BM * BK, &map_a, i * BK, token0, bar);
+                for (int i = 0; i < steps; ++i, next()) {
+                    if (filled == PAIR_STAGES) {
+                        if (!mbar_wait(&empty[s], parity ^ 1, PAIR_LIMIT)) { ok = false; break; }
+                    } else {
+                        ++filled;
+                    }
+                    if (issuing) {
+                        unsigned char* stage = ring + s * PAIR_STAGE;
+                        const uint32_t bar = full0 + 8 * s;
+                        if (rank == 0) mbar_arrive_expect_tx(&full[s], bytes);
+                        tile_g2s_pair(stage, &map_b, i * BK, channel0, bar);
+                        tile_g2s_pair(stage + BM * BK, &map_a, i * BK, token0, bar);
+                    }
+                    __syncwarp();
                 }
             }
-            if (!ok) atomicExch(&s_lost, 1);
-        }
-    } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
-            const uint32_t instruction = i8_instruction(2 * BM, tokens);
-            int n = 0, done = 0;                    // stages, tiles
-            bool ok = true;
+        } else if (rank == 0) {
+            const uint32_t instruction = i8_instruction(2 * BM, tokens), ring0 = smem_addr(ring);
+            int done = 0;                           // tiles
             for (int tile = pair; ok && tile < tiles; tile += pairs, ++done) {
                 const uint32_t d = acc + (done & 1) * 256;
-                if (done >= 2 && !mbar_wait_cluster(&taken[done & 1], (done / 2 - 1) & 1, PAIR_LIMIT)) { ok = false; break; }
+                if (done >= 2 && !mbar_wait(&taken[done & 1], (done / 2 - 1) & 1, PAIR_LIMIT)) { ok = false; break; }
                 tmem_fence_after();
-                for (int i = 0; i < steps; ++i, ++n) {
-                    const int s = n % PAIR_STAGES, round = n / PAIR_STAGES;
-                    if (!mbar_wait_cluster(&full[s], round & 1, PAIR_LIMIT)) { ok = false; break; }
+                for (int i = 0; i < steps; ++i, next()) {
+                    if (!mbar_wait(&full[s], parity, PAIR_LIMIT)) { ok = false; break; }
                     tmem_fence_after();
-                    const uint32_t stage = smem_addr(ring + s * PAIR_STAGE);
+                    const uint32_t stage = ring0 + s * PAIR_STAGE;
                     const uint64_t wd = operand_desc(stage), td = operand_desc(stage + BM * BK);
+                    if (issuing) {
 #pragma unroll
-                    for (int j = 0; j < BK / 32; ++j) mma_i8_pair(d, wd + 2 * j, td + 2 * j, instruction, i > 0 || j > 0);
-                    mma_commit_pair(&empty[s]);
+                        for (int j = 0; j < BK / 32; ++j) mma_i8_pair(d, wd + 2 * j, td + 2 * j, instruction, i > 0 || j > 0);
+                        mma_commit_pair(&empty[s]);
+                    }
+                    __syncwarp();
                 }
-                if (ok) mma_commit_pair(&ready[done & 1]);
+                if (ok && issuing) mma_commit_pair(&ready[done & 1]);
+                __syncwarp();
             }
-            if (!ok) {                              // copies that may still be on their way must not outlive the CTAs
-                atomicExch(&s_lost, 1);
-                for (int i = 0; i < PAIR_STAGES; ++i, ++n) mbar_wait_cluster(&full[n % PAIR_STAGES], n / PAIR_STAGES & 1, 1 << 10);
-            }
+            if (!ok)                                // copies that may still be on their way must not outlive the CTAs
+                for (int i = 0; i < PAIR_STAGES; ++i, next()) mbar_wait(&full[s], parity, 1 << 10);
         }
+        if (!ok) s_lost = 1;
     } else {
-        // 32 channels and every other group of 32 tokens a warp
-        const int quarter = warp & 3, half = (warp - 2) >> 2, groups = tokens / 32;
+        // 32 channels and every fourth group of 32 tokens a warp
+        constexpr int S = PAIR_SLICES, PER = 8 / S;
+        const int quarter = warp & 3, slice = (warp - 2) >> 2, groups = tokens / 32;
         int done = 0;
         for (int tile = pair; tile < tiles; tile += pairs, ++done) {
             const int token0 = tile % g.token_tiles * tokens, channel = tile / g.token_tiles * 2 * BM + rank * BM + 32 * quarter + lane;
             const bool there = channel < g.n;
             const float cs = there ? g.b_scales[channel] : 0.0f, bias = g.bias && there ? g.bias[channel] : 0.0f;
-            float scale[4];                         // of the tokens of this warp's groups, one a lane
+            float scale[PER];                         // of the tokens of this warp's groups, one a lane
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int token = token0 + (2 * j + half) * 32 + lane;
-                scale[j] = 2 * j + half < groups && token < g.m ? g.a_scales[token] : 0.0f;
+            for (int j = 0; j < PER; ++j) {
+                const int token = token0 + (S * j + slice) * 32 + lane;
+                scale[j] = S * j + slice < groups && token < g.m ? g.a_scales[token] : 0.0f;
             }
-            if (!mbar_wait_cluster(&ready[done & 1], done / 2 & 1, PAIR_LIMIT)) { if (lane == 0) atomicExch(&s_lost, 1); break; }
+            if (!mbar_wait(&ready[done & 1], done / 2 & 1, PAIR_LIMIT)) { if (lane == 0) atomicExch(&s_lost, 1); break; }
             tmem_fence_after();
             const uint32_t from = acc + ((uint32_t)(32 * quarter) << 16) + (done & 1) * 256;
-            if (half >= groups && lane == 0) mbar_arrive_cluster(cluster_addr(&taken[done & 1], 0));
+            if (slice >= groups && lane == 0) mbar_arrive_cluster(cluster_addr(&taken[done & 1], 0));
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int group = 2 * j + half;
+            for (int j = 0; j < PER; ++j) {
+                const int group = S * j + slice;
                 if (group >= groups) break;
                 int r[32];
                 tmem_load(from + 32 * group, r);
-                tmem_wait_load();
-                if (group + 2 >= groups) {          // the warp's sums of the tile are in registers
+                tmem_wait_load(r);
+                if (group + S >= groups) {          // the warp's sums of the tile are in registers
                     tmem_fence_before();
                     if (lane == 0) mbar_arrive_cluster(cluster_addr(&taken[done & 1], 0));
                 }
@@ -344,21 +373,42 @@ static int make_map(CUtensorMap* map, const int8_t* p, int64_t rows, int64_t k, 
     return MAB_OK;
 }
 
+// Tiles of at most 128 channels for all tokens; where those are fewer than the SMs, the inner size split over 2, 4 or 8 CTAs.  The height of the tiles and the split
+// are those by which the SM with the most has the least to load.
 template <typename T, int BN> int launch_tiles(Args g, int sms, cudaStream_t s) {
+    const int steps = (g.k + BK - 1) / BK;
+    g.token_tiles = (g.m + BN - 1) / BN;
+    int64_t best = INT64_MAX;
+    for (int split = 1; split <= 8 && (split == 1 || steps >= 2 * split); split *= 2)
+        for (int height = BM; height >= 64; height -= 8) {
+            const int64_t tiles = (int64_t)g.token_tiles * ceil_div64(g.n, height);
+            const int64_t load = ceil_div64(tiles * split, split > 2 ? sms - sms / 8 : sms) * ((int64_t)ceil_div64(steps, split) * (height + BN) + 128 * (split > 1));
+            if (load < best) { best = load; g.split = split; g.height = height; }
+        }
+    const int64_t ctas = (int64_t)g.token_tiles * ceil_div64(g.n, g.height) * g.split;
+    const int stage = (BM + BN) * BK, most = (ctas > sms ? RING_TWO : RING_ONE) / stage;
+    const int sums = g.split > 1 ? BM * BN * 4 : 0;                        // the partial sums have to fit the ring
+    g.stages = std::max({1, std::min({most, MOST_STAGES, (steps + g.split - 1) / g.split}), (sums + stage - 1) / stage});
     CUtensorMap map_a, map_b;
     if (int rc = make_map(&map_a, g.a, g.m, g.k, g.a_pitch, BN)) return rc;
-    if (int rc = make_map(&map_b, g.b, g.n, g.k, g.b_pitch, BM)) return rc;
-    g.token_tiles = (g.m + BN - 1) / BN;
-    const int64_t tiles = (int64_t)g.token_tiles * ((g.n + BM - 1) / BM);
-    const int steps = (g.k + BK - 1) / BK;
-    g.split = 1;
-    while (g.split < 8 && tiles * g.split * 2 <= sms && steps >= 4 * g.split) g.split *= 2;
-    return launch_rows(int8_matmul_kernel<T, BN>, "int8_matmul", tiles * g.split, THREADS, Ring<BN>::BYTES, g.split, s, map_a, map_b, g);
+    if (int rc = make_map(&map_b, g.b, g.n, g.k, g.b_pitch, g.height)) return rc;
+    return launch_rows(int8_matmul_kernel<T, BN>, "int8_matmul", ctas, THREADS, (size_t)stage * g.stages + 1024, g.split, s, map_a, map_b, g);
 }
 
-// Tiles of 256 channels and as few tokens as cover them all evenly (a multiple of 32).
+// Tiles of 256 channels and a multiple of 32 tokens, as many tokens as give the shortest time: a step of the inner size takes tokens x 2 cycles of products or
+// the loading of 16 KB of weights and the tokens at some 50 bytes a cycle, whichever is more; the epilogue is seen once, after the last tile.
 template <typename T> int launch_pairs(Args g, int sms, cudaStream_t s) {
-    const int parts = (g.m + 255) / 256, tokens = ((g.m + parts - 1) / parts + 31) / 32 * 32;
+    const int steps = (g.k + BK - 1) / BK, channel_tiles = (g.n + 2 * BM - 1) / (2 * BM);
+    int tokens = 256;
+    double best = 1e300;
+    for (int parts = (g.m + 255) / 256, n = 0; n < 8; ++n, ++parts) {
+        const int each = ((g.m + parts - 1) / parts + 31) / 32 * 32;
+        const double waves = (double)ceil_div64((int64_t)ceil_div64(g.m, each) * channel_tiles, sms / 2);
+        const double step = std::max(2.0 * each, (BM + each / 2) * BK / 50.0), epilogue = 2500 + 24.0 * each;
+        const double time = waves * std::max(steps * step, epilogue) + epilogue;
+        if (time < best * 0.98) { best = time; tokens = each; }
+        if (each == 32) break;
+    }
     CUtensorMap map_a, map_b;
     if (int rc = make_map(&map_a, g.a, g.m, g.k, g.a_pitch, tokens / 2)) return rc;
     if (int rc = make_map(&map_b, g.b, g.n, g.k, g.b_pitch, BM)) return rc;
@@ -368,21 +418,23 @@ template <typename T> int launch_pairs(Args g, int sms, cudaStream_t s) {
     return launch_rows(int8_matmul_pair_kernel<T>, "int8_matmul", pairs * 2, PAIR_THREADS, PAIR_BYTES, 2, s, map_a, map_b, g, tokens, (int)tiles);
 }
 
+#ifndef ROWS_MOST
+#define ROWS_MOST 4
+#endif
 template <typename T> int launch(const Args& g, cudaStream_t s) {
     const int sms = device_sm_count();
     if (sms < 0) return MAB_ERR_CUDA;
-    if (g.m <= 4) {
+    if (g.m <= ROWS_MOST) {
         const int64_t ctas = ceil_div64(g.n, 16);
         if (g.m == 1) return launch_rows(int8_rows_kernel<T, 1, 2>, "int8_matmul", ctas, 256, 0, 1, s, g);
         if (g.m == 2) return launch_rows(int8_rows_kernel<T, 2, 2>, "int8_matmul", ctas, 256, 0, 1, s, g);
-        return launch_rows(int8_rows_kernel<T, 4, 2>, "int8_matmul", ctas, 256, 0, 1, s, g);
+        if (g.m <= 4) return launch_rows(int8_rows_kernel<T, 4, 2>, "int8_matmul", ctas, 256, 0, 1, s, g);
+        return launch_rows(int8_rows_kernel<T, 8, 2>, "int8_matmul", ctas, 256, 0, 1, s, g);
     }
-    if (g.m > 64 && ceil_div64(g.m, 256) * ceil_div64(g.n, 2 * BM) * 4 >= sms) return launch_pairs<T>(g, sms, s);
+    if (g.m > 64) return launch_pairs<T>(g, sms, s);
     if (g.m <= 16) return launch_tiles<T, 16>(g, sms, s);
     if (g.m <= 32) return launch_tiles<T, 32>(g, sms, s);
-    if (g.m <= 64) return launch_tiles<T, 64>(g, sms, s);
-    if (g.m <= 128) return launch_tiles<T, 128>(g, sms, s);
-    return launch_tiles<T, 256>(g, sms, s);
+    return launch_tiles<T, 64>(g, sms, s);
 }
 
 }  // namespace int8mm
@@ -412,6 +464,6 @@ extern "C" int mab_int8_matmul(int64_t m, int64_t n, int64_t k, const int8_t* a,
                 "mab_int8_matmul: codes have to start on 16 bytes, their rows a multiple of 16 apart (%lld, %lld)", (long long)a_pitch, (long long)b_pitch);
     MAB_REQUIRE(aligned_to(a_scales, 4) && aligned_to(b_scales, 4) && aligned_to(bias, 4) && aligned_to(out, out_dtype == MAB_F32 ? 4 : 2),
                 MAB_ERR_BAD_ARG, "mab_int8_matmul: misaligned buffer");
-    int8mm::Args g = {a, b, a_pitch, b_pitch, out_pitch, a_scales, b_scales, bias, out, (int)m, (int)n, (int)k, 1, 1};
+    int8mm::Args g = {a, b, a_pitch, b_pitch, out_pitch, a_scales, b_scales, bias, out, (int)m, (int)n, (int)k, 1, 1, 1, int8mm::BM};
     return out_dtype == MAB_F32 ? int8mm::launch<float>(g, (cudaStream_t)stream) : int8mm::launch<uint16_t>(g, (cudaStream_t)stream);
 }

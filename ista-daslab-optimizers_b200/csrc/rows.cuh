@@ -128,6 +128,11 @@ __device__ __forceinline__ uint32_t cluster_load_u32(const void* p, int rank) {
     asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(cluster_addr(p, rank)) : "memory");
     return v;
 }
+__device__ __forceinline__ int4 cluster_load_int4(const void* p, int rank) {
+    int4 v;
+    asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(cluster_addr(p, rank)) : "memory");
+    return v;
+}
 __device__ __forceinline__ unsigned long long cluster_load_u64(const void* p, int rank) {
     unsigned long long v;
     asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(cluster_addr(p, rank)) : "memory");

@@ -5,6 +5,14 @@
 
 namespace mab {
 
+// One lane of a whole warp.  The loops around copies and products are run by the whole warp and only the issuing is this lane's: what those instructions take comes
+// from registers that a warp shares, and where a single lane runs the loop each of them costs some 100 cycles more (a step of the inner size 0.36 us against 0.19).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred P;\n\telect.sync _|P, 0xffffffff;\n\tselp.u32 %0, 1, 0, P;\n\t}" : "=r"(p));
+    return p != 0;
+}
+
 __device__ __forceinline__ void tmem_alloc(uint32_t* to_smem, uint32_t columns) {       // a whole warp; columns: a power of two, at least 32
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(to_smem)), "r"(columns) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
@@ -46,7 +54,12 @@ __device__ __forceinline__ void tmem_load(uint32_t at, int (&r)[32]) {
                    "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
                    "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]) : "r"(at));
 }
-__device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// Loads are asynchronous: their registers pass through the wait, so that nothing is computed from them before it.
+template <int N> __device__ __forceinline__ void tmem_wait_load(int (&r)[N]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
+}
 
 // ---- two CTAs of a cluster with one tile (cta_group::2): the even one's thread issues for both; operands lie at the same place in either's shared memory
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t* to_smem, uint32_t columns) {
@@ -70,19 +83,10 @@ __device__ __forceinline__ void tile_g2s_pair(void* dst, const CUtensorMap* map,
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];"
                  ::"r"(smem_addr(dst)), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
 }
+// An arrival at a barrier of either CTA.  It says that this thread's reads of tensor memory are done (they are complete after their wait), not that its stores
+// are: a release over the cluster would wait for every one of them.
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-// A bounded wait that also sees what the other CTA did before its arrival.
-__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, int limit) {
-    const uint32_t a = smem_addr(bar);
-    for (int it = 0; it < limit; ++it) {
-        uint32_t done;
-        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                     : "=r"(done) : "r"(a), "r"(parity) : "memory");
-        if (done) return true;
-    }
-    return false;
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 // A box of the tensor map at (x, y) into shared memory; x in bytes, a multiple of 16.
