@@ -59,6 +59,11 @@ __device__ __forceinline__ void prefetch_l2(uintptr_t base, int64_t bytes) {
         asm volatile("prefetch.global.L2 [%0];" ::"l"(first + ((uintptr_t)i << 7)));
 }
 
+// The same for one run of `bytes` (address and size multiples of 16), by one thread.
+__device__ __forceinline__ void prefetch_bulk_l2(const void* p, uint32_t bytes) {
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
+}
+
 __device__ __forceinline__ void cp_async_4(void* dst_smem, const void* src_gmem) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_addr(dst_smem)), "l"(src_gmem) : "memory");
 }

@@ -56,14 +56,15 @@ extern "C" const char* mab_last_error(void) { return g_error; }
 extern "C" int64_t mab_kernel_launch_count(void) { return g_launches.load(std::memory_order_relaxed); }
 
 extern "C" int mab_device_error(void) {
-    int a = 0, b = 0, c = 0, d = 0, e = 0, f = 0;
+    int a = 0, b = 0, c = 0, d = 0, e = 0, f = 0, g = 0;
     if (int rc = copy_timeout_f32(&a, false)) return rc;
     if (int rc = copy_timeout_f32_split(&d, false)) return rc;
     if (int rc = copy_timeout_bf16(&b, false)) return rc;
     if (int rc = copy_timeout_bf16_warps(&e, false)) return rc;
     if (int rc = copy_timeout_window(&c, false)) return rc;
     if (int rc = copy_timeout_int8_matmul(&f, false)) return rc;
-    return (a | b | c | d | e | f) ? 1 : 0;
+    if (int rc = copy_timeout_distill(&g, false)) return rc;
+    return (a | b | c | d | e | f | g) ? 1 : 0;
 }
 
 extern "C" int mab_device_error_clear(void) {
@@ -73,6 +74,7 @@ extern "C" int mab_device_error_clear(void) {
     if (int rc = copy_timeout_bf16(&v, true)) return rc;
     if (int rc = copy_timeout_bf16_warps(&v, true)) return rc;
     if (int rc = copy_timeout_int8_matmul(&v, true)) return rc;
+    if (int rc = copy_timeout_distill(&v, true)) return rc;
     return copy_timeout_window(&v, true);
 }
 

@@ -7,20 +7,25 @@
 //   tau dloss/dz_v = P q_v - sum_{j: index_j = v} p_j              for v in the list
 //                  = exp(y_v - L_t) (P q_t - p_t)                  elsewhere
 //
-// One pass over a row with a running maximum and sum, in which a bitmap in shared memory leaves out the positions of the list: the
-// sum over the others is their own, not a difference of two large ones.  The k terms of the list are in 64 bits: near the optimum the loss is what is
-// left of a difference, and there an error of S_t only enters with the factor q_t - p_t as long as the terms that share it are exact.
-//
-// A row belongs to a cluster of one to eight CTAs (few rows: more CTAs a row), which exchange six numbers through distributed shared
-// memory in rank order: results do not depend on timing.
+// A row belongs to a cluster of one to eight CTAs, each of which has its part of the row in shared memory from the beginning to the end (a bulk copy, on its way while
+// the list is worked on): one pass with a running maximum and sum, and for the gradient a second one that reads no global memory.  The list's positions are
+// overwritten by -inf there, so the sum over the others is their own, not a difference of two large ones.  The k terms of the list are in 64 bits: near the
+// optimum the loss is what is left of a difference, and there an error of S_t only enters with the factor q_t - p_t as long as the terms that share it are exact.
+// Rows too long for that are read twice, with a bitmap of the list's positions.  The CTAs exchange five numbers through distributed shared memory, in rank order:
+// results do not depend on timing.
 #include "rows.cuh"
+#include "async_copy.cuh"
 
 namespace mab {
 namespace distill {
 
-constexpr int NT = 512, WARPS = NT / 32;
-constexpr int MAX_K = 1024, PER_THREAD = MAX_K / NT;
+constexpr int GRAD_NT = 512, MOST_WARPS = 16;
+constexpr int MAX_K = 1024;
 constexpr int UNROLL = 4;                          // vectors of 16 bytes a thread has in flight
+constexpr int PART = 66 * 1024;                    // bytes of a row's part with which three CTAs share an SM
+constexpr int STEP_SHARED = 108 * 1024;            // ... of shared memory with which two do
+constexpr int AHEAD = 64 * 1024;                  // bytes of a row asked into L2 before the list is worked on
+__device__ int g_timeout;
 enum Mode { LOSS, STEP };
 
 struct Args {
@@ -31,7 +36,7 @@ struct Args {
     int values_bf16;
     const float* rest;
     const float* weights;
-    double tau;
+    double inv_tau;                                // 1 / tau
     float scale;                                   // log2(e) / tau
     float* loss;
     float2* stats;                                 // per row: reference, factor of the positions outside the list (LOSS)
@@ -40,16 +45,17 @@ struct Args {
     int64_t grad_pitch;
     const float* grad_loss;                        // GRAD: [rows], `grad_loss_stride` apart
     int64_t grad_loss_stride;
-    int vocab, k, cluster;
+    int vocab, k, cluster, held;
 };
 
 struct Shared {
-    double red[WARPS][3];
-    double out[3];                                 // sums over the block
+    uint64_t bar;
+    double red[MOST_WARPS][3];
     double part[5];                                // this CTA's part, read by the cluster: reference, S_t, m_k, S_k, B
-    double stat[4];                                // Lp, 1 / Sp, L, P
-    float fmax[WARPS][2], fsum[WARPS];
+    double inv, L, P;
+    float max_t[MOST_WARPS], max_k[MOST_WARPS], ref_w[MOST_WARPS], sum_w[MOST_WARPS];
     float ref, off;
+    uint32_t edge[2];                              // the list's positions in the first and the last, partial vector
     int dup;
 };
 
@@ -57,54 +63,75 @@ __device__ __forceinline__ double list_value(const Args& a, int64_t at) {
     return a.values_bf16 ? (double)bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(a.values)[at]) : (double)reinterpret_cast<const float*>(a.values)[at];
 }
 
-// Sums of three doubles over the block, in every thread.
-__device__ __forceinline__ void block_sum(Shared& sh, double& x, double& y, double& z) {
+// Sums of three doubles over the first `warps` warps, in every thread.
+__device__ __forceinline__ void block_sum(Shared& sh, int warps, double& x, double& y, double& z) {
+    if (warp_id() < warps) {
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        x += __shfl_xor_sync(0xffffffffu, x, o);
-        y += __shfl_xor_sync(0xffffffffu, y, o);
-        z += __shfl_xor_sync(0xffffffffu, z, o);
+        for (int o = 16; o; o >>= 1) {
+            x += __shfl_xor_sync(0xffffffffu, x, o);
+            y += __shfl_xor_sync(0xffffffffu, y, o);
+            z += __shfl_xor_sync(0xffffffffu, z, o);
+        }
+        if (lane_id() == 0) { sh.red[warp_id()][0] = x; sh.red[warp_id()][1] = y; sh.red[warp_id()][2] = z; }
     }
-    if (lane_id() == 0) { sh.red[warp_id()][0] = x; sh.red[warp_id()][1] = y; sh.red[warp_id()][2] = z; }
     __syncthreads();
     x = y = z = 0.0;
-    for (int w = 0; w < WARPS; ++w) { x += sh.red[w][0]; y += sh.red[w][1]; z += sh.red[w][2]; }
+    for (int w = 0; w < warps; ++w) { x += sh.red[w][0]; y += sh.red[w][1]; z += sh.red[w][2]; }
 }
 
-// Writes factor * exp2((z - ref) scale) over the vectors [v0, v1) of the row.
-template <typename T>
-__device__ __forceinline__ void write_outside(const RowGrid<T>& g, int v0, int v1, T* out, float ref, float scale, float factor) {
+// factor * exp2((x - ref) scale) of a vector.
+template <typename T, int N> __device__ __forceinline__ uint4 outside(uint4 r, uint64_t ref2, uint64_t scale2, uint64_t factor2) {
+    uint64_t x[N / 2];
+    unpack_pairs(r, x, (const T*)nullptr);
+    float y[N];
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+        float lo, hi;
+        split(mul2(add2(x[i], ref2), scale2), lo, hi);
+        split(mul2(pair_of(ex2(lo), ex2(hi)), factor2), y[2 * i], y[2 * i + 1]);
+    }
+    return pack(y, (const T*)nullptr);
+}
+
+// Writes that over the vectors [v0, v1) of the row; `load(v)` gives the whole ones.
+template <typename T, int THREADS, typename F>
+__device__ __forceinline__ void write_outside(const RowGrid<T>& g, int v0, int v1, T* out, float ref, float scale, float factor, F load) {
     constexpr int N = RowGrid<T>::N;
     const bool same = ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(g.p)) & 15) == 0;
-    auto put = [&](int v, float (&x)[N], bool vector) {
+    const uint64_t ref2 = pair_of(-ref, -ref), scale2 = pair_of(scale, scale), factor2 = pair_of(factor, factor);
+    auto put = [&](int v, uint4 r) {
+        r = outside<T, N>(r, ref2, scale2, factor2);
+        if (same) { __stcs(reinterpret_cast<uint4*>(out + g.first(v)), r); return; }
+        float x[N];
+        unpack(r, x, (const T*)nullptr);
 #pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = factor * ex2((x[i] - ref) * scale);
-        if (vector) *reinterpret_cast<uint4*>(out + g.first(v)) = pack(x, (const T*)nullptr);
-        else
-#pragma unroll
-            for (int i = 0; i < N; ++i) if (g.first(v) + i >= 0 && g.first(v) + i < g.n) Elem<T>::store(out, g.first(v) + i, x[i]);
+        for (int i = 0; i < N; ++i) Elem<T>::store(out, g.first(v) + i, x[i]);
     };
     const int w0 = g.whole_from(v0), w1 = g.whole_to(v1);
     int v = w0 + threadIdx.x;
-    for (; v + (UNROLL - 1) * NT < w1; v += UNROLL * NT) {
+    for (; v + (UNROLL - 1) * THREADS < w1; v += UNROLL * THREADS) {
         uint4 r[UNROLL];
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) r[u] = g.load(v + u * NT);
+        for (int u = 0; u < UNROLL; ++u) r[u] = load(v + u * THREADS);
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) { float x[N]; unpack(r[u], x, (const T*)nullptr); put(v + u * NT, x, same); }
+        for (int u = 0; u < UNROLL; ++u) put(v + u * THREADS, r[u]);
     }
-    for (; v < w1; v += NT) { float x[N]; unpack(g.load(v), x, (const T*)nullptr); put(v, x, same); }
+    for (; v < w1; v += THREADS) put(v, load(v));
     if (threadIdx.x < 2) {                          // the partial vectors
         const int pv = threadIdx.x == 0 ? 0 : g.count - 1;
-        if (pv >= v0 && pv < v1 && !g.whole(pv) && (threadIdx.x == 0 || g.count > 1)) { float x[N]; g.load_part(pv, x, 0.0f); put(pv, x, false); }
+        if (pv >= v0 && pv < v1 && !g.whole(pv) && (threadIdx.x == 0 || g.count > 1))
+            for (int i = 0; i < N; ++i) {
+                const int e = g.first(pv) + i;
+                if (e >= 0 && e < g.n) Elem<T>::store(out, e, factor * ex2((Elem<T>::load(g.p, e) - ref) * scale));
+            }
     }
 }
 
 // Zeros over the vectors [v0, v1) of a row.
-template <typename T>
+template <typename T, int THREADS>
 __device__ __forceinline__ void write_zeros(T* row, int n, int v0, int v1) {
     const RowGrid<T> o(row, n);
-    for (int v = v0 + threadIdx.x; v < v1 && v < o.count; v += NT) {
+    for (int v = v0 + threadIdx.x; v < v1 && v < o.count; v += THREADS) {
         if (o.whole(v)) *reinterpret_cast<uint4*>(row + o.first(v)) = make_uint4(0, 0, 0, 0);
         else
 #pragma unroll
@@ -120,258 +147,381 @@ __device__ __forceinline__ void part_of(int count, int part, int parts, int& v0,
 }
 
 // A row whose weight is zero: zeros in this CTA's part.
-template <typename T>
+template <typename T, int THREADS>
 __device__ __forceinline__ void zero_part(const Args& a, int64_t row, int part, int parts) {
     T* out = reinterpret_cast<T*>(a.grad) + row * a.grad_pitch;
     const RowGrid<T> o(out, a.vocab);
     int v0, v1;
     part_of(o.count, part, parts, v0, v1);
-    write_zeros(out, a.vocab, v0, v1);
+    write_zeros<T, THREADS>(out, a.vocab, v0, v1);
 }
 
-template <typename T, int MODE>
-__global__ void __launch_bounds__(NT, 2) distill_kernel(Args a) {
-    constexpr int N = RowGrid<T>::N;
+// RESIDENT: the part of the row is in shared memory; otherwise only its first `a.held` whole vectors are.
+template <typename T, int MODE, bool RESIDENT, int NT>
+__global__ void __launch_bounds__(NT, 1024 / NT) distill_kernel(Args a) {
+    constexpr int N = RowGrid<T>::N, WARPS = NT / 32, PER_THREAD = MAX_K / NT;
     extern __shared__ __align__(16) unsigned char dyn[];
     __shared__ Shared sh;
-    const int C = a.cluster, rank = C > 1 ? (int)(blockIdx.x % C) : 0, t = threadIdx.x;
+    const int C = a.cluster, rank = C > 1 ? (int)(blockIdx.x % C) : 0, t = threadIdx.x, k = a.k;
     const int64_t row = blockIdx.x / C;
     const float w = a.weights ? a.weights[row] : 1.0f;
     if (w == 0.0f) {                                // the row's logits are not looked at
         if (rank == 0 && t == 0) a.loss[row] = 0.0f;
-        if (MODE == STEP) zero_part<T>(a, row, rank, C);
+        if (MODE == STEP) zero_part<T, NT>(a, row, rank, C);
         return;
     }
     const RowGrid<T> g(reinterpret_cast<const T*>(a.logits) + row * a.pitch, a.vocab);
     int v0, v1;
     part_of(g.count, rank, C, v0, v1);
+    const int w0 = g.whole_from(v0), w1 = max(w0, g.whole_to(v1));
     const int e0 = max(g.first(v0), 0), e1 = min(g.first(v1), a.vocab), base = g.first(v0);     // elements of this CTA; bit 0 of the bitmap
-    double* s_e = reinterpret_cast<double*>(dyn);                      // [k] exp(t_j - M), then p_j
-    int* s_idx = reinterpret_cast<int*>(s_e + a.k);                    // [k]
-    uint32_t* bitmap = reinterpret_cast<uint32_t*>(s_idx + (a.k + 1) / 2 * 2);
-    const int words = ((v1 - v0) * N + 31) / 32;
-    for (int i = t; i < words; i += NT) bitmap[i] = 0;
-    if (t == 0) sh.dup = 0;
-
+    const int f0 = g.first(w0), f1 = g.first(w1);                      // elements of its whole vectors
+    double* s_e = reinterpret_cast<double*>(dyn);                      // [k] exp(t_j - M)
+    int* s_idx = reinterpret_cast<int*>(s_e + k);                      // [k]
+    uint4* part = reinterpret_cast<uint4*>(dyn + ((size_t)k * 12 + 15) / 16 * 16);               // the vectors that are held
+    const int held = RESIDENT ? w1 - w0 : min(a.held, w1 - w0), h1 = w0 + held;
+    uint32_t* bitmap = reinterpret_cast<uint32_t*>(part + (RESIDENT ? 0 : a.held));              // of the list's positions, where not everything is held
     // the list
     int idx[PER_THREAD];
     double tj[PER_THREAD], yj[PER_THREAD];
+#pragma unroll
+    for (int i = 0; i < PER_THREAD; ++i) {
+        if (i * NT >= k) break;
+        const bool there = t + i * NT < k;
+        idx[i] = there ? a.indices[row * k + t + i * NT] : -1;
+        tj[i] = there ? list_value(a, row * k + t + i * NT) * a.inv_tau : 0.0;
+    }
+    const double rest = a.rest ? (double)a.rest[row] : -(double)INF_F;
+    // (the loads above are on their way)
+    if (t == 0) {
+        mbar_init(&sh.bar, 1);
+        mbar_arrive_expect_tx(&sh.bar, (uint32_t)held * 16);
+        if (held > 0) bulk_g2s(part, g.p + f0, (uint32_t)held * 16, &sh.bar);
+        if (!RESIDENT && w1 > h1) prefetch_bulk_l2(g.p + g.first(h1), (uint32_t)min((w1 - h1) * 16, AHEAD));   // on its way while the list is worked on
+    }
+    if (!RESIDENT)
+        for (int i = t; i < ((v1 - v0) * N + 31) / 32; i += NT) bitmap[i] = 0;
+    if (t == 0) { sh.dup = 0; sh.edge[0] = sh.edge[1] = 0; }
+
     float mt = -INF_F, mk = -INF_F;                 // largest t, largest y of this CTA's entries: as floats, only references
 #pragma unroll
     for (int i = 0; i < PER_THREAD; ++i) {
-        const int j = t + i * NT;
-        idx[i] = -1;
-        tj[i] = yj[i] = 0.0;
-        if (j < a.k) {
-            idx[i] = a.indices[row * a.k + j];
-            if (idx[i] < 0 || idx[i] >= a.vocab) idx[i] = -1;
-            s_idx[j] = idx[i];
-            if (idx[i] >= 0) {
-                tj[i] = list_value(a, row * a.k + j) / a.tau;
-                mt = fmaxf(mt, (float)tj[i]);
-                if (idx[i] >= e0 && idx[i] < e1) {
-                    yj[i] = (double)Elem<T>::load(g.p, idx[i]) / a.tau;
-                    mk = fmaxf(mk, (float)yj[i]);
-                }
-            }
-        }
+        if (i * NT >= k) break;
+        if (idx[i] < 0 || idx[i] >= a.vocab) idx[i] = -1;
+        const bool own = idx[i] >= e0 && idx[i] < e1;
+        const float z = own ? Elem<T>::load(g.p, idx[i]) : 0.0f;
+        if (t + i * NT < k) s_idx[t + i * NT] = idx[i];
+        if (idx[i] >= 0) mt = fmaxf(mt, (float)tj[i]);
+        yj[i] = (double)z * a.inv_tau;
+        if (own) mk = fmaxf(mk, (float)yj[i]);
     }
-    const double rest = a.rest ? (double)a.rest[row] : -(double)INF_F;
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
         mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, o));
         mk = fmaxf(mk, __shfl_xor_sync(0xffffffffu, mk, o));
     }
-    if (lane_id() == 0) { sh.fmax[warp_id()][0] = mt; sh.fmax[warp_id()][1] = mk; }
-    __syncthreads();                                // (the bitmap is clear, too)
-    mt = mk = -INF_F;
-    for (int i = 0; i < WARPS; ++i) { mt = fmaxf(mt, sh.fmax[i][0]); mk = fmaxf(mk, sh.fmax[i][1]); }
-    mt = fmaxf(mt, (float)rest);
+    if (lane_id() == 0) { sh.max_t[warp_id()] = mt; sh.max_k[warp_id()] = mk; }
+    __syncthreads();                                // (the barrier of the copy is there, or the bitmap is clear, too)
+    mt = (float)rest;
+    mk = -INF_F;
+#pragma unroll
+    for (int i = 0; i < WARPS; ++i) { mt = fmaxf(mt, sh.max_t[i]); mk = fmaxf(mk, sh.max_k[i]); }
     const double M = mt == -INF_F ? 0.0 : (double)mt, Mk = mk == -INF_F ? 0.0 : (double)mk;
-    double sum_p = 0.0, sum_k = 0.0, cross = 0.0;
+    double sum_p = 0.0, sum_k = 0.0, cross = 0.0, ek[PER_THREAD];
 #pragma unroll
     for (int i = 0; i < PER_THREAD; ++i) {
+        if (i * NT >= k) break;
         const int j = t + i * NT;
-        if (j >= a.k) continue;
+        ek[i] = 0.0;
+        if (j >= k) continue;
         const double e = idx[i] >= 0 ? exp(tj[i] - M) : 0.0;
         s_e[j] = e;
         sum_p += e;
         if (idx[i] >= e0 && idx[i] < e1) {
-            const int bit = idx[i] - base;
-            const uint32_t was = atomicOr(&bitmap[bit >> 5], 1u << (bit & 31));
-            if (was >> (bit & 31) & 1u) sh.dup = 1;
-            else sum_k += exp(yj[i] - Mk);
+            ek[i] = exp(yj[i] - Mk);
             if (!(e == 0.0)) cross += e * (tj[i] - yj[i]);
         }
     }
-    block_sum(sh, sum_p, sum_k, cross);             // (its barrier: the bitmap is complete)
     const double e_rest = rest == -(double)INF_F ? 0.0 : exp(rest - M);
+    bool lost = false;
+    auto arrived = [&] {
+        lost = !mbar_wait(&sh.bar, 0);
+        if (lost) atomicExch(&g_timeout, 1);
+    };
+    if (RESIDENT) arrived();
+    // the list's positions leave the row; who finds one gone already has an index that occurs again (or a logit of -inf, which adds nothing)
+#pragma unroll
+    for (int i = 0; i < PER_THREAD; ++i) {
+        if (i * NT >= k) break;
+        if (!(idx[i] >= e0 && idx[i] < e1)) continue;
+        bool again;
+        if (!RESIDENT) {
+            const int bit = idx[i] - base;
+            again = atomicOr(&bitmap[bit >> 5], 1u << (bit & 31)) >> (bit & 31) & 1u;
+        } else if (idx[i] < f0 || idx[i] >= f1) {
+            const int which = idx[i] < f0 ? 0 : 1, bit = idx[i] - (which ? f1 : g.first(0));
+            again = atomicOr(&sh.edge[which], 1u << bit) >> bit & 1u;
+        } else if (N == 4) {
+            again = atomicExch(reinterpret_cast<uint32_t*>(part) + (idx[i] - f0), 0xFF800000u) == 0xFF800000u;
+        } else {
+            const int shift = (idx[i] - f0 & 1) * 16;
+            uint32_t* word = reinterpret_cast<uint32_t*>(part) + (idx[i] - f0 >> 1);
+            again = (atomicOr(word, 0xFF80u << shift) >> shift & 0xFF80u) == 0xFF80u;
+            atomicAnd(word, ~(0x007Fu << shift));
+        }
+        if (again) sh.dup = 1;
+        else sum_k += ek[i];
+    }
+    block_sum(sh, min(WARPS, (k + 31) / 32), sum_p, sum_k, cross);             // (its barrier: the positions are gone)
     const double Sp = sum_p + e_rest;
 
     // everything else: running maximum and sum a thread
-    float m = -INF_F, mr = 0.0f, s = 0.0f;
+    float m = -INF_F, mr = 0.0f;
+    uint64_t sum2 = 0;                              // two floats
     const float scale = a.scale;
-    auto add = [&](float (&x)[N], uint32_t marked) {
-        if (marked) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) if (marked >> i & 1u) x[i] = -INF_F;
-        }
-        float vm = x[0];
-#pragma unroll
-        for (int i = 1; i < N; ++i) vm = fmaxf(vm, x[i]);
+    const uint64_t scale2 = pair_of(scale, scale);
+    auto raise = [&](float vm) {
         if (vm > m) {
-            s *= ex2((m - vm) * scale);
+            const float f = ex2((m - vm) * scale);
+            sum2 = mul2(sum2, pair_of(f, f));
             m = mr = vm;
         }
+    };
+    auto add = [&](uint4 r) {
+        uint64_t x[N / 2];
+        unpack_pairs(r, x, (const T*)nullptr);
+        const uint64_t ref2 = pair_of(-mr, -mr);
 #pragma unroll
-        for (int i = 0; i < N; ++i) s += ex2((x[i] - mr) * scale);
+        for (int i = 0; i < N / 2; ++i) {
+            float lo, hi;
+            split(mul2(add2(x[i], ref2), scale2), lo, hi);
+            sum2 = add2(sum2, pair_of(ex2(lo), ex2(hi)));
+        }
     };
-    auto marks = [&](int v) -> uint32_t {
+    auto get = [&](int v) -> uint4 { return part[v - w0]; };
+    auto marked = [&](uint4 r, int v) -> uint4 {    // without the list's positions
+        if (RESIDENT) return r;
         const int bit = (v - v0) * N;
-        return reinterpret_cast<const unsigned char*>(bitmap)[bit >> 3] >> (bit & 7) & ((1u << N) - 1u);
+        const uint32_t marks = reinterpret_cast<const unsigned char*>(bitmap)[bit >> 3] >> (bit & 7) & ((1u << N) - 1u);
+        if (!marks) return r;
+        float x[N];
+        unpack(r, x, (const T*)nullptr);
+#pragma unroll
+        for (int i = 0; i < N; ++i) if (marks >> i & 1u) x[i] = -INF_F;
+        return pack(x, (const T*)nullptr);
     };
-    {
-        const int w0 = g.whole_from(v0), w1 = g.whole_to(v1);
-        int v = w0 + t;
-        for (; v + (UNROLL - 1) * NT < w1; v += UNROLL * NT) {
+    auto run = [&](int from, int to, auto load) {
+        int v = from + t;
+        for (; v + (UNROLL - 1) * NT < to; v += UNROLL * NT) {
             uint4 r[UNROLL];
 #pragma unroll
-            for (int u = 0; u < UNROLL; ++u) r[u] = g.load(v + u * NT);
+            for (int u = 0; u < UNROLL; ++u) r[u] = load(v + u * NT);
+            float vm = -INF_F;
 #pragma unroll
-            for (int u = 0; u < UNROLL; ++u) { float x[N]; unpack(r[u], x, (const T*)nullptr); add(x, marks(v + u * NT)); }
+            for (int u = 0; u < UNROLL; ++u) { r[u] = marked(r[u], v + u * NT); vm = fmaxf(vm, vector_max(r[u], (const T*)nullptr)); }
+            raise(vm);
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u) add(r[u]);
         }
-        for (; v < w1; v += NT) { float x[N]; unpack(g.load(v), x, (const T*)nullptr); add(x, marks(v)); }
-        if (t < 2) {
+        for (; v < to; v += NT) {
+            const uint4 r = marked(load(v), v);
+            raise(vector_max(r, (const T*)nullptr));
+            add(r);
+        }
+    };
+    {
+        if (!RESIDENT) {
+            run(h1, w1, [&](int v) { return g.load(v); });
+            arrived();
+        }
+        if (RESIDENT || held > 0) run(w0, h1, get);
+        if (t < 2) {                                // the partial vectors
             const int pv = t == 0 ? 0 : g.count - 1;
-            if (pv >= v0 && pv < v1 && !g.whole(pv) && (t == 0 || g.count > 1)) { float x[N]; g.load_part(pv, x, -INF_F); add(x, marks(pv)); }
+            if (pv >= v0 && pv < v1 && !g.whole(pv) && (t == 0 || g.count > 1))
+                for (int i = 0; i < N; ++i) {
+                    const int e = g.first(pv) + i;
+                    if (e < 0 || e >= g.n) continue;
+                    const bool gone = RESIDENT ? sh.edge[e < f0 ? 0 : 1] >> (e - (e < f0 ? g.first(0) : f1)) & 1u : bitmap[(e - base) >> 5] >> ((e - base) & 31) & 1u;
+                    if (gone) continue;
+                    const float x = Elem<T>::load(g.p, e);
+                    raise(x);
+                    sum2 = add2(sum2, pair_of(ex2((x - mr) * scale), 0.0f));
+                }
         }
     }
-    // the block's reference and sum
+    // the warps' references and sums, then the block's
+    float s, s_hi;
+    split(sum2, s, s_hi);
+    s += s_hi;
     float ref = m;
 #pragma unroll
     for (int o = 16; o; o >>= 1) ref = fmaxf(ref, __shfl_xor_sync(0xffffffffu, ref, o));
-    if (lane_id() == 0) sh.fmax[warp_id()][0] = ref;
-    __syncthreads();
-    ref = -INF_F;
-    for (int i = 0; i < WARPS; ++i) ref = fmaxf(ref, sh.fmax[i][0]);
     if (ref == -INF_F) ref = 0.0f;
     if (!(s == 0.0f)) s *= ex2((mr - ref) * scale);
+    if (lost) s = __uint_as_float(0x7FC00000u);
 #pragma unroll
     for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (lane_id() == 0) sh.fsum[warp_id()] = s;
+    if (lane_id() == 0) { sh.ref_w[warp_id()] = ref; sh.sum_w[warp_id()] = s; }
     __syncthreads();
-    if (t == 0) {
-        double St = 0.0;
-        for (int i = 0; i < WARPS; ++i) St += (double)sh.fsum[i];
-        sh.part[0] = ref; sh.part[1] = St; sh.part[2] = Mk; sh.part[3] = sum_k; sh.part[4] = cross;
+    const double none = -(double)INF_F;
+    // from here the first warp: lane by lane the warps, then the CTAs of the cluster, every CTA the same in the same order
+    float R = -INF_F;                               // reference of the rest, a logit
+    double St = 0.0, K = none, Sk = sum_k, B = cross;
+    if (warp_id() == 0) {
+        const int l = lane_id();
+        const float ws = l < WARPS ? sh.sum_w[l] : 0.0f, wr = ws == 0.0f ? -INF_F : sh.ref_w[l & (WARPS - 1)];
+        R = wr;
+#pragma unroll
+        for (int o = WARPS / 2; o; o >>= 1) R = fmaxf(R, __shfl_xor_sync(0xffffffffu, R, o));
+        St = ws == 0.0f ? 0.0 : (double)(ws * ex2((wr - R) * scale));
+#pragma unroll
+        for (int o = WARPS / 2; o; o >>= 1) St += __shfl_xor_sync(0xffffffffu, St, o);
+        if (C > 1 && l == 0) { sh.part[0] = (double)R; sh.part[1] = St; sh.part[2] = Mk; sh.part[3] = sum_k; sh.part[4] = cross; }
     }
     if (C > 1) cluster_arrive_wait();
-    if (t == 0) {                                   // every CTA of the cluster computes the same row's numbers in the same order
-        double R = -(double)INF_F, K = -(double)INF_F, St = 0.0, Sk = 0.0, B = 0.0;
-        double part[5];
-        auto fetch = [&](int c) { for (int i = 0; i < 5; ++i) part[i] = C > 1 ? cluster_load_f64(&sh.part[i], c) : sh.part[i]; };
-        for (int c = 0; c < C; ++c) {
-            fetch(c);
-            if (!(part[1] == 0.0)) R = fmax(R, part[0]);
-            if (!(part[3] == 0.0)) K = fmax(K, part[2]);
+    if (warp_id() == 0) {
+        const int l = lane_id();
+        if (C > 1) {
+            const bool there = l < C;
+            const float r = there ? (float)cluster_load_f64(&sh.part[0], l) : -INF_F;
+            const double st = there ? cluster_load_f64(&sh.part[1], l) : 0.0, mkk = there ? cluster_load_f64(&sh.part[2], l) : none;
+            const double sk = there ? cluster_load_f64(&sh.part[3], l) : 0.0;
+            B = there ? cluster_load_f64(&sh.part[4], l) : 0.0;
+            R = st == 0.0 ? -INF_F : r;
+            K = sk == 0.0 ? none : mkk;
+#pragma unroll
+            for (int o = 4; o; o >>= 1) {
+                R = fmaxf(R, __shfl_xor_sync(0xffffffffu, R, o));
+                K = fmax(K, __shfl_xor_sync(0xffffffffu, K, o));
+            }
+            St = st == 0.0 ? 0.0 : st * (double)ex2((r - R) * scale);
+            Sk = sk == 0.0 ? 0.0 : sk * exp(mkk - K);
+#pragma unroll
+            for (int o = 4; o; o >>= 1) {
+                St += __shfl_xor_sync(0xffffffffu, St, o);
+                Sk += __shfl_xor_sync(0xffffffffu, Sk, o);
+                B += __shfl_xor_sync(0xffffffffu, B, o);
+            }
+        } else {
+            K = sum_k == 0.0 ? none : Mk;
         }
-        if (R == -(double)INF_F) R = 0.0;
-        if (K == -(double)INF_F) K = 0.0;
-        for (int c = 0; c < C; ++c) {
-            fetch(c);
-            if (!(part[1] == 0.0)) St += part[1] * exp((part[0] - R) / a.tau);
-            if (!(part[3] == 0.0)) Sk += part[3] * exp(part[2] - K);
-            B += part[4];
-        }
-        const double none = -(double)INF_F;
-        const double Lt = St == 0.0 ? none : R / a.tau + log(St), Lk = Sk == 0.0 ? none : K + log(Sk);
-        const double top = fmax(Lt, Lk);
-        const double L = top == none ? none : top + log(exp(Lt - top) + exp(Lk - top));
-        const double Lp = Sp == 0.0 ? 0.0 : M + log(Sp), inv = Sp == 0.0 ? 0.0 : 1.0 / Sp;
+        const bool no_rest = St == 0.0, no_list = Sk == 0.0;
+        // Everything relative to A.  The factor that brings S_t there is one of fp32 (where it cannot leave its range): L and L_t share it, so its error
+        // enters the loss like S_t's own.
+        const double y = (double)R * a.inv_tau, A = no_list ? y : K;
+        const double far = (y - A) * 1.4426950408889634;
+        double Sr = St;                             // S_t relative to A
+        if (!no_rest && !no_list) Sr = fabs(far) < 120.0 ? St * (double)ex2((float)far) : St * exp(fmin(y - A, 700.0));
+        const double Sa = Sr + Sk;
+        const bool apart = !no_rest && !no_list && !(fabs(far) < 120.0);       // S_t's logarithm is taken of itself then
+        // three logarithms in three lanes
+        const double lg = log(l == 0 ? Sa : l == 1 ? (apart ? St : Sr) : Sp);
+        const double log_a = __shfl_sync(0xffffffffu, lg, 0), log_t = __shfl_sync(0xffffffffu, lg, 1), log_p = __shfl_sync(0xffffffffu, lg, 2);
+        const bool above = apart && y - A > 700.0;                             // the list is nothing against the rest
+        const double Lt = (apart ? y : A) + log_t, L = above ? Lt : A + log_a;
+        const double inv = Sp == 0.0 ? 0.0 : 1.0 / Sp, Lp = Sp == 0.0 ? 0.0 : M + log_p;
         const double pt = e_rest * inv, mass = sum_p * inv, P = Sp == 0.0 ? 0.0 : 1.0;
-        double l = 0.0, off = 0.0;
-        if (!(Sp == 0.0)) l = B * inv - Lp * mass + L * P;
-        if (!(pt == 0.0)) l += St == 0.0 ? (double)INF_F : pt * (rest - Lp - Lt);
-        if (!(St == 0.0)) off = (P * exp(Lt - L) - pt) / St;
-        if (rank == 0) a.loss[row] = (float)(l * (double)w);
-        if (rank == 0 && MODE == LOSS) a.stats[row] = make_float2((float)R, (float)off);
-        sh.stat[0] = inv; sh.stat[1] = L; sh.stat[2] = P;
-        sh.ref = (float)R; sh.off = (float)off;
+        double l_ = 0.0, off = 0.0;
+        if (!(Sp == 0.0)) l_ = B * inv - Lp * mass + (no_rest && no_list ? none : L) * P;
+        if (!(pt == 0.0)) l_ += no_rest ? (double)INF_F : pt * (rest - Lp - Lt);
+        if (!no_rest) off = (P * (above ? 1.0 : Sr / Sa) - pt) / St;
+        if (l == 0) {
+            if (rank == 0) a.loss[row] = (float)(l_ * (double)w);
+            if (rank == 0 && MODE == LOSS) a.stats[row] = make_float2(no_rest ? 0.0f : R, (float)off);
+            sh.inv = inv; sh.L = no_rest && no_list ? none : L; sh.P = P;
+            sh.ref = no_rest ? 0.0f : R;
+            sh.off = (float)off;
+        }
     }
     if (C > 1) cluster_arrive_wait();               // (the other CTAs' parts stay until everybody has read them)
     else __syncthreads();
 
     // tau dloss/dz at this CTA's entries; an index that occurs again has the same number at every place
-    const double inv = sh.stat[0], L = sh.stat[1], P = sh.stat[2];
-    const float back = (float)((double)w / a.tau);
+    const double inv = sh.inv, L = sh.L, P = sh.P;
+    const float back = (float)((double)w * a.inv_tau);
     float d[PER_THREAD];
 #pragma unroll
     for (int i = 0; i < PER_THREAD; ++i) {
+        if (i * NT >= k) break;
         const int j = t + i * NT;
         d[i] = 0.0f;
-        if (j < a.k && idx[i] >= e0 && idx[i] < e1) {
+        if (idx[i] >= e0 && idx[i] < e1) {
             double p = s_e[j];
             if (sh.dup) {
                 p = 0.0;
-                for (int n = 0; n < a.k; ++n) if (s_idx[n] == idx[i]) p += s_e[n];
+                for (int n = 0; n < k; ++n) if (s_idx[n] == idx[i]) p += s_e[n];
             }
             d[i] = (float)(P * exp(yj[i] - L) - p * inv);
-            if (MODE == LOSS) a.list_grad[row * a.k + j] = d[i];
+            if (MODE == LOSS) a.list_grad[row * k + j] = d[i];
         }
     }
     if (MODE == STEP) {
         T* out = reinterpret_cast<T*>(a.grad) + row * a.grad_pitch;
-        write_outside(g, v0, v1, out, sh.ref, scale, sh.off * back);
+        // (the last time that the row is read, and what is written is not read here: neither has to stay in L2, where the rows of the other CTAs wait)
+        if (RESIDENT) {
+            write_outside<T, NT>(g, v0, v1, out, sh.ref, scale, sh.off * back, get);
+        } else {
+            write_outside<T, NT>(g, v0, v1, out, sh.ref, scale, sh.off * back, [&](int v) {
+                return v < h1 ? part[v - w0] : __ldcs(reinterpret_cast<const uint4*>(g.p + g.first(v)));
+            });
+        }
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < PER_THREAD; ++i)
-            if (t + i * NT < a.k && idx[i] >= e0 && idx[i] < e1) Elem<T>::store(out, idx[i], d[i] * back);
+        for (int i = 0; i < PER_THREAD; ++i) {
+            if (i * NT >= k) break;
+            if (idx[i] >= e0 && idx[i] < e1) Elem<T>::store(out, idx[i], d[i] * back);
+        }
     }
 }
 
 // The gradient from what the loss left: one pass, several CTAs a row.
 template <typename T>
-__global__ void __launch_bounds__(NT, 3) distill_grad_kernel(Args a) {
+__global__ void __launch_bounds__(GRAD_NT, 3) distill_grad_kernel(Args a) {
     const int parts = a.cluster, part = blockIdx.x % parts, t = threadIdx.x;
     const int64_t row = blockIdx.x / parts;
     const float w = a.weights ? a.weights[row] : 1.0f;
-    if (w == 0.0f) { zero_part<T>(a, row, part, parts); return; }
+    if (w == 0.0f) { zero_part<T, GRAD_NT>(a, row, part, parts); return; }
     const float2 st = a.stats[row];
-    const float back = (float)((double)w * (double)a.grad_loss[row * a.grad_loss_stride] / a.tau);
+    const float back = (float)((double)w * (double)a.grad_loss[row * a.grad_loss_stride] * a.inv_tau);
     const RowGrid<T> g(reinterpret_cast<const T*>(a.logits) + row * a.pitch, a.vocab);
     int v0, v1;
     part_of(g.count, part, parts, v0, v1);
     const int e0 = max(g.first(v0), 0), e1 = min(g.first(v1), a.vocab);
     T* out = reinterpret_cast<T*>(a.grad) + row * a.grad_pitch;
-    write_outside(g, v0, v1, out, st.x, a.scale, st.y * back);
+    write_outside<T, GRAD_NT>(g, v0, v1, out, st.x, a.scale, st.y * back, [&](int v) { return g.load(v); });
     __syncthreads();
-    for (int j = t; j < a.k; j += NT) {
+    for (int j = t; j < a.k; j += GRAD_NT) {
         const int i = a.indices[row * a.k + j];
         if (i >= e0 && i < e1) Elem<T>::store(out, i, a.list_grad[row * a.k + j] * back);
     }
 }
 
-// CTAs of a row: as many as give every SM one, up to eight, but no part below 4 KB; and as many as its bitmap needs.
+// CTAs of a row: as many as give every SM two or three, up to eight, but no part below 4 KB.
 static int cluster_of(int64_t rows, int64_t bytes, int sms) {
     int c = 1;
-    while (c < 8 && rows * c * 2 <= sms * 2 && bytes / (2 * c) >= 4096) c *= 2;
+    while (c < 8 && rows * c * 2 <= sms * 3 && bytes / (2 * c) >= 4096) c *= 2;
     return c;
 }
 
 template <typename T, int MODE> int launch(Args a, int64_t rows, cudaStream_t s) {
     const int sms = device_sm_count();
     if (sms < 0) return MAB_ERR_CUDA;
+    constexpr int N = RowGrid<T>::N;
     a.cluster = cluster_of(rows, (int64_t)a.vocab * sizeof(T), sms);
-    const size_t bits = ((size_t)(a.vocab + RowGrid<T>::N) / a.cluster + 2 * RowGrid<T>::N + 63) / 32 * 4;
-    const size_t smem = (size_t)a.k * 8 + (size_t)(a.k + 1) / 2 * 8 + bits;
-    return launch_rows(distill_kernel<T, MODE>, "distill", rows * a.cluster, NT, smem, a.cluster, s, a);
+    const size_t list = ((size_t)a.k * 12 + 15) / 16 * 16;
+    const size_t vectors = ((size_t)a.vocab / N + 2 + a.cluster - 1) / a.cluster, bits = (vectors * N + 31) / 32 * 4;
+    if (vectors * 16 <= PART)
+        return launch_rows(distill_kernel<T, MODE, true, 256>, "distill", rows * a.cluster, 256, list + vectors * 16, a.cluster, s, a);
+    if (MODE == LOSS) return launch_rows(distill_kernel<T, MODE, false, 256>, "distill", rows * a.cluster, 256, list + bits, a.cluster, s, a);
+    a.held = (int)std::min<int64_t>((int64_t)vectors, std::max<int64_t>(0, STEP_SHARED - (int64_t)(list + bits)) / 16);
+    return launch_rows(distill_kernel<T, MODE, false, 512>, "distill", rows * a.cluster, 512, list + bits + (size_t)a.held * 16, a.cluster, s, a);
 }
 
 template <typename T> int launch_grad(Args a, int64_t rows, cudaStream_t s) {
     const int sms = device_sm_count();
     if (sms < 0) return MAB_ERR_CUDA;
     a.cluster = cluster_of(rows, (int64_t)a.vocab * sizeof(T), sms);
-    return launch_rows(distill_grad_kernel<T>, "distill_grad", rows * a.cluster, NT, 0, 1, s, a);
+    return launch_rows(distill_grad_kernel<T>, "distill_grad", rows * a.cluster, GRAD_NT, 0, 1, s, a);
 }
 
 static int check(const char* who, int64_t rows, int64_t vocab, int64_t k, const void* logits, int dtype, int64_t pitch, const int32_t* indices,
@@ -406,12 +556,19 @@ static Args args_of(int64_t vocab, int64_t k, const void* logits, int64_t pitch,
                     const float* rest, const float* weights, double tau) {
     Args a = {};
     a.logits = logits; a.pitch = pitch; a.indices = indices; a.values = values; a.values_bf16 = v_dtype == MAB_BF16;
-    a.rest = rest; a.weights = weights; a.tau = tau; a.scale = (float)(1.4426950408889634 / tau);
+    a.rest = rest; a.weights = weights; a.inv_tau = 1.0 / tau; a.scale = (float)(1.4426950408889634 / tau);
     a.vocab = (int)vocab; a.k = (int)k;
     return a;
 }
 
 }  // namespace distill
+
+int copy_timeout_distill(int* out, bool clear) {
+    cudaError_t e = cudaMemcpyFromSymbol(out, distill::g_timeout, sizeof(int));
+    if (e == cudaSuccess && clear) { const int z = 0; e = cudaMemcpyToSymbol(distill::g_timeout, &z, sizeof(int)); }
+    return e == cudaSuccess ? MAB_OK : cuda_fail(e, "distill wait flag");
+}
+
 }  // namespace mab
 
 using namespace mab;

@@ -130,5 +130,6 @@ int copy_timeout_bf16(int* out, bool clear);     // ef_topk_quant_bf16.cu
 int copy_timeout_bf16_warps(int* out, bool clear);  // ef_topk_quant_bf16_warps.cu
 int copy_timeout_window(int* out, bool clear);   // window_adam.cu
 int copy_timeout_int8_matmul(int* out, bool clear);   // int8_matmul.cu
+int copy_timeout_distill(int* out, bool clear);   // distill.cu
 
 }  // namespace mab

@@ -69,6 +69,11 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
 __device__ __forceinline__ void unpack_pairs(uint4 r, uint64_t (&x)[2], const float*) {
     x[0] = (uint64_t)r.y << 32 | r.x; x[1] = (uint64_t)r.w << 32 | r.z;
 }
@@ -104,8 +109,10 @@ constexpr uint32_t KEY_NEG_INF = 0x007FFFFFu;       // ord_key(-inf); every numb
 __device__ __forceinline__ uint32_t row_key(float x) { return x == x ? ord_key(x + 0.0f) : 0u; }
 
 // ----------------------------------------------------------------------------- clusters of CTAs, one per row
+// (every thread of every CTA, warps whole: the unaligned form costs microseconds where a warp comes to it in pieces)
 __device__ __forceinline__ void cluster_arrive_wait() {
-    asm volatile("barrier.cluster.arrive;\n\tbarrier.cluster.wait;" ::: "memory");
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
 // Address of `p` (in this CTA's shared memory) in that of CTA `rank` of the cluster.
 __device__ __forceinline__ uint32_t cluster_addr(const void* p, int rank) {
