@@ -18,18 +18,28 @@ CSRC = os.path.join(HERE, 'csrc')
 OUT_DIR = os.path.join(HERE, 'ista_daslab_optimizers_b200', 'lib')
 LIB_PATH = os.path.join(OUT_DIR, 'libmicroadam_b200.so')
 HOST_SRC = os.path.join(HERE, 'csrc_host', 'step_plan.cpp')
+CALLS_SRC = os.path.join(HERE, 'csrc_host', 'distill_calls.cpp')
 INCLUDE = os.path.join(os.path.dirname(HERE), 'include')
 
 
 def host_path() -> str:
     """The extension, next to its users.  It is compiled against the layout of torch's and Python's objects, so its file
     name carries their versions: for others it does not exist."""
+    return _native().step_plan_path()
+
+
+def calls_path() -> str:
+    """The same for the distillation operators' host side."""
+    return _native().distill_calls_path()
+
+
+def _native():
     sys.path.insert(0, HERE)
     try:
-        from ista_daslab_optimizers_b200._native import step_plan_path
+        from ista_daslab_optimizers_b200 import _native
     finally:
         sys.path.remove(HERE)
-    return step_plan_path()
+    return _native
 
 
 def _nvcc() -> str:
@@ -44,28 +54,28 @@ def sources():
 
 
 def _inputs():
-    deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)] + [HOST_SRC]
+    deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)] + [HOST_SRC, CALLS_SRC]
     deps += [os.path.join(INCLUDE, f) for f in os.listdir(INCLUDE)]
     return deps
 
 
 def up_to_date() -> bool:
-    built = (LIB_PATH, host_path())
+    built = (LIB_PATH, host_path(), calls_path())
     if not all(os.path.exists(p) for p in built):
         return False
     t = min(os.path.getmtime(p) for p in built)
     return all(os.path.getmtime(p) <= t for p in _inputs())
 
 
-def host_command():
-    """The g++ line of the extension that walks the optimizer's tensors (it reads torch's tensors directly)."""
+def host_command(source=HOST_SRC, out=None):
+    """The g++ line of an extension that reads torch's tensors directly: the one that walks the optimizer's tensors, or another."""
     import sysconfig
     import torch
     base = os.path.dirname(torch.__file__)
     cuda = os.path.dirname(os.path.dirname(os.path.realpath(_nvcc())))
     return [os.environ.get('CXX', 'g++'), '-O2', '-std=c++17', '-fPIC', '-shared', '-I', INCLUDE, '-I', os.path.join(base, 'include'),
             '-I', os.path.join(base, 'include', 'torch', 'csrc', 'api', 'include'), '-I', os.path.join(cuda, 'include'),
-            '-I', sysconfig.get_paths()['include'], HOST_SRC, '-o', host_path(), '-L', os.path.join(base, 'lib'),
+            '-I', sysconfig.get_paths()['include'], source, '-o', out or host_path(), '-L', os.path.join(base, 'lib'),
             '-ltorch_python', '-lc10_cuda', '-lc10', '-ltorch_cpu']
 
 
@@ -82,7 +92,8 @@ def build(verbose: bool = False, force: bool = False) -> str:
         common += ['-Xptxas', '-v']
     if os.environ.get('MAB_STATS'):
         common += ['-DMAB_STATS']       # development-only tile statistics
-    procs = [(HOST_SRC, subprocess.Popen(host_command(), stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True))]
+    procs = [(s, subprocess.Popen(host_command(s, o), stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True))
+             for s, o in ((HOST_SRC, host_path()), (CALLS_SRC, calls_path()))]
     for src in sources():
         obj = os.path.join(obj_dir, os.path.basename(src)[:-3] + '.o')
         objs.append(obj)

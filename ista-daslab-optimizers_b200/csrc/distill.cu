@@ -503,16 +503,28 @@ static int cluster_of(int64_t rows, int64_t bytes, int sms) {
     return c;
 }
 
+// Parts of up to 66 KB are held as a whole, by clusters of four where a step has few rows (us, one CTA a row and four: 300 rows of 128256 bf16 53 and 47, 600 rows 84
+// and 85: a cluster's exchange costs some 2 us a row).  Longer rows: the loss reads its row once anyway; a step reads what it does not hold a second time, from L2 if the
+// rows under way fit there.  Up to 140 KB they do with four CTAs of 256 threads an SM (2048 rows of 50257 bf16: 97, with two of 512 threads that hold 100 KB each 114; of
+// 80000: 153 and 147), beyond 400 KB a part only with more CTAs a row (1000 rows of 151936 fp32: 325, with two 266, with four 262).
 template <typename T, int MODE> int launch(Args a, int64_t rows, cudaStream_t s) {
     const int sms = device_sm_count();
     if (sms < 0) return MAB_ERR_CUDA;
     constexpr int N = RowGrid<T>::N;
-    a.cluster = cluster_of(rows, (int64_t)a.vocab * sizeof(T), sms);
+    const int64_t bytes = (int64_t)a.vocab * sizeof(T);
+    a.cluster = cluster_of(rows, bytes, sms);
+    if (MODE == STEP) {
+        int whole = a.cluster;                      // CTAs that hold the row
+        while (whole < 4 && bytes / whole > PART - 64) whole *= 2;
+        if (bytes / whole <= PART - 64 && rows * whole <= sms * 8) a.cluster = whole;
+        while (a.cluster < 8 && bytes / a.cluster > 400 * 1024) a.cluster *= 2;
+    }
     const size_t list = ((size_t)a.k * 12 + 15) / 16 * 16;
     const size_t vectors = ((size_t)a.vocab / N + 2 + a.cluster - 1) / a.cluster, bits = (vectors * N + 31) / 32 * 4;
     if (vectors * 16 <= PART)
         return launch_rows(distill_kernel<T, MODE, true, 256>, "distill", rows * a.cluster, 256, list + vectors * 16, a.cluster, s, a);
-    if (MODE == LOSS) return launch_rows(distill_kernel<T, MODE, false, 256>, "distill", rows * a.cluster, 256, list + bits, a.cluster, s, a);
+    if (MODE == LOSS || vectors * 16 <= 140 * 1024)
+        return launch_rows(distill_kernel<T, MODE, false, 256>, "distill", rows * a.cluster, 256, list + bits, a.cluster, s, a);
     a.held = (int)std::min<int64_t>((int64_t)vectors, std::max<int64_t>(0, STEP_SHARED - (int64_t)(list + bits)) / 16);
     return launch_rows(distill_kernel<T, MODE, false, 512>, "distill", rows * a.cluster, 512, list + bits + (size_t)a.held * 16, a.cluster, s, a);
 }

@@ -119,31 +119,57 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
 
 
 _step_plan = None
+_distill_calls = None
+
+
+def _extension_path(name: str) -> str:
+    here = os.path.dirname(os.path.abspath(__file__))
+    return os.path.join(here, f'{name}.{sys.implementation.cache_tag}.torch-{torch.__version__}.so')
 
 
 def step_plan_path() -> str:
     """The step's native host side, as built for this torch and this Python (it reads their objects' fields directly, so
     a file built for others must not be loaded)."""
-    here = os.path.dirname(os.path.abspath(__file__))
-    return os.path.join(here, f'_step_plan.{sys.implementation.cache_tag}.torch-{torch.__version__}.so')
+    return _extension_path('_step_plan')
+
+
+def distill_calls_path() -> str:
+    """The same for the distillation operators' native host side."""
+    return _extension_path('_distill_calls')
+
+
+def _load_extension(path: str, name: str):
+    hint = 'build it with `python ista-daslab-optimizers_b200/build.py` (needs g++ and Python\'s headers)'
+    if not os.path.exists(path):
+        raise NativeError(f'{path} is missing: {hint}')
+    try:
+        spec = importlib.util.spec_from_file_location(name, path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+    except ImportError as e:
+        raise NativeError(f'{path} cannot be loaded ({e}): {hint}') from e
+    return module
 
 
 def load_step_plan():
     """The module of the step's native host side (csrc_host/step_plan.cpp).  Raises if it is not built."""
     global _step_plan
     if _step_plan is None:
-        path, name = step_plan_path(), __package__ + '._step_plan'
-        hint = 'build it with `python ista-daslab-optimizers_b200/build.py` (needs g++ and Python\'s headers)'
-        if not os.path.exists(path):
-            raise NativeError(f'{path} is missing: {hint}')
-        try:
-            spec = importlib.util.spec_from_file_location(name, path)
-            module = importlib.util.module_from_spec(spec)
-            spec.loader.exec_module(module)
-        except ImportError as e:
-            raise NativeError(f'{path} cannot be loaded ({e}): {hint}') from e
-        _step_plan = module
+        _step_plan = _load_extension(step_plan_path(), __package__ + '._step_plan')
     return _step_plan
+
+
+def load_distill_calls():
+    """The module of the distillation operators' native host side (csrc_host/distill_calls.cpp), bound to the library.  Raises if either is not
+    built."""
+    global _distill_calls
+    if _distill_calls is None:
+        lib = load()
+        module = _load_extension(distill_calls_path(), __package__ + '._distill_calls')
+        module.bind(*(ctypes.cast(getattr(lib, 'mab_' + name), c_void_p).value for name in
+                      ('quantize_rows', 'int8_matmul', 'topk_logits', 'distill_loss', 'distill_grad', 'distill_step', 'last_error')))
+        _distill_calls = module
+    return _distill_calls
 
 
 def check(status: int, what: str) -> None:

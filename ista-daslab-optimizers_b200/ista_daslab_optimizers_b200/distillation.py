@@ -18,6 +18,8 @@ NativeError before anything is launched; there is no other implementation behind
 """
 from __future__ import annotations
 
+import operator
+
 import torch
 
 from . import _native as N
@@ -26,7 +28,7 @@ __all__ = ['quantize_rows', 'int8_matmul', 'topk_logits', 'distill_loss', 'disti
 
 
 def _rows(t, what, dtypes=(torch.float32, torch.bfloat16)):
-    """(pointer, distance of the rows) of a matrix whose rows are contiguous."""
+    """Raises unless t is a CUDA matrix of one of these types whose rows are contiguous and do not overlap."""
     if not isinstance(t, torch.Tensor) or t.dim() != 2:
         raise N.NativeError(f'{what} must be a two-dimensional tensor')
     if not t.is_cuda:
@@ -36,19 +38,16 @@ def _rows(t, what, dtypes=(torch.float32, torch.bfloat16)):
     rows, cols = t.shape
     if cols > 1 and t.stride(1) != 1:
         raise N.NativeError(f'the rows of {what} must be contiguous')
-    pitch = t.stride(0) if rows > 1 else max(cols, 1)
-    if pitch < cols:
+    if rows > 1 and t.stride(0) < cols:
         raise N.NativeError(f'the rows of {what} overlap')
-    return t.data_ptr(), pitch
 
 
-def _vector(t, n, what, device):
-    """Pointer of n contiguous float32 values, or None."""
-    if t is None:
-        return None
-    if t.dtype != torch.float32 or t.shape != (n,) or t.device != device or not t.is_contiguous():
-        raise N.NativeError(f'{what} must be {n} contiguous float32 values on {device} (got {tuple(t.shape)}, {t.dtype}, {t.device})')
-    return t.data_ptr()
+def _vector(t, n, what, device, optional=False):
+    if optional and t is None:
+        return
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.shape != (n,) or t.device != device or not t.is_contiguous():
+        got = f'{tuple(t.shape)}, {t.dtype}, {t.device}' if isinstance(t, torch.Tensor) else f'{t!r}'
+        raise N.NativeError(f'{what} must be {n} contiguous float32 values on {device} (got {got})')
 
 
 def _same_device(device, **tensors):
@@ -57,111 +56,93 @@ def _same_device(device, **tensors):
             raise N.NativeError(f'{what} is on {t.device}, not on {device}')
 
 
-def _no_grad_for(what, *tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise N.NativeError(f'{what} has no gradient: its inputs belong to a frozen teacher (call it under torch.no_grad())')
+def _no_grad_for(call, **tensors):
+    for what, t in tensors.items():
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise N.NativeError(f'{call} has no gradient for {what}: what belongs to a frozen teacher is handed over detached, or under torch.no_grad()')
+
+
+def _done(result, what, explain):
+    """What the native side answers: tensors, a status of the library, or None where an argument is not as it should be."""
+    if result is None:
+        explain()
+        raise N.NativeError(f'{what} cannot take these arguments')
+    if isinstance(result, int):
+        N.check(result, what)
+    return result
 
 
 def quantize_rows(x, codes=None, scales=None):
     """8-bit codes and one float32 scale per row of x (float32 or bfloat16 [rows, cols]): scale = max |x| / 127, code = the integer nearest
     x / scale, half to even.  A row with a NaN or an infinity gets the scale NaN and zeros.  Returns (codes, scales); codes made here
     lie a multiple of 16 bytes apart, as `int8_matmul` wants them.  Not differentiable."""
-    p, pitch = _rows(x, 'x')
-    _no_grad_for('quantize_rows', x)
-    rows, cols = x.shape
-    if codes is None:
-        codes = torch.empty(rows, (cols + 15) // 16 * 16, dtype=torch.int8, device=x.device)[:, :cols]
-    cp, codes_pitch = _rows(codes, 'codes', (torch.int8,))
-    if codes.shape != x.shape:
-        raise N.NativeError(f'codes must have the shape of x, {tuple(x.shape)} (got {tuple(codes.shape)})')
-    if scales is None:
-        scales = torch.empty(rows, dtype=torch.float32, device=x.device)
-    _same_device(x.device, codes=codes)
-    sp = _vector(scales, rows, 'scales', x.device)
-    N._run(x, 'quantize_rows', N.load().mab_quantize_rows, rows, cols, p, N.dtype_code(x), pitch, cp, codes_pitch, sp)
-    return codes, scales
+    def explain():
+        _rows(x, 'x')
+        _no_grad_for('quantize_rows', x=x)
+        if codes is not None:
+            _rows(codes, 'codes', (torch.int8,))
+            if codes.shape != x.shape:
+                raise N.NativeError(f'codes must have the shape of x, {tuple(x.shape)} (got {tuple(codes.shape)})')
+            _same_device(x.device, codes=codes)
+        _vector(scales, x.shape[0], 'scales', x.device, optional=True)
+    return _done(N.load_distill_calls().quantize_rows(x, codes, scales), 'quantize_rows', explain)
 
 
 def int8_matmul(a, b, a_scales, b_scales, bias=None, out=None, dtype=torch.bfloat16):
     """out[i, j] = (sum_c a[i, c] b[j, c]) a_scales[i] b_scales[j] + bias[j] for int8 a [tokens, inner] and b [channels, inner]: the sum exact in
     32-bit integers, then fp32, rounded once to `dtype` (float32 or bfloat16; that of `out` where it is given).  The codes start on 16 bytes and
     their rows lie a multiple of 16 bytes apart (`quantize_rows` makes them so); the inner size is at most 131071.  Not differentiable."""
-    ap, a_pitch = _rows(a, 'a', (torch.int8,))
-    bp, b_pitch = _rows(b, 'b', (torch.int8,))
-    (m, k), (n, kb) = a.shape, b.shape
-    if k != kb:
-        raise N.NativeError(f'a and b have inner sizes {k} and {kb}')
-    _no_grad_for('int8_matmul', a_scales, b_scales, bias)
-    if out is None:
-        out = torch.empty(m, n, dtype=dtype, device=a.device)
-    op, out_pitch = _rows(out, 'out')
-    if out.shape != (m, n):
-        raise N.NativeError(f'out must have the shape {(m, n)} (got {tuple(out.shape)})')
-    _same_device(a.device, b=b, out=out)
-    if m == 1:
-        a_pitch = (a_pitch + 15) // 16 * 16             # one row: no distance
-    if n == 1:
-        b_pitch = (b_pitch + 15) // 16 * 16
-    N._run(a, 'int8_matmul', N.load().mab_int8_matmul, m, n, k, ap, a_pitch, bp, b_pitch, _vector(a_scales, m, 'a_scales', a.device),
-           _vector(b_scales, n, 'b_scales', a.device), _vector(bias, n, 'bias', a.device), op, N.dtype_code(out), out_pitch)
-    return out
+    def explain():
+        _rows(a, 'a', (torch.int8,))
+        _rows(b, 'b', (torch.int8,))
+        if a.shape[1] != b.shape[1]:
+            raise N.NativeError(f'a and b have inner sizes {a.shape[1]} and {b.shape[1]}')
+        _same_device(a.device, b=b)
+        m, n = a.shape[0], b.shape[0]
+        _vector(a_scales, m, 'a_scales', a.device)
+        _vector(b_scales, n, 'b_scales', a.device)
+        _vector(bias, n, 'bias', a.device, optional=True)
+        _no_grad_for('int8_matmul', a_scales=a_scales, b_scales=b_scales, bias=bias, out=out)
+        if out is not None:
+            _rows(out, 'out')
+            if out.shape != (m, n):
+                raise N.NativeError(f'out must have the shape {(m, n)} (got {tuple(out.shape)})')
+            _same_device(a.device, out=out)
+    if out is None and dtype not in (torch.float32, torch.bfloat16):
+        raise N.NativeError(f'unsupported element type {dtype}: the kernels write float32 and bfloat16')
+    return _done(N.load_distill_calls().int8_matmul(a, b, a_scales, b_scales, bias, out, dtype is torch.bfloat16), 'int8_matmul', explain)[0]
 
 
 def topk_logits(logits, k, temperature=1.0):
     """(values, indices, rest): the k largest logits of every row (float32 or bfloat16 [rows, vocab], k at most 1024) in descending order,
     ties to the lower index, in the logits' type; their int32 indices; and the float32 logarithm of sum exp(logit / temperature) over all others, -inf
     where there is nothing else.  NaN ranks below -inf and makes `rest` NaN.  Not differentiable."""
-    p, pitch = _rows(logits, 'logits')
-    _no_grad_for('topk_logits', logits)
-    rows, vocab = logits.shape
-    values = torch.empty(rows, k, dtype=logits.dtype, device=logits.device)
-    indices = torch.empty(rows, k, dtype=torch.int32, device=logits.device)
-    rest = torch.empty(rows, dtype=torch.float32, device=logits.device)
-    N._run(logits, 'topk_logits', N.load().mab_topk_logits, rows, vocab, k, p, N.dtype_code(logits), pitch, float(temperature), values.data_ptr(),
-           indices.data_ptr(), rest.data_ptr())
-    return values, indices, rest
+    k = operator.index(k)
+
+    def explain():
+        _rows(logits, 'logits')
+        _no_grad_for('topk_logits', logits=logits)
+        if not 1 <= k <= logits.shape[1]:
+            raise N.NativeError(f'k={k} is not between 1 and the {logits.shape[1]} logits of a row')
+    return _done(N.load_distill_calls().topk_logits(logits, k, float(temperature)), 'topk_logits', explain)
 
 
-def _teacher(logits, indices, values, rest, weights):
-    """The arguments that the loss and the step share, checked: (rows, vocab, k) and the pointers."""
-    p, pitch = _rows(logits, 'logits')
+def _explain_lists(what, logits, indices, values, rest, weights, temperature):
+    _no_grad_for(what, values=values, rest=rest, weights=weights)
+    _rows(logits, 'logits')
     rows, vocab = logits.shape
-    device = logits.device
     if indices.dim() != 2 or indices.shape[0] != rows or values.shape != indices.shape:
         raise N.NativeError(f'indices and values must be [{rows}, k] (got {tuple(indices.shape)} and {tuple(values.shape)})')
-    if indices.dtype != torch.int32:
-        raise N.NativeError(f'indices must be int32 (got {indices.dtype})')
-    _same_device(device, indices=indices, values=values)
-    return (rows, vocab, indices.shape[1]), (p, N.dtype_code(logits), pitch, N.dev_ptr(indices, 'indices'), N.dev_ptr(values, 'values'),
-                                             N.dtype_code(values), _vector(rest, rows, 'rest', device), _vector(weights, rows, 'weights', device))
-
-
-class _DistillLoss(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, indices, values, rest, weights, temperature):
-        (rows, vocab, k), args = _teacher(logits, indices, values, rest, weights)
-        loss = torch.empty(rows, dtype=torch.float32, device=logits.device)
-        stats = torch.empty(rows, 2, dtype=torch.float32, device=logits.device)
-        list_grad = torch.empty(rows, k, dtype=torch.float32, device=logits.device)
-        N._run(logits, 'distill_loss', N.load().mab_distill_loss, rows, vocab, k, *args, temperature, loss.data_ptr(), stats.data_ptr(),
-               list_grad.data_ptr())
-        ctx.save_for_backward(logits, indices, weights, stats, list_grad)
-        ctx.temperature = temperature
-        return loss
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_loss):
-        logits, indices, weights, stats, list_grad = ctx.saved_tensors
-        p, pitch = _rows(logits, 'logits')
-        rows, vocab = logits.shape
-        if grad_loss.dtype != torch.float32:
-            grad_loss = grad_loss.float()
-        grad = torch.empty(rows, vocab, dtype=logits.dtype, device=logits.device)
-        N._run(logits, 'distill_loss backward', N.load().mab_distill_grad, rows, vocab, indices.shape[1], p, N.dtype_code(logits), pitch,
-               indices.data_ptr(), None if weights is None else weights.data_ptr(), ctx.temperature, stats.data_ptr(), list_grad.data_ptr(),
-               grad_loss.data_ptr(), grad_loss.stride(0), grad.data_ptr(), vocab)
-        return grad, None, None, None, None, None
+    if indices.dtype != torch.int32 or values.dtype not in (torch.float32, torch.bfloat16):
+        raise N.NativeError(f'indices must be int32, values float32 or bfloat16 (got {indices.dtype} and {values.dtype})')
+    _same_device(logits.device, indices=indices, values=values)
+    N.dev_ptr(indices, 'indices')
+    N.dev_ptr(values, 'values')
+    _vector(rest, rows, 'rest', logits.device, optional=True)
+    _vector(weights, rows, 'weights', logits.device, optional=True)
+    if not 1 <= indices.shape[1] <= N.MAB_MAX_LIST or not 1 <= vocab <= N.MAB_MAX_VOCAB or not 1e-6 < temperature < 1e6:
+        raise N.NativeError(f'lists of {indices.shape[1]} entries (at most {N.MAB_MAX_LIST}), rows of {vocab} logits (at most {N.MAB_MAX_VOCAB}), '
+                            f'temperature {temperature} (between 1e-6 and 1e6)')
 
 
 def distill_loss(logits, indices, values, rest=None, weights=None, temperature=1.0):
@@ -176,24 +157,23 @@ def distill_loss(logits, indices, values, rest=None, weights=None, temperature=1
     weights         float32 [rows] or None: a row with weight 0 is not read, whatever it holds, and has loss and gradient 0.  (Multiply by
                     temperature ** 2 here for gradients that do not shrink with the temperature.)
 
-    The gradient comes from a second pass over the logits; `distill_step` reads them once."""
-    for what, t in (('values', values), ('rest', rest), ('weights', weights)):
-        if t is not None and t.requires_grad and torch.is_grad_enabled():
-            raise N.NativeError(f'distill_loss has no gradient for {what}')
-    return _DistillLoss.apply(logits, indices, values, rest, weights, float(temperature))
+    The gradient comes from a second pass over the logits; `distill_step` gives both in one call.  Differentiable once."""
+    temperature = float(temperature)
+    return _done(N.load_distill_calls().distill_loss(logits, indices, values, rest, weights, temperature), 'distill_loss',
+                 lambda: _explain_lists('distill_loss', logits, indices, values, rest, weights, temperature))
 
 
 def distill_step(logits, indices, values, rest=None, weights=None, temperature=1.0, grad=None):
     """(loss, grad): the losses of `distill_loss` and the gradient of their sum with respect to the logits, in the logits' type, in one call.  Nothing is
     recorded for autograd: hand the gradient on with `logits.backward(grad)`.  `grad` can be given, and can be the logits' own memory
     (`grad=logits.detach()`): the gradient then replaces them."""
-    (rows, vocab, k), args = _teacher(logits, indices, values, rest, weights)
-    if grad is None:
-        grad = torch.empty(rows, vocab, dtype=logits.dtype, device=logits.device)
-    elif grad.shape != logits.shape or grad.dtype != logits.dtype or grad.requires_grad:
-        raise N.NativeError(f'grad must be like the logits, {tuple(logits.shape)} of {logits.dtype}, and require no gradient itself')
-    gp, grad_pitch = _rows(grad, 'grad')
-    _same_device(logits.device, grad=grad)
-    loss = torch.empty(rows, dtype=torch.float32, device=logits.device)
-    N._run(logits, 'distill_step', N.load().mab_distill_step, rows, vocab, k, *args, float(temperature), loss.data_ptr(), gp, grad_pitch)
-    return loss, grad
+    temperature = float(temperature)
+
+    def explain():
+        _explain_lists('distill_step', logits, indices, values, rest, weights, temperature)
+        if grad is not None:
+            if grad.shape != logits.shape or grad.dtype != logits.dtype or grad.requires_grad:
+                raise N.NativeError(f'grad must be like the logits, {tuple(logits.shape)} of {logits.dtype}, and require no gradient itself')
+            _rows(grad, 'grad')
+            _same_device(logits.device, grad=grad)
+    return _done(N.load_distill_calls().distill_step(logits, indices, values, rest, weights, temperature, grad), 'distill_step', explain)
