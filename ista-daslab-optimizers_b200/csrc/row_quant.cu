@@ -1,15 +1,14 @@
 // Rows into 8-bit integers with one scale each: s = max |x| / 127, code = the integer nearest x / s (half to even).
 //
-// A row is held in the registers of its threads between the maximum and the codes, so it is read once: bound by HBM (2 or 4 bytes in, one
-// out).  A quotient next to a half decides by its exact value: y = x RN(1/s) is off by a few units of its last place, and where the residual
-// x - c s of the code c = rint(y) (exact in one FMA: c has 7 bits and cancels all but the last bits of x) lies beyond s / 2, or on it with
-// c odd, the neighbour is the code.  That is 8 operations a value instead of a division's twenty.
+// A row is held in the registers of its threads between the maximum and the codes, so it is read once: bound by HBM (2 or 4 bytes in, one out).  y = x RN(1/s) is off
+// the quotient by less than 2^-15, so rint(y) is the code unless y lies that near to a half; a vector in which one does is coded again by exact residuals:
+// where x - c s of the code c = rint(y) (exact in one FMA: c has 7 bits and cancels all but the last bits of x) lies beyond s / 2, or on it with c odd,
+// the neighbour is the code.  The first way takes 5 operations a value (packed products, the rounding by adding 1.5 2^23, whose low byte is the code), the
+// second, for every value, took 43: 14336 x 4096 bf16 72 us.
 #include "rows.cuh"
 
 namespace mab {
 namespace quant8 {
-
-constexpr int HELD = 8;                       // vectors of 16 bytes a thread holds
 
 struct Args {
     const void* x;
@@ -30,96 +29,122 @@ __device__ __forceinline__ int code_of(float x, float s, float inv) {
     return __float2int_rn(c);
 }
 
-// TPR threads share a row.
-template <typename T, int TPR, int NT>
-__global__ void __launch_bounds__(NT) quantize_rows_kernel(Args a) {
+// |x| of a vector, the largest; NaN where there is one.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float magnitude(uint4 r, const float*) {
+    return max_nan(max_nan(fabsf(__uint_as_float(r.x)), fabsf(__uint_as_float(r.y))), max_nan(fabsf(__uint_as_float(r.z)), fabsf(__uint_as_float(r.w))));
+}
+__device__ __forceinline__ float magnitude(uint4 r, const uint16_t*) {
+    uint32_t a, b;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(r.x & 0x7FFF7FFFu), "r"(r.y & 0x7FFF7FFFu));
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(b) : "r"(r.z & 0x7FFF7FFFu), "r"(r.w & 0x7FFF7FFFu));
+    asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(a) : "r"(b));
+    return max_nan(__uint_as_float(a << 16), __uint_as_float(a & 0xFFFF0000u));
+}
+
+// The codes of a vector, a byte each.
+template <typename T, int N> __device__ __forceinline__ void codes_of(uint4 r, float s, float inv, uint32_t (&w)[N / 4]) {
+    constexpr float MAGIC = 12582912.0f;             // 1.5 2^23
+    uint64_t x[N / 2];
+    unpack_pairs(r, x, (const T*)nullptr);
+    const uint64_t inv2 = pair_of(inv, inv), up = pair_of(MAGIC, MAGIC), down = pair_of(-MAGIC, -MAGIC), minus = pair_of(-1.0f, -1.0f);
+    float far = 0.0f;
+    uint32_t c[N];
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+        const uint64_t y = mul2(x[i], inv2), m = add2(y, up), t = fma2(add2(m, down), minus, y);      // y - rint(y), exact
+        float lo, hi;
+        split(t, lo, hi);
+        far = fmaxf(far, fmaxf(fabsf(lo), fabsf(hi)));
+        c[2 * i] = (uint32_t)m;
+        c[2 * i + 1] = (uint32_t)(m >> 32);
+    }
+    if (far > 0.5f - 6.103515625e-05f) {
+        float v[N];
+        unpack(r, v, (const T*)nullptr);
+#pragma unroll
+        for (int i = 0; i < N; ++i) c[i] = (uint32_t)code_of(v[i], s, inv);
+    }
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i)
+        w[i] = __byte_perm(__byte_perm(c[4 * i], c[4 * i + 1], 0x0040), __byte_perm(c[4 * i + 2], c[4 * i + 3], 0x0040), 0x5410);
+}
+
+// TPR threads share a row, each holds up to HELD vectors of it.  What limits the rate is how many bytes are on their way, so the registers are kept to those of
+// 1536 threads an SM where four vectors are enough.
+template <typename T, int TPR, int NT, int HELD>
+__global__ void __launch_bounds__(NT, HELD == 4 ? 1536 / NT : 1024 / NT) quantize_rows_kernel(Args a) {
     constexpr int N = RowGrid<T>::N;
-    __shared__ uint32_t s_max[NT / 32];
+    __shared__ float s_max[NT / 32];
     const int64_t row = (int64_t)blockIdx.x * (NT / TPR) + threadIdx.x / TPR;
     const int t = threadIdx.x % TPR;
     const bool there = row < a.rows;
     const RowGrid<T> g(reinterpret_cast<const T*>(a.x) + (there ? row : 0) * a.pitch, a.cols);
-    // |x| bits: an infinity or a NaN is not below those of infinity
-    uint32_t top = 0;
-    auto see = [&](const float (&x)[N]) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+    const int w0 = g.whole_from(0), w1 = g.whole_to(g.count);
+    auto fetch = [&](int v) {                       // any vector; zeros outside the row
+        if (v >= w0 && v < w1) return g.load(v);
+        float x[N];
+        g.load_part(v, x, 0.0f);
+        return pack(x, (const T*)nullptr);
     };
     uint4 held[HELD];
+    float top = 0.0f;
     if (there) {
-        const int w0 = g.whole_from(0), w1 = g.whole_to(g.count);
 #pragma unroll
-        for (int i = 0; i < HELD; ++i) if (t + i * TPR >= w0 && t + i * TPR < w1) held[i] = g.load(t + i * TPR);
+        for (int i = 0; i < HELD; ++i) if (t + i * TPR < g.count) held[i] = fetch(t + i * TPR);
 #pragma unroll
-        for (int i = 0; i < HELD; ++i) if (t + i * TPR >= w0 && t + i * TPR < w1) {
-            float x[N];
-            unpack(held[i], x, (const T*)nullptr);
-            see(x);
-        }
-        for (int v = t; v < g.count; v += TPR) {               // what the registers do not hold, and the partial vectors
-            if (v < HELD * TPR && v >= w0 && v < w1) continue;
-            float x[N];
-            if (v >= w0 && v < w1) unpack(g.load(v), x, (const T*)nullptr);
-            else g.load_part(v, x, 0.0f);
-            see(x);
-        }
+        for (int i = 0; i < HELD; ++i) if (t + i * TPR < g.count) top = max_nan(top, magnitude(held[i], (const T*)nullptr));
+        for (int v = t + HELD * TPR; v < g.count; v += TPR) top = max_nan(top, magnitude(fetch(v), (const T*)nullptr));      // what the registers do not hold
     }
 #pragma unroll
-    for (int o = 16; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    for (int o = 16; o; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
     if (TPR > 32) {
         if (lane_id() == 0) s_max[warp_id()] = top;
         __syncthreads();
-        const int w0 = threadIdx.x / TPR * (TPR / 32);
+        const int first = threadIdx.x / TPR * (TPR / 32);
 #pragma unroll
-        for (int w = 0; w < TPR / 32; ++w) top = max(top, s_max[w0 + w]);
+        for (int w = 0; w < TPR / 32; ++w) top = max_nan(top, s_max[first + w]);
     }
     if (!there) return;
-    float s = __fdiv_rn(__uint_as_float(top), 127.0f);
+    float s = __fdiv_rn(top, 127.0f);
     if (s < 1.17549435e-38f) s = 0.0f;
-    const bool coded = s > 0.0f && top < 0x7F800000u;
-    if (top >= 0x7F800000u) s = __uint_as_float(0x7FC00000u);
+    const bool finite = top < INF_F, coded = s > 0.0f && finite;               // (a NaN is not below)
+    if (!finite) s = __uint_as_float(0x7FC00000u);
     if (t == 0) a.scales[row] = s;
     const float inv = coded ? __frcp_rn(s) : 0.0f;
     int8_t* out = a.codes + row * a.codes_pitch;
-    auto put = [&](int v, const float (&x)[N]) {
-        int c[N];
+    const bool aligned = (reinterpret_cast<uintptr_t>(out + g.first(0)) & (N - 1)) == 0;
+    auto put = [&](int v, uint4 r) {
+        uint32_t w[N / 4];
 #pragma unroll
-        for (int i = 0; i < N; ++i) c[i] = coded ? code_of(x[i], s, inv) : 0;
+        for (int i = 0; i < N / 4; ++i) w[i] = 0;
+        if (coded) codes_of<T, N>(r, s, inv, w);
         const int e = g.first(v);
-        int8_t* o = out + e;
-        if (e >= 0 && e + N <= g.n && (reinterpret_cast<uintptr_t>(o) & (N - 1)) == 0) {
-            uint32_t w[N / 4];
-#pragma unroll
-            for (int i = 0; i < N / 4; ++i)
-                w[i] = (uint32_t)(c[4 * i] & 255) | (uint32_t)(c[4 * i + 1] & 255) << 8 | (uint32_t)(c[4 * i + 2] & 255) << 16 | (uint32_t)c[4 * i + 3] << 24;
-            if (N == 8) *reinterpret_cast<uint2*>(o) = make_uint2(w[0], w[N / 4 - 1]);
-            else *reinterpret_cast<uint32_t*>(o) = w[0];
+        if (aligned && v >= w0 && v < w1) {
+            if (N == 8) *reinterpret_cast<uint2*>(out + e) = make_uint2(w[0], w[N / 4 - 1]);
+            else *reinterpret_cast<uint32_t*>(out + e) = w[0];
         } else {
 #pragma unroll
-            for (int i = 0; i < N; ++i) if (e + i >= 0 && e + i < g.n) o[i] = (int8_t)c[i];
+            for (int i = 0; i < N; ++i) if (e + i >= 0 && e + i < g.n) out[e + i] = (int8_t)(w[i / 4] >> (8 * (i % 4)));
         }
     };
-    const int w0 = g.whole_from(0), w1 = g.whole_to(g.count);
 #pragma unroll
-    for (int i = 0; i < HELD; ++i) if (t + i * TPR >= w0 && t + i * TPR < w1) {
-        float x[N];
-        unpack(held[i], x, (const T*)nullptr);
-        put(t + i * TPR, x);
-    }
-    for (int v = t; v < g.count; v += TPR) {
-        if (v < HELD * TPR && v >= w0 && v < w1) continue;
-        float x[N];
-        if (v >= w0 && v < w1) unpack(g.load(v), x, (const T*)nullptr);
-        else g.load_part(v, x, 0.0f);
-        put(v, x);
-    }
+    for (int i = 0; i < HELD; ++i) if (t + i * TPR < g.count) put(t + i * TPR, held[i]);
+    for (int v = t + HELD * TPR; v < g.count; v += TPR) put(v, fetch(v));
 }
 
 template <typename T> int launch(const Args& a, cudaStream_t s) {
+    // a warp for short rows (four rows a CTA), otherwise as many threads as hold the row
     const int64_t vectors = ceil_div64(a.cols, RowGrid<T>::N) + 1;
-    if (vectors <= 32 * 2) return launch_rows(quantize_rows_kernel<T, 32, 128>, "quantize_rows", ceil_div64(a.rows, 4), 128, 0, 1, s, a);
-    if (vectors <= 128 * HELD) return launch_rows(quantize_rows_kernel<T, 128, 128>, "quantize_rows", a.rows, 128, 0, 1, s, a);
-    return launch_rows(quantize_rows_kernel<T, 512, 512>, "quantize_rows", a.rows, 512, 0, 1, s, a);
+    if (vectors <= 32 * 4) return launch_rows(quantize_rows_kernel<T, 32, 128, 4>, "quantize_rows", ceil_div64(a.rows, 4), 128, 0, 1, s, a);
+    if (vectors <= 128 * 4 + 1) return launch_rows(quantize_rows_kernel<T, 128, 128, 4>, "quantize_rows", a.rows, 128, 0, 1, s, a);
+    if (vectors <= 256 * 4 + 1) return launch_rows(quantize_rows_kernel<T, 256, 256, 4>, "quantize_rows", a.rows, 256, 0, 1, s, a);
+    if (vectors <= 512 * 4 + 1) return launch_rows(quantize_rows_kernel<T, 512, 512, 4>, "quantize_rows", a.rows, 512, 0, 1, s, a);
+    return launch_rows(quantize_rows_kernel<T, 512, 512, 8>, "quantize_rows", a.rows, 512, 0, 1, s, a);
 }
 
 }  // namespace quant8
