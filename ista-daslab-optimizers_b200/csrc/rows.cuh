@@ -114,6 +114,9 @@ __device__ __forceinline__ void cluster_arrive_wait() {
     __syncwarp();
     asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
+// The same in two halves.  Between the beginning of a kernel and the first access to another CTA's shared memory: that CTA has begun then.
+__device__ __forceinline__ void cluster_arrive() { __syncwarp(); asm volatile("barrier.cluster.arrive.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { __syncwarp(); asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
 // Address of `p` (in this CTA's shared memory) in that of CTA `rank` of the cluster.
 __device__ __forceinline__ uint32_t cluster_addr(const void* p, int rank) {
     uint32_t a;
@@ -144,6 +147,16 @@ __device__ __forceinline__ unsigned long long cluster_load_u64(const void* p, in
     unsigned long long v;
     asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(cluster_addr(p, rank)) : "memory");
     return v;
+}
+
+__device__ __forceinline__ void cluster_store_u32(void* p, int rank, uint32_t v) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr(p, rank)), "r"(v) : "memory");
+}
+__device__ __forceinline__ void cluster_store_u64(void* p, int rank, unsigned long long v) {
+    asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(cluster_addr(p, rank)), "l"(v) : "memory");
+}
+__device__ __forceinline__ void cluster_store_f64(void* p, int rank, double v) {
+    asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(cluster_addr(p, rank)), "d"(v) : "memory");
 }
 
 // Launches `kernel` with clusters of `cluster` CTAs (1: without) and counts it.

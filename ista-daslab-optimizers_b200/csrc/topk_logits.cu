@@ -41,12 +41,11 @@ struct Shared {
     int reach[REACH];                               // those that reach the second bound
     int n_list, n_reach;
     double red[WARPS];
-    double sum;                                     // this CTA's sum over the rest, and its reference
-    float ref;
-    int far;
+    double peer_sum[8], peer_ref[8];                // of the cluster's CTAs: sum over the rest, its reference (infinite: far), number of candidates
+    uint32_t peer_n[8];
     int n;                                          // candidates (counts beyond CAP where they do not fit)
     int count[64];                                  // counters of a bisection, one per step
-    uint32_t warp_max[WARPS];
+    uint32_t warp_max[WARPS], found;
     int scan[40];
     double terms[WARPS];                            // of candidates that go into the rest
 };                                                  //   a sum of integers does not depend on it
@@ -132,28 +131,40 @@ template <typename F> __device__ __forceinline__ uint32_t kth_key(Shared& sh, ui
     return lo;
 }
 
-// The same for one key per thread, from either end: the range is first narrowed in growing steps from where the answer is expected.
-template <typename T, bool FROM_TOP> __device__ __forceinline__ uint32_t kth_of_threads(bool there, uint32_t mine, uint32_t lo, uint32_t hi, int k, int most) {
-    uint32_t step = 128u << (16 - Key<T>::SHIFT);                  // an octave
-    bool narrowing = true;
-    while (lo < hi) {
-        uint32_t mid = lo + (hi - lo) / 2 + 1;
-        if (narrowing && (hi - lo) / 2 > step) mid = FROM_TOP ? hi - step : lo + step;
-        else narrowing = false;
-        step *= 2;
-        const int r = __syncthreads_count(there && mine >= mid);
-        if (r < k) { hi = mid - 1; narrowing &= FROM_TOP; continue; }
-        lo = mid;
-        narrowing &= !FROM_TOP;
-        if (r <= most) break;
+// The same for keys[0 .. n) in shared memory, n <= 32 PER, by the first warp alone: no barrier in its steps, and the other warps' slots are free for the SM's other
+// CTAs.  The range is first narrowed in growing steps from where the answer is expected.  The answer is in every thread after the barrier at the end.
+template <typename T, bool FROM_TOP, int PER> __device__ __forceinline__ uint32_t kth_by_warp(Shared& sh, const uint32_t* keys, int n, uint32_t lo, uint32_t hi, int k, int most) {
+    if (warp_id() == 0) {
+        uint32_t key[PER];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) key[i] = lane_id() + 32 * i < n ? keys[lane_id() + 32 * i] : 0u;         // (0 is below every mid)
+        uint32_t step = 128u << (16 - Key<T>::SHIFT);              // an octave
+        bool narrowing = true;
+        while (lo < hi) {
+            uint32_t mid = lo + (hi - lo) / 2 + 1;
+            if (narrowing && (hi - lo) / 2 > step) mid = FROM_TOP ? hi - step : lo + step;
+            else narrowing = false;
+            step *= 2;
+            int q[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < PER; ++i) q[i & 3] += key[i] >= mid;
+            const int r = __reduce_add_sync(0xffffffffu, q[0] + q[1] + (q[2] + q[3]));
+            if (r < k) { hi = mid - 1; narrowing &= FROM_TOP; continue; }
+            lo = mid;
+            narrowing &= !FROM_TOP;
+            if (r <= most) break;
+        }
+        if (lane_id() == 0) sh.found = lo;
     }
-    return lo;
+    __syncthreads();
+    return sh.found;
 }
 
 // The key of the k-th largest of n >= k keys, or one between that and the (k + slack)-th; all lie in [lo, hi], n <= LIST.
 template <typename T> __device__ __noinline__ uint32_t kth_of_list(Shared& sh, int n, int k, int slack, uint32_t lo, uint32_t hi) {
     const int t = threadIdx.x;
-    if (n <= NT) return kth_of_threads<T, false>(t < n, t < n ? sh.list_key[t] : 0u, lo, hi, k, k + slack);
+    if (n <= 512) return kth_by_warp<T, false, 16>(sh, sh.list_key, n, lo, hi, k, k + slack);
+    if (n <= 1024) return kth_by_warp<T, false, 32>(sh, sh.list_key, n, lo, hi, k, k + slack);
     int reached;
     return kth_key(sh, lo, hi, k, k + slack, reached, [&](uint32_t mid) {
         int r = 0;
@@ -185,7 +196,9 @@ template <typename T> __device__ __noinline__ uint32_t bound_of_sample(Shared& s
             top = fmaxf(top, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])));
         }
         const uint32_t mine = K::of(top);
-        return kth_of_threads<T, true>(true, mine, K::NEG_INF, largest(mine), k, k + k / 8);
+        sh.list_key[threadIdx.x] = mine;
+        const uint32_t most = largest(mine);
+        return kth_by_warp<T, true, NT / 32>(sh, sh.list_key, NT, K::NEG_INF, most, k, k + k / 8);
     }
     uint32_t key[SAMPLE], top = 0;
 #pragma unroll
@@ -205,27 +218,19 @@ template <typename T> __device__ __noinline__ uint32_t prune(Shared& sh, int k, 
     const int t = threadIdx.x, n = sh.n;
     unsigned long long c[ITEMS];
     int reached;
-    uint32_t key;
-    c[0] = t < n ? sh.cand[t] : 0ull;
-    if (n <= NT) {
-        const uint32_t mine = t < n ? (uint32_t)(c[0] >> 32) : 0u;
-        key = kth_of_threads<T, false>(t < n, mine, lo, hi, k, k + slack);
-        reached = __syncthreads_count(t < n && mine >= key);
-    } else {
 #pragma unroll
-        for (int i = 1; i < ITEMS; ++i) c[i] = t + i * NT < n ? sh.cand[t + i * NT] : 0ull;
-        key = kth_key(sh, lo, hi, k, k + slack, reached, [&](uint32_t mid) {
-            int r = 0;
+    for (int i = 0; i < ITEMS; ++i) c[i] = t + i * NT < n ? sh.cand[t + i * NT] : 0ull;
+    const uint32_t key = kth_key(sh, lo, hi, k, k + slack, reached, [&](uint32_t mid) {
+        int r = 0;
 #pragma unroll
-            for (int i = 0; i < ITEMS; ++i) r += t + i * NT < n && (uint32_t)(c[i] >> 32) >= mid;
-            return r;
-        });
-    }
+        for (int i = 0; i < ITEMS; ++i) {
+            if (i * NT >= n) break;
+            r += t + i * NT < n && (uint32_t)(c[i] >> 32) >= mid;
+        }
+        return r;
+    });
     unsigned long long last = (unsigned long long)key << 32;
     if (reached > k + slack) {                      // more equals of the k-th than places: the lowest indices
-        if (n <= NT)
-#pragma unroll
-            for (int i = 1; i < ITEMS; ++i) c[i] = 0ull;
         clear_counts(sh);
         int above = 0;
 #pragma unroll
@@ -326,6 +331,7 @@ __global__ void __launch_bounds__(NT, 3) topk_logits_kernel(Args a) {
     extern __shared__ __align__(16) unsigned char dyn[];
     Shared& sh = *reinterpret_cast<Shared*>(dyn);
     const int C = a.cluster, rank = C > 1 ? (int)(blockIdx.x % C) : 0, t = threadIdx.x, k = a.k;
+    if (C > 1) cluster_arrive();
     const int64_t row = blockIdx.x / C;
     const RowGrid<T> g(reinterpret_cast<const T*>(a.logits) + row * a.pitch, a.vocab);
     const int per = (g.count + C - 1) / C, v0 = min(rank * per, g.count), v1 = min(v0 + per, g.count);
@@ -442,47 +448,46 @@ __global__ void __launch_bounds__(NT, 3) topk_logits_kernel(Args a) {
     }
 
     if (C > 1) {                                    // the first CTA takes over the others' candidates and sums
-        if (sh.n > k) prune<T>(sh, k, 0, lo_key, K::MOST, rest);
+        if (sh.n > CAP / C) prune<T>(sh, k, CAP / C - k, lo_key, K::MOST, rest);      // (what all of them have fits the first one's room)
         lo_key = 0;                                 // (the others' bounds are others)
         float s = rest.s;
 #pragma unroll
         for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
         if (lane_id() == 0) sh.red[warp_id()] = (double)s;
         __syncthreads();
-        if (t == 0) {
+        cluster_wait();
+        if (t < C) {                                // everybody learns how many candidates everybody has, the first CTA the sums, too
             double sum = 0.0;
             for (int i = 0; i < WARPS; ++i) sum += sh.red[i];
-            sh.sum = sum;
-            sh.ref = rest.ref;
-            sh.far = rest.far;
+            cluster_store_u32(&sh.peer_n[rank], t, (uint32_t)sh.n);
+            cluster_store_f64(&sh.peer_sum[rank], t, sum);
+            cluster_store_f64(&sh.peer_ref[rank], t, rest.far ? (double)INF_F : (double)rest.ref);
         }
         cluster_arrive_wait();
+        const int n = sh.n;
         if (rank == 0) {
-            int at = sh.n;
-            for (int c = 1; c < C; ++c) {
-                const int n = (int)cluster_load_u32(&sh.n, c);
-                for (int i = t; i < n; i += NT) sh.cand[at + i] = cluster_load_u64(&sh.cand[i], c);
-                at += n;
+            // the sums, relative to the largest reference of those that have one
+            float ref = -INF_F;
+            for (int c = 0; c < C; ++c) {
+                rest.far |= sh.peer_ref[c] == (double)INF_F;
+                if (!(sh.peer_sum[c] == 0.0)) ref = fmaxf(ref, (float)sh.peer_ref[c]);
             }
-            for (int c = 1; c < C; ++c) rest.far |= cluster_load_u32(&sh.far, c) != 0u;
-            float ref = -INF_F;                     // the largest reference of those that have a sum
-            for (int c = 0; c < C; ++c)
-                if (!(cluster_load_f64(&sh.sum, c) == 0.0)) ref = fmaxf(ref, cluster_load_f32(&sh.ref, c));
-            if (ref != -INF_F) {
-                if (!(rest.s == 0.0f)) rest.s *= ex2(rest.ref - ref);
-                rest.ref = ref;
-                if (t == 0)
-                    for (int c = 1; c < C; ++c) {
-                        const double sum = cluster_load_f64(&sh.sum, c);
-                        if (!(sum == 0.0)) rest.s += (float)(sum * exp2((double)cluster_load_f32(&sh.ref, c) - (double)ref));
-                    }
-            }
-            __syncthreads();
-            if (t == 0) sh.n = at;
-            __syncthreads();
+            rest.s = 0.0f;
+            rest.ref = ref == -INF_F ? 0.0f : ref;
+            if (t < C && !(sh.peer_sum[t] == 0.0)) rest.s = (float)(sh.peer_sum[t] * (double)ex2((float)sh.peer_ref[t] - rest.ref));
+        } else {
+            int at = 0;
+            for (int c = 0; c < rank; ++c) at += (int)sh.peer_n[c];
+            for (int i = t; i < n; i += NT) cluster_store_u64(&sh.cand[at + i], 0, sh.cand[i]);
         }
         cluster_arrive_wait();
         if (rank != 0) return;
+        if (t == 0) {
+            int at = 0;
+            for (int c = 0; c < C; ++c) at += (int)sh.peer_n[c];
+            sh.n = at;
+        }
+        __syncthreads();
     }
     // those from the k-th on, in order: a few by the number of larger ones, many by a sorting network
     const bool few = k <= 128;
@@ -490,16 +495,32 @@ __global__ void __launch_bounds__(NT, 3) topk_logits_kernel(Args a) {
     unsigned long long* cand = sh.cand;
     const int kept = sh.n;                          // k, or up to 192 where few
     if (few) {
-        const unsigned long long mine = t < kept ? cand[t] : 0ull;
-        int place = 0;
-        if (t < kept)
-            for (int j = 0; j < kept; ++j) place += cand[j] > mine;
+        // two threads a candidate, each counts half of the others
+        const int item = t & (NT / 2 - 1), half = t / (NT / 2);
+        const unsigned long long mine = item < kept ? cand[item] : 0ull;
+        if (t == 0) cand[kept] = cand[kept + 1] = cand[kept + 2] = 0ull;
+        if (t < NT / 2) sh.list[t] = 0;
         __syncthreads();
-        if (t < kept && place < k) cand[place] = mine;
+        int place = 0;
+        if ((item & ~31) < kept) {
+            const ulonglong2* pairs = reinterpret_cast<const ulonglong2*>(cand);
+            const int quads = (kept + 3) / 4;
+            int other = 0;
+#pragma unroll 4
+            for (int j = half * ((quads + 1) / 2); j < min(quads, (half + 1) * ((quads + 1) / 2)); ++j) {
+                const ulonglong2 p = pairs[2 * j], q = pairs[2 * j + 1];
+                place += (int)(p.x > mine) + (int)(p.y > mine);
+                other += (int)(q.x > mine) + (int)(q.y > mine);
+            }
+            atomicAdd(&sh.list[item], place + other);
+        }
+        __syncthreads();
+        place = half == 0 ? sh.list[item] : k;
+        if (half == 0 && item < kept && place < k) cand[place] = mine;
         __syncthreads();
         if (kept > k) {
             rest.move(K::bound((uint32_t)(cand[k - 1] >> 32)));
-            add_terms(sh.terms, t < kept && place >= k ? grid_term(rest, K::value_of(mine)) : 0.0, rest);
+            add_terms(sh.terms, half == 0 && item < kept && place >= k ? grid_term(rest, K::value_of(mine)) : 0.0, rest);
         }
     } else {
         int size = 256;
