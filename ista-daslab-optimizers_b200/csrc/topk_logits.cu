@@ -13,15 +13,19 @@
 namespace mab {
 namespace toplogits {
 
-constexpr int NT = 512, WARPS = NT / 32;
 constexpr int UNROLL = 4;                          // vectors a thread has in flight
 constexpr int SLOW_UNROLL = 2;                     // vectors a thread holds of a chunk that is selected from exactly
-constexpr int CAP = 3072;                          // candidates
-constexpr int LIST = 3072, REACH = 1536;           // vectors that hold one by the first bound, and by the second
 constexpr int MAX_K = 1024;
-constexpr int ITEMS = CAP / NT;
-constexpr int SAMPLE = 16;                         // most vectors a thread samples
-static_assert(2 * MAX_K <= CAP, "what is held and what a chunk adds have room");
+
+// Lists of up to 128 by CTAs of 256 threads, six on an SM: their chains of phases overlap the others' streams (2048 rows of 128256 bf16, k = 64: 138 us with the larger form).
+template <bool LARGE> struct Form {
+    static constexpr int NT = LARGE ? 512 : 256, WARPS = NT / 32, CTAS = LARGE ? 3 : 6;
+    static constexpr int CAP = LARGE ? 3072 : 1024;             // candidates
+    static constexpr int LIST = LARGE ? 3072 : 1536;            // vectors that hold one by the first bound ...
+    static constexpr int REACH = LARGE ? 1536 : 512;            // ... and by the second
+    static constexpr int MOST_K = LARGE ? MAX_K : 128, ITEMS = CAP / NT;
+    static_assert(2 * MOST_K <= CAP && 8 * MOST_K <= (LARGE ? 8 * MAX_K : CAP), "what is held and what a chunk adds have room, and the lists of a cluster");
+};
 
 struct Args {
     const void* logits;
@@ -31,23 +35,23 @@ struct Args {
     float* rest;
     double tau;
     float scale;
-    int vocab, k, cluster, sample;
+    int vocab, k, cluster, groups, per;
 };
 
-struct Shared {
-    unsigned long long cand[CAP];
-    int list[LIST];                                 // vectors with a value above the bound ...
-    uint32_t list_key[LIST];                        // ... and the keys of their largest
-    int reach[REACH];                               // those that reach the second bound
+template <class F> struct Shared {
+    unsigned long long cand[F::CAP];
+    int list[F::LIST];                                 // vectors with a value above the bound ...
+    uint32_t list_key[F::LIST];                        // ... and the keys of their largest
+    int reach[F::REACH];                               // those that reach the second bound
     int n_list, n_reach;
-    double red[WARPS];
+    double red[F::WARPS];
     double peer_sum[8], peer_ref[8];                // of the cluster's CTAs: sum over the rest, its reference (infinite: far), number of candidates
     uint32_t peer_n[8];
-    int n;                                          // candidates (counts beyond CAP where they do not fit)
+    int n;                                          // candidates (counts beyond F::CAP where they do not fit)
     int count[64];                                  // counters of a bisection, one per step
-    uint32_t warp_max[WARPS], found;
+    uint32_t warp_max[F::WARPS], found;
     int scan[40];
-    double terms[WARPS];                            // of candidates that go into the rest
+    double terms[F::WARPS];                            // of candidates that go into the rest
 };                                                  //   a sum of integers does not depend on it
 
 // Order keys of as many bits as the type has; NaN (0) below -inf, one key for the two zeros.
@@ -89,27 +93,27 @@ __device__ __forceinline__ double grid_term(const Rest& rest, float x) {
     return __dadd_rn(__dadd_rn(d, 24576.0), -24576.0);
 }
 // Adds the block's terms to the rest, in the first thread.
-__device__ __forceinline__ void add_terms(double* parts, double mine, Rest& rest) {
+template <class F> __device__ __forceinline__ void add_terms(double* parts, double mine, Rest& rest) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
     if (lane_id() == 0) parts[warp_id()] = mine;
     __syncthreads();
     if (warp_id() == 0) {
-        double all = lane_id() < WARPS ? parts[lane_id()] : 0.0;
+        double all = lane_id() < F::WARPS ? parts[lane_id()] : 0.0;
 #pragma unroll
-        for (int o = WARPS / 2; o; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+        for (int o = F::WARPS / 2; o; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
         if (lane_id() == 0) rest.s += (float)all;
     }
 }
 
 // Sum of one int per thread, step `i` of a bisection: counters are cleared by `clear_counts`, each is used once.
-__device__ __forceinline__ int block_count(Shared& sh, int c, int i) {
+template <class F> __device__ __forceinline__ int block_count(Shared<F>& sh, int c, int i) {
     c = __reduce_add_sync(0xffffffffu, c);
     if (lane_id() == 0 && c) atomicAdd(&sh.count[i], c);
     __syncthreads();
     return sh.count[i];
 }
-__device__ __forceinline__ void clear_counts(Shared& sh) {
+template <class F> __device__ __forceinline__ void clear_counts(Shared<F>& sh) {
     __syncthreads();
     if (threadIdx.x < 64) sh.count[threadIdx.x] = 0;
     __syncthreads();
@@ -117,7 +121,7 @@ __device__ __forceinline__ void clear_counts(Shared& sh) {
 
 // Largest key T in [lo, hi] with count(>= T) >= k, or any with count(>= T) in [k, most], `counted(mid)` being the calling thread's number of keys >= mid.
 // Needs count(>= lo) >= k, count(> hi) < k.  `reached`: count(>= T).
-template <typename F> __device__ __forceinline__ uint32_t kth_key(Shared& sh, uint32_t lo, uint32_t hi, int k, int most, int& reached, F counted) {
+template <class F, typename G> __device__ __forceinline__ uint32_t kth_key(Shared<F>& sh, uint32_t lo, uint32_t hi, int k, int most, int& reached, G counted) {
     clear_counts(sh);
     reached = 0x7FFFFFFF;
     for (int i = 0; lo < hi; ++i) {
@@ -133,7 +137,7 @@ template <typename F> __device__ __forceinline__ uint32_t kth_key(Shared& sh, ui
 
 // The same for keys[0 .. n) in shared memory, n <= 32 PER, by the first warp alone: no barrier in its steps, and the other warps' slots are free for the SM's other
 // CTAs.  The range is first narrowed in growing steps from where the answer is expected.  The answer is in every thread after the barrier at the end.
-template <typename T, bool FROM_TOP, int PER> __device__ __forceinline__ uint32_t kth_by_warp(Shared& sh, const uint32_t* keys, int n, uint32_t lo, uint32_t hi, int k, int most) {
+template <typename T, bool FROM_TOP, int PER, class F> __device__ __forceinline__ uint32_t kth_by_warp(Shared<F>& sh, const uint32_t* keys, int n, uint32_t lo, uint32_t hi, int k, int most) {
     if (warp_id() == 0) {
         uint32_t key[PER];
 #pragma unroll
@@ -160,72 +164,77 @@ template <typename T, bool FROM_TOP, int PER> __device__ __forceinline__ uint32_
     return sh.found;
 }
 
-// The key of the k-th largest of n >= k keys, or one between that and the (k + slack)-th; all lie in [lo, hi], n <= LIST.
-template <typename T> __device__ __noinline__ uint32_t kth_of_list(Shared& sh, int n, int k, int slack, uint32_t lo, uint32_t hi) {
+// The key of the k-th largest of n >= k keys, or one between that and the (k + slack)-th; all lie in [lo, hi], n <= F::LIST.
+template <typename T, class F> __device__ __noinline__ uint32_t kth_of_list(Shared<F>& sh, int n, int k, int slack, uint32_t lo, uint32_t hi) {
     const int t = threadIdx.x;
     if (n <= 512) return kth_by_warp<T, false, 16>(sh, sh.list_key, n, lo, hi, k, k + slack);
     if (n <= 1024) return kth_by_warp<T, false, 32>(sh, sh.list_key, n, lo, hi, k, k + slack);
     int reached;
     return kth_key(sh, lo, hi, k, k + slack, reached, [&](uint32_t mid) {
         int r = 0;
-        for (int i = t; i < n; i += NT) r += sh.list_key[i] >= mid;
+        for (int i = t; i < n; i += F::NT) r += sh.list_key[i] >= mid;
         return r;
     });
 }
 
-// A key that at least k values of the whole vectors [w0, w1) reach, near the k-th largest: of the maxima of vectors spread evenly over them.
-// NEG_INF where there are not enough.
-template <typename T> __device__ __noinline__ uint32_t bound_of_sample(Shared& sh, const RowGrid<T>& g, int w0, int w1, int k, int sample) {
+// A key that at least k values of the whole vectors [w0, w1) reach, near the k-th largest: of the maxima of `groups` groups a thread of `per` vectors each, spread
+// evenly over them.  NEG_INF where there are not enough.
+template <typename T, class F> __device__ __noinline__ uint32_t bound_of_sample(Shared<F>& sh, const RowGrid<T>& g, int w0, int w1, int k, int groups, int per) {
     using K = Key<T>;
-    const int every = (max(w1 - w0, 0) + 31) / 32, groups = min(sample * WARPS, every), apart = groups ? every / groups * 32 : 0;
+    const int total = groups * per, every = (max(w1 - w0, 0) + 31) / 32, runs = min(total * F::WARPS, every), apart = runs ? every / runs * 32 : 0;
     auto maximum = [&](int u) {                     // of the u-th vector of this thread
-        const int j = u * WARPS + warp_id(), v = w0 + j * apart + lane_id();
-        return u < sample && j < groups && v < w1 ? vector_max(g.load(v), (const T*)nullptr) : -INF_F;
+        const int j = u * F::WARPS + warp_id(), v = w0 + j * apart + lane_id();
+        return u < total && j < runs && v < w1 ? vector_max(g.load(v), (const T*)nullptr) : -INF_F;
     };
-    auto largest = [&](uint32_t top) {
-        top = __reduce_max_sync(0xffffffffu, top);
-        if (lane_id() == 0) sh.warp_max[warp_id()] = top;
-        __syncthreads();
-        return max(__reduce_max_sync(0xffffffffu, sh.warp_max[lane_id() & (WARPS - 1)]), K::NEG_INF);
-    };
-    if (k <= NT / 4) {                              // the threads' maxima are enough of them
-        float m[4], top = -INF_F;
-        for (int b = 0; b < sample; b += 4) {
+    uint32_t top = 0;
+    float m[4], of_group = -INF_F;
+    int in_group = 0, group = 0;
+    for (int b = 0; b < total; b += 4) {
 #pragma unroll
-            for (int u = 0; u < 4; ++u) m[u] = maximum(b + u);
-            top = fmaxf(top, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])));
+        for (int u = 0; u < 4; ++u) m[u] = maximum(b + u);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (b + u >= total) break;
+            of_group = fmaxf(of_group, m[u]);
+            if (++in_group == per) {
+                const uint32_t key = K::of(of_group);
+                sh.list_key[group++ * F::NT + threadIdx.x] = key;
+                top = max(top, key);
+                in_group = 0;
+                of_group = -INF_F;
+            }
         }
-        const uint32_t mine = K::of(top);
-        sh.list_key[threadIdx.x] = mine;
-        const uint32_t most = largest(mine);
-        return kth_by_warp<T, true, NT / 32>(sh, sh.list_key, NT, K::NEG_INF, most, k, k + k / 8);
     }
-    uint32_t key[SAMPLE], top = 0;
-#pragma unroll
-    for (int u = 0; u < SAMPLE; ++u) { key[u] = K::of(maximum(u)); top = max(top, key[u]); }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (lane_id() == 0) sh.warp_max[warp_id()] = top;
+    __syncthreads();
+    top = max(__reduce_max_sync(0xffffffffu, sh.warp_max[lane_id() & (F::WARPS - 1)]), K::NEG_INF);
+    const int n = groups * F::NT;
+    if (n <= 256) return kth_by_warp<T, true, 8>(sh, sh.list_key, n, K::NEG_INF, top, k, k + k / 8);
+    if (n <= 512) return kth_by_warp<T, true, 16>(sh, sh.list_key, n, K::NEG_INF, top, k, k + k / 8);
+    if (n <= 1024) return kth_by_warp<T, true, 32>(sh, sh.list_key, n, K::NEG_INF, top, k, k + k / 8);
     int reached;
-    return kth_key(sh, K::NEG_INF, largest(top), k, k + k / 8, reached, [&](uint32_t mid) {
+    return kth_key(sh, K::NEG_INF, top, k, k + k / 8, reached, [&](uint32_t mid) {
         int r = 0;
-#pragma unroll
-        for (int u = 0; u < SAMPLE; ++u) r += key[u] >= mid;
+        for (int i = threadIdx.x; i < n; i += F::NT) r += sh.list_key[i] >= mid;
         return r;
     });
 }
 
-// Of the n > k candidates (n <= CAP) those from the k-th on stay, in no order, k to k + slack of them; the others go into the rest, relative to a bound below
+// Of the n > k candidates (n <= F::CAP) those from the k-th on stay, in no order, k to k + slack of them; the others go into the rest, relative to a bound below
 // the former.  Returns the bound's key; [lo, hi] holds all keys.
-template <typename T> __device__ __noinline__ uint32_t prune(Shared& sh, int k, int slack, uint32_t lo, uint32_t hi, Rest& rest) {
+template <typename T, class F> __device__ __noinline__ uint32_t prune(Shared<F>& sh, int k, int slack, uint32_t lo, uint32_t hi, Rest& rest) {
     const int t = threadIdx.x, n = sh.n;
-    unsigned long long c[ITEMS];
+    unsigned long long c[F::ITEMS];
     int reached;
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i) c[i] = t + i * NT < n ? sh.cand[t + i * NT] : 0ull;
+    for (int i = 0; i < F::ITEMS; ++i) c[i] = t + i * F::NT < n ? sh.cand[t + i * F::NT] : 0ull;
     const uint32_t key = kth_key(sh, lo, hi, k, k + slack, reached, [&](uint32_t mid) {
         int r = 0;
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-            if (i * NT >= n) break;
-            r += t + i * NT < n && (uint32_t)(c[i] >> 32) >= mid;
+        for (int i = 0; i < F::ITEMS; ++i) {
+            if (i * F::NT >= n) break;
+            r += t + i * F::NT < n && (uint32_t)(c[i] >> 32) >= mid;
         }
         return r;
     });
@@ -234,12 +243,12 @@ template <typename T> __device__ __noinline__ uint32_t prune(Shared& sh, int k, 
         clear_counts(sh);
         int above = 0;
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i) above += t + i * NT < n && (uint32_t)(c[i] >> 32) > key;
+        for (int i = 0; i < F::ITEMS; ++i) above += t + i * F::NT < n && (uint32_t)(c[i] >> 32) > key;
         above = block_count(sh, above, 0);
         last |= kth_key(sh, 0xFFFFFFFFu - (uint32_t)MAB_MAX_VOCAB, 0xFFFFFFFFu, k - above, k - above, reached, [&](uint32_t mid) {
             int r = 0;
 #pragma unroll
-            for (int i = 0; i < ITEMS; ++i) r += t + i * NT < n && (uint32_t)(c[i] >> 32) == key && (uint32_t)c[i] >= mid;
+            for (int i = 0; i < F::ITEMS; ++i) r += t + i * F::NT < n && (uint32_t)(c[i] >> 32) == key && (uint32_t)c[i] >= mid;
             return r;
         });
     }
@@ -249,18 +258,18 @@ template <typename T> __device__ __noinline__ uint32_t prune(Shared& sh, int k, 
     rest.move(Key<T>::bound(key));
     double terms = 0.0;
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-        if (t + i * NT >= n) break;
+    for (int i = 0; i < F::ITEMS; ++i) {
+        if (t + i * F::NT >= n) break;
         if (c[i] >= last) sh.cand[atomicAdd(&sh.n, 1)] = c[i];
         else terms += grid_term(rest, Key<T>::value_of(c[i]));
     }
-    add_terms(sh.terms, terms, rest);
+    add_terms<F>(sh.terms, terms, rest);
     return key;
 }
 
 // The candidates and the rest of the vectors [v0, v1), whatever they hold: every chunk's k largest that lie above the bound are found exactly, in
 // registers; the bound is the k-th of the chunk before, and of all candidates whenever those outgrow their room.
-template <typename T> __device__ __noinline__ void select_slowly(Shared& sh, const RowGrid<T>& g, int v0, int v1, int k, Rest& rest) {
+template <typename T, class F> __device__ __noinline__ void select_slowly(Shared<F>& sh, const RowGrid<T>& g, int v0, int v1, int k, Rest& rest) {
     constexpr int N = RowGrid<T>::N;
     using K = Key<T>;
     const int t = threadIdx.x;
@@ -268,12 +277,12 @@ template <typename T> __device__ __noinline__ void select_slowly(Shared& sh, con
     if (t == 0) sh.n = 0;
     rest.s = rest.ref = 0.0f;
     uint32_t floor_key = 0;                         // smaller keys cannot be among the k largest any more
-    for (int base = v0; base < v1; base += NT * SLOW_UNROLL) {
+    for (int base = v0; base < v1; base += F::NT * SLOW_UNROLL) {
         float x[SLOW_UNROLL][N];
         uint32_t valid[SLOW_UNROLL];                // bits of the elements that are there
 #pragma unroll
         for (int u = 0; u < SLOW_UNROLL; ++u) {
-            const int v = base + u * NT + t;
+            const int v = base + u * F::NT + t;
             valid[u] = 0;
             if (v < v1) {
                 if (g.whole(v)) unpack(g.load(v), x[u], (const T*)nullptr);
@@ -312,24 +321,24 @@ template <typename T> __device__ __noinline__ void select_slowly(Shared& sh, con
                 if (!(valid[u] >> i & 1u)) continue;
                 const uint32_t key = K::of(x[u][i]);
                 if (key > kth || (key == kth && (need == 0x7FFFFFFF || before++ < need)))
-                    sh.cand[atomicAdd(&sh.n, 1)] = K::composite(x[u][i], g.first(base + u * NT + t) + i);
+                    sh.cand[atomicAdd(&sh.n, 1)] = K::composite(x[u][i], g.first(base + u * F::NT + t) + i);
                 else rest.add(x[u][i]);
             }
             if (need != 0x7FFFFFFF) need = max(0, need - total);
             __syncthreads();
         }
         if (eligible > k) floor_key = kth + 1u;     // k values from the k-th on are held, with lower indices than all that follow
-        if (sh.n > CAP - k) floor_key = prune<T>(sh, k, 0, 0u, K::MOST, rest) + 1u;
+        if (sh.n > F::CAP - k) floor_key = prune<T>(sh, k, 0, 0u, K::MOST, rest) + 1u;
     }
     __syncthreads();
 }
 
-template <typename T>
-__global__ void __launch_bounds__(NT, 3) topk_logits_kernel(Args a) {
+template <typename T, class F>
+__global__ void __launch_bounds__(F::NT, F::CTAS) topk_logits_kernel(Args a) {
     constexpr int N = RowGrid<T>::N;
     using K = Key<T>;
     extern __shared__ __align__(16) unsigned char dyn[];
-    Shared& sh = *reinterpret_cast<Shared*>(dyn);
+    Shared<F>& sh = *reinterpret_cast<Shared<F>*>(dyn);
     const int C = a.cluster, rank = C > 1 ? (int)(blockIdx.x % C) : 0, t = threadIdx.x, k = a.k;
     if (C > 1) cluster_arrive();
     const int64_t row = blockIdx.x / C;
@@ -341,10 +350,10 @@ __global__ void __launch_bounds__(NT, 3) topk_logits_kernel(Args a) {
     float bound = -INF_F;                           // values above it are candidates
     uint32_t lo_key = 0, top_key = K::MOST;         // no candidate's key lies outside
     bool slow = false;
-    const bool all = (v1 - v0) * N <= CAP;          // everything is a candidate
+    const bool all = (v1 - v0) * N <= F::CAP;          // everything is a candidate
 
     if (!all) {
-        const uint32_t at = bound_of_sample<T>(sh, g, w0, w1, k, a.sample);
+        const uint32_t at = bound_of_sample<T>(sh, g, w0, w1, k, a.groups, a.per);
         slow = at == K::NEG_INF;                    // fewer than k numbers among the maxima
         if (!slow) {
             bound = K::below(at);
@@ -360,7 +369,7 @@ __global__ void __launch_bounds__(NT, 3) topk_logits_kernel(Args a) {
             const float m = vector_max(r, (const T*)nullptr);
             if (m > bound) {
                 const int at = atomicAdd(&sh.n_list, 1);
-                if (at < LIST) { sh.list[at] = v; sh.list_key[at] = K::of(m); }
+                if (at < F::LIST) { sh.list[at] = v; sh.list_key[at] = K::of(m); }
             } else {
                 uint64_t x[N / 2];
                 unpack_pairs(r, x, (const T*)nullptr);
@@ -374,18 +383,18 @@ __global__ void __launch_bounds__(NT, 3) topk_logits_kernel(Args a) {
         };
         auto push = [&](float x, int e) {
             const int at = atomicAdd(&sh.n, 1);
-            if (at < CAP) sh.cand[at] = K::composite(x, e);
+            if (at < F::CAP) sh.cand[at] = K::composite(x, e);
         };
         if (!all) {
             int v = w0 + t;
-            for (; v + (UNROLL - 1) * NT < w1; v += UNROLL * NT) {
+            for (; v + (UNROLL - 1) * F::NT < w1; v += UNROLL * F::NT) {
                 uint4 r[UNROLL];
 #pragma unroll
-                for (int u = 0; u < UNROLL; ++u) r[u] = g.load(v + u * NT);
+                for (int u = 0; u < UNROLL; ++u) r[u] = g.load(v + u * F::NT);
 #pragma unroll
-                for (int u = 0; u < UNROLL; ++u) see(r[u], v + u * NT);
+                for (int u = 0; u < UNROLL; ++u) see(r[u], v + u * F::NT);
             }
-            for (; v < w1; v += NT) see(g.load(v), v);
+            for (; v < w1; v += F::NT) see(g.load(v), v);
         }
         float lo, hi;
         split(sum, lo, hi);
@@ -393,7 +402,7 @@ __global__ void __launch_bounds__(NT, 3) topk_logits_kernel(Args a) {
         __syncthreads();
         // the vectors of the list (or all), element by element.  As many vectors as k reach the k-th of their largest: a bound nearer to the k-th value
         const int listed = all ? w1 - w0 : sh.n_list;
-        slow = listed > LIST;
+        slow = listed > F::LIST;
         if (!slow && !all) {
             lo_key = kth_of_list<T>(sh, listed, k, k / 8, lo_key, top_key);
             bound = K::below(lo_key);
@@ -401,14 +410,14 @@ __global__ void __launch_bounds__(NT, 3) topk_logits_kernel(Args a) {
         }
         double terms = 0.0;
         if (all) {
-            for (int i = t; i < listed * N; i += NT) push(Elem<T>::load(g.p, g.first(w0) + i), g.first(w0) + i);
+            for (int i = t; i < listed * N; i += F::NT) push(Elem<T>::load(g.p, g.first(w0) + i), g.first(w0) + i);
         } else if (!slow) {
             // vectors below the new bound go into the sum; of the others, which are some k, a thread has an element at a time
-            for (int j = t; j < listed; j += NT) {
+            for (int j = t; j < listed; j += F::NT) {
                 const int v = sh.list[j];
                 if (sh.list_key[j] >= lo_key) {
                     const int at = atomicAdd(&sh.n_reach, 1);
-                    if (at < REACH) sh.reach[at] = v;
+                    if (at < F::REACH) sh.reach[at] = v;
                     continue;
                 }
                 float x[N];
@@ -418,9 +427,9 @@ __global__ void __launch_bounds__(NT, 3) topk_logits_kernel(Args a) {
             }
             __syncthreads();
             const int reaching = sh.n_reach;
-            slow = reaching > REACH;
+            slow = reaching > F::REACH;
             if (!slow)
-                for (int i = t; i < reaching * N; i += NT) {
+                for (int i = t; i < reaching * N; i += F::NT) {
                     const int e = g.first(sh.reach[i / N]) + i % N;
                     const float x = Elem<T>::load(g.p, e);
                     if (x > bound) push(x, e);
@@ -439,8 +448,8 @@ __global__ void __launch_bounds__(NT, 3) topk_logits_kernel(Args a) {
                 }
             }
         }
-        add_terms(sh.terms, terms, rest);
-        slow |= sh.n > CAP;
+        add_terms<F>(sh.terms, terms, rest);
+        slow |= sh.n > F::CAP;
     }
     if (slow) {
         select_slowly<T>(sh, g, v0, v1, k, rest);
@@ -448,7 +457,7 @@ __global__ void __launch_bounds__(NT, 3) topk_logits_kernel(Args a) {
     }
 
     if (C > 1) {                                    // the first CTA takes over the others' candidates and sums
-        if (sh.n > CAP / C) prune<T>(sh, k, CAP / C - k, lo_key, K::MOST, rest);      // (what all of them have fits the first one's room)
+        if (sh.n > F::CAP / C) prune<T>(sh, k, F::CAP / C - k, lo_key, K::MOST, rest);      // (what all of them have fits the first one's room)
         lo_key = 0;                                 // (the others' bounds are others)
         float s = rest.s;
 #pragma unroll
@@ -458,7 +467,7 @@ __global__ void __launch_bounds__(NT, 3) topk_logits_kernel(Args a) {
         cluster_wait();
         if (t < C) {                                // everybody learns how many candidates everybody has, the first CTA the sums, too
             double sum = 0.0;
-            for (int i = 0; i < WARPS; ++i) sum += sh.red[i];
+            for (int i = 0; i < F::WARPS; ++i) sum += sh.red[i];
             cluster_store_u32(&sh.peer_n[rank], t, (uint32_t)sh.n);
             cluster_store_f64(&sh.peer_sum[rank], t, sum);
             cluster_store_f64(&sh.peer_ref[rank], t, rest.far ? (double)INF_F : (double)rest.ref);
@@ -478,7 +487,7 @@ __global__ void __launch_bounds__(NT, 3) topk_logits_kernel(Args a) {
         } else {
             int at = 0;
             for (int c = 0; c < rank; ++c) at += (int)sh.peer_n[c];
-            for (int i = t; i < n; i += NT) cluster_store_u64(&sh.cand[at + i], 0, sh.cand[i]);
+            for (int i = t; i < n; i += F::NT) cluster_store_u64(&sh.cand[at + i], 0, sh.cand[i]);
         }
         cluster_arrive_wait();
         if (rank != 0) return;
@@ -490,46 +499,41 @@ __global__ void __launch_bounds__(NT, 3) topk_logits_kernel(Args a) {
         __syncthreads();
     }
     // those from the k-th on, in order: a few by the number of larger ones, many by a sorting network
-    const bool few = k <= 128;
+    constexpr bool few = F::MOST_K <= 128;
     if (sh.n > (few ? 192 : k)) prune<T>(sh, k, few ? 64 : 0, lo_key, K::MOST, rest);
     unsigned long long* cand = sh.cand;
     const int kept = sh.n;                          // k, or up to 192 where few
     if (few) {
-        // two threads a candidate, each counts half of the others
-        const int item = t & (NT / 2 - 1), half = t / (NT / 2);
-        const unsigned long long mine = item < kept ? cand[item] : 0ull;
-        if (t == 0) cand[kept] = cand[kept + 1] = cand[kept + 2] = 0ull;
-        if (t < NT / 2) sh.list[t] = 0;
+        const unsigned long long mine = t < kept ? cand[t] : 0ull;
+        if (t < 3) cand[kept + t] = 0ull;
         __syncthreads();
         int place = 0;
-        if ((item & ~31) < kept) {
+        if ((t & ~31) < kept) {
             const ulonglong2* pairs = reinterpret_cast<const ulonglong2*>(cand);
-            const int quads = (kept + 3) / 4;
             int other = 0;
 #pragma unroll 4
-            for (int j = half * ((quads + 1) / 2); j < min(quads, (half + 1) * ((quads + 1) / 2)); ++j) {
+            for (int j = 0; j < (kept + 3) / 4; ++j) {
                 const ulonglong2 p = pairs[2 * j], q = pairs[2 * j + 1];
                 place += (int)(p.x > mine) + (int)(p.y > mine);
                 other += (int)(q.x > mine) + (int)(q.y > mine);
             }
-            atomicAdd(&sh.list[item], place + other);
+            place += other;
         }
         __syncthreads();
-        place = half == 0 ? sh.list[item] : k;
-        if (half == 0 && item < kept && place < k) cand[place] = mine;
+        if (t < kept && place < k) cand[place] = mine;
         __syncthreads();
         if (kept > k) {
             rest.move(K::bound((uint32_t)(cand[k - 1] >> 32)));
-            add_terms(sh.terms, half == 0 && item < kept && place >= k ? grid_term(rest, K::value_of(mine)) : 0.0, rest);
+            add_terms<F>(sh.terms, t < kept && place >= k ? grid_term(rest, K::value_of(mine)) : 0.0, rest);
         }
     } else {
         int size = 256;
         while (size < k) size *= 2;
-        for (int i = k + t; i < size; i += NT) cand[i] = 0ull;
+        for (int i = k + t; i < size; i += F::NT) cand[i] = 0ull;
         for (int block = 2; block <= size; block *= 2)
             for (int d = block / 2; d; d /= 2) {
                 __syncthreads();
-                for (int i = t; i < size / 2; i += NT) {
+                for (int i = t; i < size / 2; i += F::NT) {
                     const int p = 2 * i - (i & (d - 1)), q = p + d;
                     const unsigned long long x = cand[p], y = cand[q];
                     if ((x < y) == ((p & block) == 0)) { cand[p] = y; cand[q] = x; }
@@ -537,7 +541,7 @@ __global__ void __launch_bounds__(NT, 3) topk_logits_kernel(Args a) {
             }
         __syncthreads();
     }
-    for (int i = t; i < k; i += NT) {
+    for (int i = t; i < k; i += F::NT) {
         const unsigned long long c = cand[i];
         const int e = index_of(c);
         a.indices[row * k + i] = e;
@@ -550,13 +554,13 @@ __global__ void __launch_bounds__(NT, 3) topk_logits_kernel(Args a) {
     if (lane_id() == 0) sh.red[warp_id()] = (double)s;
     __syncthreads();
     double sum = 0.0;
-    for (int i = 0; i < WARPS; ++i) sum += sh.red[i];
+    for (int i = 0; i < F::WARPS; ++i) sum += sh.red[i];
     double ref = (double)rest.ref * 0.69314718055994531;
     const unsigned long long last = cand[k - 1];
     if (a.vocab > k && (rest.far || (sum == sum && !(sum >= 1e-3)))) {
         // nothing to speak of relative to the bound (masked logits, a gap), or infinities: again, relative to the largest of the rest
         float m = -INF_F, bad = 0.0f;
-        for (int e = t; e < a.vocab; e += NT) {
+        for (int e = t; e < a.vocab; e += F::NT) {
             const float x = Elem<T>::load(g.p, e);
             if (x != x) bad = x;
             else if (K::composite(x, e) < last) m = fmaxf(m, x);
@@ -565,10 +569,10 @@ __global__ void __launch_bounds__(NT, 3) topk_logits_kernel(Args a) {
         if (lane_id() == 0) sh.warp_max[warp_id()] = top;
         __syncthreads();
         m = -INF_F;
-        for (int i = 0; i < WARPS; ++i) m = fmaxf(m, ord_value(sh.warp_max[i]));
+        for (int i = 0; i < F::WARPS; ++i) m = fmaxf(m, ord_value(sh.warp_max[i]));
         double part = (double)bad;
         if (m != -INF_F && m != INF_F)
-            for (int e = t; e < a.vocab; e += NT) {
+            for (int e = t; e < a.vocab; e += F::NT) {
                 const float x = Elem<T>::load(g.p, e);
                 if (x == x && K::composite(x, e) < last) part += (double)ex2((x - m) * a.scale);
             }
@@ -578,23 +582,30 @@ __global__ void __launch_bounds__(NT, 3) topk_logits_kernel(Args a) {
         if (lane_id() == 0) sh.red[warp_id()] = part;
         __syncthreads();
         sum = 0.0;
-        for (int i = 0; i < WARPS; ++i) sum += sh.red[i];
+        for (int i = 0; i < F::WARPS; ++i) sum += sh.red[i];
         ref = m == -INF_F ? 0.0 : (double)m / a.tau;
         if (m == INF_F && sum == sum) sum = 1.0;
     }
     if (t == 0) a.rest[row] = sum == 0.0 ? -INF_F : (float)(ref + log(sum));
 }
 
-template <typename T> int launch(Args a, int64_t rows, cudaStream_t s) {
-    const int sms = device_sm_count();
-    if (sms < 0) return MAB_ERR_CUDA;
+template <typename T, class F> int launch_form(Args a, int64_t rows, int sms, cudaStream_t s) {
     // CTAs of a row: until every SM has one, no part below 4 KB, and the merged lists fit the candidates' room
     a.cluster = 1;
-    while (a.cluster < 8 && rows * a.cluster * 2 <= sms && (int64_t)a.vocab * sizeof(T) / (2 * a.cluster) >= 4096 && 2 * a.cluster * a.k <= CAP) a.cluster *= 2;
-    // vectors a thread samples: so many that some k (part / sample) candidates fit, a quarter of the room for what the sample does not show
+    while (a.cluster < 8 && rows * a.cluster * 2 <= sms && (int64_t)a.vocab * sizeof(T) / (2 * a.cluster) >= 4096 && 2 * a.cluster * a.k <= F::CAP) a.cluster *= 2;
+    // the sample: an eighth of a row of 128256 bf16 at least (2048 vectors), and so many that some k (part / sample) vectors fit the list, a quarter of it for what the
+    // sample does not show; in four times as many groups as k, as far as the list's room goes
     const int64_t part = ((int64_t)a.vocab / RowGrid<T>::N + a.cluster) / a.cluster;
-    a.sample = (int)std::min<int64_t>(SAMPLE, std::max<int64_t>(4, ceil_div64(part * a.k, (int64_t)NT * CAP * 3 / 4)));
-    return launch_rows(topk_logits_kernel<T>, "topk_logits", rows * a.cluster, NT, sizeof(Shared), a.cluster, s, a);
+    const int each = (int)std::max<int64_t>(2048 / F::NT, std::min<int64_t>(64, ceil_div64(part * a.k, (int64_t)F::NT * F::LIST * 3 / 4)));
+    a.groups = std::min({F::LIST / F::NT, each, std::max(1, (4 * a.k + F::NT - 1) / F::NT)});
+    a.per = (each + a.groups - 1) / a.groups;
+    return launch_rows(topk_logits_kernel<T, F>, "topk_logits", rows * a.cluster, F::NT, sizeof(Shared<F>), a.cluster, s, a);
+}
+
+template <typename T> int launch(const Args& a, int64_t rows, cudaStream_t s) {
+    const int sms = device_sm_count();
+    if (sms < 0) return MAB_ERR_CUDA;
+    return a.k <= Form<false>::MOST_K ? launch_form<T, Form<false>>(a, rows, sms, s) : launch_form<T, Form<true>>(a, rows, sms, s);
 }
 
 }  // namespace toplogits
