@@ -13,6 +13,7 @@
 // optimum the loss is what is left of a difference, and there an error of S_t only enters with the factor q_t - p_t as long as the terms that share it are exact.
 // Rows too long for that are read twice, with a bitmap of the list's positions.  The CTAs exchange five numbers through distributed shared memory, in rank order:
 // results do not depend on timing.
+#include <type_traits>
 #include "rows.cuh"
 #include "async_copy.cuh"
 
@@ -156,10 +157,11 @@ __device__ __forceinline__ void zero_part(const Args& a, int64_t row, int part, 
     write_zeros<T, THREADS>(out, a.vocab, v0, v1);
 }
 
-// RESIDENT: the part of the row is in shared memory; otherwise only its first `a.held` whole vectors are.
-template <typename T, int MODE, bool RESIDENT, int NT>
-__global__ void __launch_bounds__(NT, 1024 / NT) distill_kernel(Args a) {
-    constexpr int N = RowGrid<T>::N, WARPS = NT / 32, PER_THREAD = MAX_K / NT;
+// RESIDENT: the part of the row is in shared memory; otherwise only its first `a.held` whole vectors are.  PER_THREAD: entries of the list a thread has.  Threads an
+// SM (us, 1024 / 1280 / 1536): loss of 1536 rows of 128256 bf16 86 / 84 / 80, step of 2048 rows of 50257 bf16 96 / 94 / 107.
+template <typename T, int MODE, bool RESIDENT, int NT, int PER_THREAD>
+__global__ void __launch_bounds__(NT, (PER_THREAD > 1 ? 1024 : MODE == LOSS ? 1536 : 1280) / NT) distill_kernel(Args a) {
+    constexpr int N = RowGrid<T>::N, WARPS = NT / 32;
     extern __shared__ __align__(16) unsigned char dyn[];
     __shared__ Shared sh;
     const int C = a.cluster, rank = C > 1 ? (int)(blockIdx.x % C) : 0, t = threadIdx.x, k = a.k;
@@ -521,12 +523,17 @@ template <typename T, int MODE> int launch(Args a, int64_t rows, cudaStream_t s)
     }
     const size_t list = ((size_t)a.k * 12 + 15) / 16 * 16;
     const size_t vectors = ((size_t)a.vocab / N + 2 + a.cluster - 1) / a.cluster, bits = (vectors * N + 31) / 32 * 4;
-    if (vectors * 16 <= PART)
-        return launch_rows(distill_kernel<T, MODE, true, 256>, "distill", rows * a.cluster, 256, list + vectors * 16, a.cluster, s, a);
-    if (MODE == LOSS || vectors * 16 <= 140 * 1024)
-        return launch_rows(distill_kernel<T, MODE, false, 256>, "distill", rows * a.cluster, 256, list + bits, a.cluster, s, a);
+    auto go = [&](auto resident, auto threads, size_t smem) {
+        constexpr bool RESIDENT = decltype(resident)::value;
+        constexpr int NT = decltype(threads)::value;
+        // (lists of up to an entry a thread leave registers for another CTA)
+        auto* kernel = a.k <= NT ? distill_kernel<T, MODE, RESIDENT, NT, 1> : distill_kernel<T, MODE, RESIDENT, NT, MAX_K / NT>;
+        return launch_rows(kernel, "distill", rows * a.cluster, NT, list + smem, a.cluster, s, a);
+    };
+    if (vectors * 16 <= PART) return go(std::true_type(), std::integral_constant<int, 256>(), vectors * 16);
+    if (MODE == LOSS || vectors * 16 <= 140 * 1024) return go(std::false_type(), std::integral_constant<int, 256>(), bits);
     a.held = (int)std::min<int64_t>((int64_t)vectors, std::max<int64_t>(0, STEP_SHARED - (int64_t)(list + bits)) / 16);
-    return launch_rows(distill_kernel<T, MODE, false, 512>, "distill", rows * a.cluster, 512, list + bits + (size_t)a.held * 16, a.cluster, s, a);
+    return go(std::false_type(), std::integral_constant<int, 512>(), bits + (size_t)a.held * 16);
 }
 
 template <typename T> int launch_grad(Args a, int64_t rows, cudaStream_t s) {

@@ -386,7 +386,7 @@ template <typename T, int BN> int launch_tiles(Args g, int sms, cudaStream_t s) 
             if (load < best) { best = load; g.split = split; g.height = height; }
         }
     const int64_t ctas = (int64_t)g.token_tiles * ceil_div64(g.n, g.height) * g.split;
-    const int stage = (BM + BN) * BK, most = (ctas > sms ? RING_TWO : RING_ONE) / stage;
+    const int stage = (BM + BN) * BK, most = (ctas > sms || g.split > 1 ? RING_TWO : RING_ONE) / stage;
     const int sums = g.split > 1 ? BM * BN * 4 : 0;                        // the partial sums have to fit the ring
     g.stages = std::max({1, std::min({most, MOST_STAGES, (steps + g.split - 1) / g.split}), (sums + stage - 1) / stage});
     CUtensorMap map_a, map_b;
