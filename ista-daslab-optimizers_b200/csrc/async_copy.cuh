@@ -12,6 +12,12 @@ __device__ __forceinline__ void mbar_init(uint64_t* bar, int arrivals) {
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
 }
 
+// The same for a kernel with many: each without the fence, and the fence once behind the last.
+__device__ __forceinline__ void mbar_init_unfenced(uint64_t* bar, int arrivals) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(bar)), "r"(arrivals));
+}
+__device__ __forceinline__ void mbar_init_fence() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
+
 // One arrival that also announces `bytes` of bulk-copy traffic.
 __device__ __forceinline__ void mbar_arrive_expect_tx(uint64_t* bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(bar)), "r"(bytes) : "memory");

@@ -53,8 +53,9 @@ __global__ void __launch_bounds__(THREADS) int8_matmul_kernel(const __grid_const
         tile_g2s(stage + BM * BK, &map_a, i * BK, token0, &full[s]);
     };
     if (t == 0) {
-        for (int i = 0; i < stages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
-        mbar_init(&done, 1);
+        for (int i = 0; i < stages; ++i) { mbar_init_unfenced(&full[i], 1); mbar_init_unfenced(&empty[i], 1); }
+        mbar_init_unfenced(&done, 1);
+        mbar_init_fence();
         s_lost = 0;
         for (int i = k0; i < k1 && i < k0 + stages; ++i) load(i, i - k0);         // (only this thread and the copy engine know of the barriers yet)
     }
@@ -179,8 +180,9 @@ __global__ void __launch_bounds__(PAIR_THREADS) int8_matmul_pair_kernel(const __
     const int warp = warp_id(), lane = lane_id(), t = threadIdx.x, rank = (int)(blockIdx.x & 1), pair = (int)(blockIdx.x >> 1), pairs = (int)(gridDim.x >> 1);
     const int steps = (g.k + BK - 1) / BK;
     if (t == 0) {
-        for (int i = 0; i < PAIR_STAGES; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(&ready[i], 1); mbar_init(&taken[i], 2 * PAIR_WARPS); }
+        for (int i = 0; i < PAIR_STAGES; ++i) { mbar_init_unfenced(&full[i], 1); mbar_init_unfenced(&empty[i], 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init_unfenced(&ready[i], 1); mbar_init_unfenced(&taken[i], 2 * PAIR_WARPS); }
+        mbar_init_fence();
         s_lost = 0;
     }
     if (warp == 1) tmem_alloc_pair(&s_tmem, 512);

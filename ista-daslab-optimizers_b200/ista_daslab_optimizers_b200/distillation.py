@@ -62,55 +62,68 @@ def _no_grad_for(call, **tensors):
             raise N.NativeError(f'{call} has no gradient for {what}: what belongs to a frozen teacher is handed over detached, or under torch.no_grad()')
 
 
-def _done(result, what, explain):
-    """What the native side answers: tensors, a status of the library, or None where an argument is not as it should be."""
+_native_calls = None
+
+
+def _calls():
+    global _native_calls
+    _native_calls = N.load_distill_calls()
+    return _native_calls
+
+
+def _fail(result, what, explain, *args):
+    """What the native side answered instead of tensors: a status of the library, or None where an argument is not as it should be."""
     if result is None:
-        explain()
+        explain(*args)
         raise N.NativeError(f'{what} cannot take these arguments')
-    if isinstance(result, int):
-        N.check(result, what)
-    return result
+    N.check(result, what)
 
 
 def quantize_rows(x, codes=None, scales=None):
     """8-bit codes and one float32 scale per row of x (float32 or bfloat16 [rows, cols]): scale = max |x| / 127, code = the integer nearest
     x / scale, half to even.  A row with a NaN or an infinity gets the scale NaN and zeros.  Returns (codes, scales); codes made here
     lie a multiple of 16 bytes apart, as `int8_matmul` wants them.  Not differentiable."""
-    def explain():
-        _rows(x, 'x')
-        _no_grad_for('quantize_rows', x=x)
-        if codes is not None:
-            _rows(codes, 'codes', (torch.int8,))
-            if codes.shape != x.shape:
-                raise N.NativeError(f'codes must have the shape of x, {tuple(x.shape)} (got {tuple(codes.shape)})')
-            _same_device(x.device, codes=codes)
-        _vector(scales, x.shape[0], 'scales', x.device, optional=True)
-    return _done(N.load_distill_calls().quantize_rows(x, codes, scales), 'quantize_rows', explain)
+    result = (_native_calls or _calls()).quantize_rows(x, codes, scales)
+    return result if type(result) is tuple else _fail(result, 'quantize_rows', _explain_quantize, x, codes, scales)
+
+
+def _explain_quantize(x, codes, scales):
+    _rows(x, 'x')
+    _no_grad_for('quantize_rows', x=x)
+    if codes is not None:
+        _rows(codes, 'codes', (torch.int8,))
+        if codes.shape != x.shape:
+            raise N.NativeError(f'codes must have the shape of x, {tuple(x.shape)} (got {tuple(codes.shape)})')
+        _same_device(x.device, codes=codes)
+    _vector(scales, x.shape[0], 'scales', x.device, optional=True)
 
 
 def int8_matmul(a, b, a_scales, b_scales, bias=None, out=None, dtype=torch.bfloat16):
     """out[i, j] = (sum_c a[i, c] b[j, c]) a_scales[i] b_scales[j] + bias[j] for int8 a [tokens, inner] and b [channels, inner]: the sum exact in
     32-bit integers, then fp32, rounded once to `dtype` (float32 or bfloat16; that of `out` where it is given).  The codes start on 16 bytes and
     their rows lie a multiple of 16 bytes apart (`quantize_rows` makes them so); the inner size is at most 131071.  Not differentiable."""
-    def explain():
-        _rows(a, 'a', (torch.int8,))
-        _rows(b, 'b', (torch.int8,))
-        if a.shape[1] != b.shape[1]:
-            raise N.NativeError(f'a and b have inner sizes {a.shape[1]} and {b.shape[1]}')
-        _same_device(a.device, b=b)
-        m, n = a.shape[0], b.shape[0]
-        _vector(a_scales, m, 'a_scales', a.device)
-        _vector(b_scales, n, 'b_scales', a.device)
-        _vector(bias, n, 'bias', a.device, optional=True)
-        _no_grad_for('int8_matmul', a_scales=a_scales, b_scales=b_scales, bias=bias, out=out)
-        if out is not None:
-            _rows(out, 'out')
-            if out.shape != (m, n):
-                raise N.NativeError(f'out must have the shape {(m, n)} (got {tuple(out.shape)})')
-            _same_device(a.device, out=out)
-    if out is None and dtype not in (torch.float32, torch.bfloat16):
+    if out is None and dtype is not torch.bfloat16 and dtype is not torch.float32:
         raise N.NativeError(f'unsupported element type {dtype}: the kernels write float32 and bfloat16')
-    return _done(N.load_distill_calls().int8_matmul(a, b, a_scales, b_scales, bias, out, dtype is torch.bfloat16), 'int8_matmul', explain)[0]
+    result = (_native_calls or _calls()).int8_matmul(a, b, a_scales, b_scales, bias, out, dtype is torch.bfloat16)
+    return result[0] if type(result) is tuple else _fail(result, 'int8_matmul', _explain_matmul, a, b, a_scales, b_scales, bias, out)
+
+
+def _explain_matmul(a, b, a_scales, b_scales, bias, out):
+    _rows(a, 'a', (torch.int8,))
+    _rows(b, 'b', (torch.int8,))
+    if a.shape[1] != b.shape[1]:
+        raise N.NativeError(f'a and b have inner sizes {a.shape[1]} and {b.shape[1]}')
+    _same_device(a.device, b=b)
+    m, n = a.shape[0], b.shape[0]
+    _vector(a_scales, m, 'a_scales', a.device)
+    _vector(b_scales, n, 'b_scales', a.device)
+    _vector(bias, n, 'bias', a.device, optional=True)
+    _no_grad_for('int8_matmul', a_scales=a_scales, b_scales=b_scales, bias=bias, out=out)
+    if out is not None:
+        _rows(out, 'out')
+        if out.shape != (m, n):
+            raise N.NativeError(f'out must have the shape {(m, n)} (got {tuple(out.shape)})')
+        _same_device(a.device, out=out)
 
 
 def topk_logits(logits, k, temperature=1.0):
@@ -118,13 +131,15 @@ def topk_logits(logits, k, temperature=1.0):
     ties to the lower index, in the logits' type; their int32 indices; and the float32 logarithm of sum exp(logit / temperature) over all others, -inf
     where there is nothing else.  NaN ranks below -inf and makes `rest` NaN.  Not differentiable."""
     k = operator.index(k)
+    result = (_native_calls or _calls()).topk_logits(logits, k, float(temperature))
+    return result if type(result) is tuple else _fail(result, 'topk_logits', _explain_topk, logits, k)
 
-    def explain():
-        _rows(logits, 'logits')
-        _no_grad_for('topk_logits', logits=logits)
-        if not 1 <= k <= logits.shape[1]:
-            raise N.NativeError(f'k={k} is not between 1 and the {logits.shape[1]} logits of a row')
-    return _done(N.load_distill_calls().topk_logits(logits, k, float(temperature)), 'topk_logits', explain)
+
+def _explain_topk(logits, k):
+    _rows(logits, 'logits')
+    _no_grad_for('topk_logits', logits=logits)
+    if not 1 <= k <= logits.shape[1]:
+        raise N.NativeError(f'k={k} is not between 1 and the {logits.shape[1]} logits of a row')
 
 
 def _explain_lists(what, logits, indices, values, rest, weights, temperature):
@@ -159,8 +174,8 @@ def distill_loss(logits, indices, values, rest=None, weights=None, temperature=1
 
     The gradient comes from a second pass over the logits; `distill_step` gives both in one call.  Differentiable once."""
     temperature = float(temperature)
-    return _done(N.load_distill_calls().distill_loss(logits, indices, values, rest, weights, temperature), 'distill_loss',
-                 lambda: _explain_lists('distill_loss', logits, indices, values, rest, weights, temperature))
+    result = (_native_calls or _calls()).distill_loss(logits, indices, values, rest, weights, temperature)
+    return result if result is not None else _fail(result, 'distill_loss', _explain_lists, 'distill_loss', logits, indices, values, rest, weights, temperature)
 
 
 def distill_step(logits, indices, values, rest=None, weights=None, temperature=1.0, grad=None):
@@ -168,12 +183,14 @@ def distill_step(logits, indices, values, rest=None, weights=None, temperature=1
     recorded for autograd: hand the gradient on with `logits.backward(grad)`.  `grad` can be given, and can be the logits' own memory
     (`grad=logits.detach()`): the gradient then replaces them."""
     temperature = float(temperature)
+    result = (_native_calls or _calls()).distill_step(logits, indices, values, rest, weights, temperature, grad)
+    return result if type(result) is tuple else _fail(result, 'distill_step', _explain_step, logits, indices, values, rest, weights, temperature, grad)
 
-    def explain():
-        _explain_lists('distill_step', logits, indices, values, rest, weights, temperature)
-        if grad is not None:
-            if grad.shape != logits.shape or grad.dtype != logits.dtype or grad.requires_grad:
-                raise N.NativeError(f'grad must be like the logits, {tuple(logits.shape)} of {logits.dtype}, and require no gradient itself')
-            _rows(grad, 'grad')
-            _same_device(logits.device, grad=grad)
-    return _done(N.load_distill_calls().distill_step(logits, indices, values, rest, weights, temperature, grad), 'distill_step', explain)
+
+def _explain_step(logits, indices, values, rest, weights, temperature, grad):
+    _explain_lists('distill_step', logits, indices, values, rest, weights, temperature)
+    if grad is not None:
+        if grad.shape != logits.shape or grad.dtype != logits.dtype or grad.requires_grad:
+            raise N.NativeError(f'grad must be like the logits, {tuple(logits.shape)} of {logits.dtype}, and require no gradient itself')
+        _rows(grad, 'grad')
+        _same_device(logits.device, grad=grad)
