@@ -333,6 +333,27 @@ template <typename T, class F> __device__ __noinline__ void select_slowly(Shared
     __syncthreads();
 }
 
+// Descending, n <= MAX_K with zeros behind them up to a power of two, in place.  A stage of a distance of up to 32 stays in the 64 elements that a warp has, so only
+// the others need the whole block's barrier.
+template <class F> __device__ __forceinline__ void sort_descending(unsigned long long* cand, int n) {
+    int size = 64;
+    while (size < n) size *= 2;
+    for (int i = n + threadIdx.x; i < size; i += F::NT) cand[i] = 0ull;
+    int before = size;
+    for (int block = 2; block <= size; block *= 2)
+        for (int d = block / 2; d; d /= 2) {
+            if (d > 32 || before > 32) __syncthreads();
+            else __syncwarp();
+            before = d;
+            for (int i = threadIdx.x; i < size / 2; i += F::NT) {
+                const int p = 2 * i - (i & (d - 1)), q = p + d;
+                const unsigned long long x = cand[p], y = cand[q];
+                if ((x < y) == ((p & block) == 0)) { cand[p] = y; cand[q] = x; }
+            }
+        }
+    __syncthreads();
+}
+
 template <typename T, class F>
 __global__ void __launch_bounds__(F::NT, F::CTAS) topk_logits_kernel(Args a) {
     constexpr int N = RowGrid<T>::N;
@@ -498,11 +519,15 @@ __global__ void __launch_bounds__(F::NT, F::CTAS) topk_logits_kernel(Args a) {
         }
         __syncthreads();
     }
-    // those from the k-th on, in order: a few by the number of larger ones, many by a sorting network
+    // in order: a few by the number of larger ones, many by a sorting network; what lies behind the k-th goes into the rest
     constexpr bool few = F::MOST_K <= 128;
-    if (sh.n > (few ? 192 : k)) prune<T>(sh, k, few ? 64 : 0, lo_key, K::MOST, rest);
+    int most = 192;                                 // a network of k's power of two, not of a larger one: twice the size takes more than the bisection
+    if (!few)
+        for (most = 64; most < k;) most *= 2;
+    if (sh.n > most) prune<T>(sh, k, few ? 64 : most - k, lo_key, K::MOST, rest);
     unsigned long long* cand = sh.cand;
-    const int kept = sh.n;                          // k, or up to 192 where few
+    const int kept = sh.n;
+    unsigned long long behind[few ? 1 : MAX_K / F::NT];
     if (few) {
         const unsigned long long mine = t < kept ? cand[t] : 0ull;
         if (t < 3) cand[kept + t] = 0ull;
@@ -522,24 +547,18 @@ __global__ void __launch_bounds__(F::NT, F::CTAS) topk_logits_kernel(Args a) {
         __syncthreads();
         if (t < kept && place < k) cand[place] = mine;
         __syncthreads();
-        if (kept > k) {
-            rest.move(K::bound((uint32_t)(cand[k - 1] >> 32)));
-            add_terms<F>(sh.terms, t < kept && place >= k ? grid_term(rest, K::value_of(mine)) : 0.0, rest);
-        }
+        behind[0] = t < kept && place >= k ? mine : 0ull;
     } else {
-        int size = 256;
-        while (size < k) size *= 2;
-        for (int i = k + t; i < size; i += F::NT) cand[i] = 0ull;
-        for (int block = 2; block <= size; block *= 2)
-            for (int d = block / 2; d; d /= 2) {
-                __syncthreads();
-                for (int i = t; i < size / 2; i += F::NT) {
-                    const int p = 2 * i - (i & (d - 1)), q = p + d;
-                    const unsigned long long x = cand[p], y = cand[q];
-                    if ((x < y) == ((p & block) == 0)) { cand[p] = y; cand[q] = x; }
-                }
-            }
-        __syncthreads();
+        sort_descending<F>(cand, kept);
+#pragma unroll
+        for (int i = 0; i < (few ? 1 : MAX_K / F::NT); ++i) behind[i] = t + i * F::NT >= k && t + i * F::NT < kept ? cand[t + i * F::NT] : 0ull;
+    }
+    if (kept > k) {
+        rest.move(K::bound((uint32_t)(cand[k - 1] >> 32)));
+        double terms = 0.0;
+#pragma unroll
+        for (int i = 0; i < (few ? 1 : MAX_K / F::NT); ++i) if (behind[i]) terms += grid_term(rest, K::value_of(behind[i]));
+        add_terms<F>(sh.terms, terms, rest);
     }
     for (int i = t; i < k; i += F::NT) {
         const unsigned long long c = cand[i];
