@@ -88,6 +88,11 @@ bool tensor(PyObject* o, at::Tensor* out, bool optional = false) {
 }
 bool wants_gradient(const at::Tensor& t) { return t.defined() && t.requires_grad() && c10::GradMode::is_enabled(); }
 
+// A tensor of the caller's that the library has written to: autograd has to know, where it keeps it (or what shares its memory) for a backward pass.
+void written(const at::Tensor& t, PyObject* given) {
+    if (given != Py_None && !t.is_inference()) torch::autograd::impl::bump_version(t);
+}
+
 PyObject* tuple(std::initializer_list<at::Tensor> tensors) {
     PyObject* r = PyTuple_New(static_cast<Py_ssize_t>(tensors.size()));
     if (r == nullptr) return nullptr;
@@ -138,6 +143,8 @@ PyObject* quantize_rows(PyObject*, PyObject* const* args, Py_ssize_t n) try {
         const ReleasedInterpreter other_threads_run;
         status = g_library.quantize_rows(rows, cols, xr.p, code(x), xr.pitch, static_cast<int8_t*>(cr.p), cr.pitch, vector_at(scales), on.stream);
     }
+    written(codes, args[1]);
+    written(scales, args[2]);
     return answer(status, {codes, scales});
 } catch (...) {
     return raise_python();
@@ -164,6 +171,7 @@ PyObject* int8_matmul(PyObject*, PyObject* const* args, Py_ssize_t n) try {
         status = g_library.int8_matmul(m, channels, k, static_cast<const int8_t*>(ar.p), ar.pitch, static_cast<const int8_t*>(br.p), br.pitch, vector_at(a_scales),
                                        vector_at(b_scales), vector_at(bias), outr.p, code(out), outr.pitch, on.stream);
     }
+    written(out, args[5]);
     return answer(status, {out});
 } catch (...) {
     return raise_python();
@@ -297,6 +305,7 @@ PyObject* distill_step(PyObject*, PyObject* const* args, Py_ssize_t n) try {
         status = g_library.distill_step(l.rows, l.vocab, l.k, l.z.p, code(l.logits), l.z.pitch, static_cast<const int32_t*>(l.indices.data_ptr()), l.values.data_ptr(),
                                         code(l.values), vector_at(l.rest), vector_at(l.weights), temperature, vector_at(loss), g.p, g.pitch, on.stream);
     }
+    written(grad, args[6]);
     return answer(status, {loss, grad});
 } catch (...) {
     return raise_python();

@@ -338,6 +338,74 @@ def test_distill_saved_logits_cannot_change_unnoticed():
         loss.sum().backward()
 
 
+def test_outputs_that_autograd_keeps_are_noticed():
+    """A step whose gradient replaces logits that something has saved for its own backward pass: that pass refuses."""
+    from ista_daslab_optimizers_b200 import distill_step
+    z, idx, val, rest, _ = _problem(3, 500, 4, F32, F32, 1.0, True, False, False)
+    logits = (z.clone().requires_grad_() * 1.0).exp()      # exp saves its result
+    distill_step(logits.detach(), idx, val, rest, grad=logits.detach())
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        logits.sum().backward()
+
+
+def test_distill_twice_differentiated_is_refused():
+    from ista_daslab_optimizers_b200 import distill_loss
+    z, idx, val, rest, _ = _problem(3, 500, 4, F32, F32, 1.0, True, False, False)
+    leaf = z.clone().requires_grad_()
+    grad, = torch.autograd.grad(distill_loss(leaf, idx, val, rest).sum(), leaf, create_graph=True)
+    D.assert_distill(distill_loss(leaf, idx, val, rest).detach(), grad.detach(), D.distill(z, idx, val, rest, None, 1.0), 500, 'with a graph')
+    with pytest.raises(RuntimeError, match='differentiable once'):
+        grad.sum().backward()
+
+
+def test_nothing_to_do():
+    from ista_daslab_optimizers_b200 import distill_loss, distill_step, int8_matmul, quantize_rows, topk_logits
+    e = lambda *s, dtype=F32: torch.empty(*s, dtype=dtype, device='cuda')      # noqa: E731
+    codes, scales = quantize_rows(e(0, 64))
+    assert codes.shape == (0, 64) and scales.shape == (0,)
+    assert int8_matmul(codes, e(5, 64, dtype=torch.int8), scales, e(5)).shape == (0, 5)
+    assert int8_matmul(e(5, 64, dtype=torch.int8), codes, e(5), scales).shape == (5, 0)
+    assert [tuple(t.shape) for t in topk_logits(e(0, 100), 3)] == [(0, 3), (0, 3), (0,)]
+    idx, val = e(0, 3, dtype=torch.int32), e(0, 3)
+    assert [tuple(t.shape) for t in distill_step(e(0, 100), idx, val)] == [(0,), (0, 100)]
+    leaf = e(0, 100).requires_grad_()
+    distill_loss(leaf, idx, val).sum().backward()
+    assert leaf.grad.shape == (0, 100)
+
+
+@pytest.mark.parametrize('call,match', [
+    (lambda P, z, i, v, r: P.quantize_rows(z.half()), 'element type'), (lambda P, z, i, v, r: P.quantize_rows(z.t()), 'contiguous'),
+    (lambda P, z, i, v, r: P.quantize_rows(z[0].expand(6, -1)), 'overlap'), (lambda P, z, i, v, r: P.quantize_rows(z, z), 'element type'),
+    (lambda P, z, i, v, r: P.quantize_rows(z, scales=r.double()), 'scales must be'), (lambda P, z, i, v, r: P.quantize_rows(z, scales=r[:5]), 'scales must be'),
+    (lambda P, z, i, v, r: P.quantize_rows(z.clone().requires_grad_()), 'no gradient'),
+    (lambda P, z, i, v, r: P.topk_logits(z, 65), 'between 1 and'), (lambda P, z, i, v, r: P.topk_logits(z, 0), 'between 1 and'),
+    (lambda P, z, i, v, r: P.topk_logits(z, 3, 0.0), 'temperature'), (lambda P, z, i, v, r: P.topk_logits(z.clone().requires_grad_(), 3), 'no gradient'),
+    (lambda P, z, i, v, r: P.topk_logits(torch.zeros(2, 2000, device='cuda'), 1025), '1024'),
+    (lambda P, z, i, v, r: P.distill_step(z, i.long(), v, r), 'int32'), (lambda P, z, i, v, r: P.distill_step(z, i[:5], v, r), 'must be'),
+    (lambda P, z, i, v, r: P.distill_step(z, i, v[:, :3], r), 'must be'), (lambda P, z, i, v, r: P.distill_step(z, i.t().contiguous().t(), v, r), 'contiguous'),
+    (lambda P, z, i, v, r: P.distill_step(z, i, v, r.cpu()), 'rest must be'), (lambda P, z, i, v, r: P.distill_step(z, i, v, r, r.double()), 'weights must be'),
+    (lambda P, z, i, v, r: P.distill_step(z, i, v, r, grad=z.bfloat16()), 'grad must be'), (lambda P, z, i, v, r: P.distill_step(z, i, v, r, temperature=-1.0), 'temperature'),
+    (lambda P, z, i, v, r: P.distill_step(z[:5], i[:5], v[:5], r[:5], grad=z[1:]), 'overlaps'),
+    (lambda P, z, i, v, r: P.distill_loss(z, i, v.clone().requires_grad_(), r), 'no gradient for values'),
+    (lambda P, z, i, v, r: P.distill_loss(z, i, v, r, temperature=1e9), 'temperature'),
+    (lambda P, z, i, v, r: P.int8_matmul(z, z, r, r), 'element type'),
+    (lambda P, z, i, v, r: P.int8_matmul(z.char(), z.char()[:, :60], r, r), 'inner sizes'),
+    (lambda P, z, i, v, r: P.int8_matmul(z.char()[:, :50].contiguous(), z.char()[:, :50].contiguous(), r, r), 'multiple of 16'),
+    (lambda P, z, i, v, r: P.int8_matmul(z.char()[:, 8:56], z.char()[:, 8:56], r, r), 'start on 16'),
+    (lambda P, z, i, v, r: P.int8_matmul(z.char(), z.char(), r[:3], r), 'a_scales must be'),
+    (lambda P, z, i, v, r: P.int8_matmul(z.char(), z.char(), r, r, dtype=torch.float16), 'unsupported'),
+    (lambda P, z, i, v, r: P.int8_matmul(z.char(), z.char(), r, r, out=z), 'shape')])
+def test_what_is_refused(call, match):
+    import ista_daslab_optimizers_b200 as P
+    from ista_daslab_optimizers_b200 import _native as N
+    z, r = torch.randn(6, 64, device='cuda'), torch.ones(6, device='cuda')
+    i, v = torch.zeros(6, 4, dtype=torch.int32, device='cuda'), torch.zeros(6, 4, device='cuda')
+    before = N.kernel_launch_count()
+    with pytest.raises(N.NativeError, match=match):
+        call(P, z, i, v, r)
+    assert N.kernel_launch_count() == before
+
+
 # ------------------------------------------------------------------------------------------------ together
 
 def test_teacher_to_optimizer_step():
@@ -408,6 +476,65 @@ def test_captured_and_replayed_with_other_streams():
         for a, b in zip(out, eager):
             assert torch.equal(a, b)
     assert N.device_error() == 0
+
+
+def test_forward_and_backward_captured_and_replayed():
+    from ista_daslab_optimizers_b200 import distill_loss
+    z, idx, val, rest, w = _problem(20, 5001, 12, BF16, F32, 1.0, True, True, True)
+    leaf = z.clone().requires_grad_()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        distill_loss(leaf, idx, val, rest, w).sum().backward()
+    torch.cuda.current_stream().wait_stream(side)
+    leaf.grad = None
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss = distill_loss(leaf, idx, val, rest, w)
+        loss.sum().backward()
+    for seed in (6, 7):
+        new = _normal(_gen(seed), 20, 5001).to(BF16)
+        with torch.no_grad():
+            leaf.copy_(new)
+            leaf.grad.zero_()
+        graph.replay()
+        other = new.clone().requires_grad_()
+        want = distill_loss(other, idx, val, rest, w)
+        want.sum().backward()
+        assert torch.equal(loss, want) and torch.equal(leaf.grad, other.grad)
+
+
+def test_calls_of_two_threads():
+    """Two threads on streams of their own, one call behind the other without a wait between them: each has its own results."""
+    import threading
+    from ista_daslab_optimizers_b200 import distill_step, int8_matmul, quantize_rows, topk_logits
+    results, errors = {}, []
+
+    def work(seed):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                g = _gen(seed)
+                x, w, s = _normal(g, 90, 640).to(BF16), _normal(g, 4003, 640, scale=0.1), _normal(g, 90, 4003)
+                for _ in range(10):
+                    a, sa = quantize_rows(x)
+                    b, sb = quantize_rows(w)
+                    v, i, r = topk_logits(int8_matmul(a, b, sa, sb), 30)
+                    results.setdefault(seed, []).append(distill_step(s, i, v, r))
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:                           # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(seed,)) for seed in (11, 12, 11, 12)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors
+    for seed in (11, 12):
+        assert len(results[seed]) == 20
+        for loss, grad in results[seed][1:]:
+            assert torch.equal(loss, results[seed][0][0]) and torch.equal(grad, results[seed][0][1])
 
 
 def test_repeated_calls_give_the_same_bits():
