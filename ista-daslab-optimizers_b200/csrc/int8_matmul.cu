@@ -1,11 +1,18 @@
 // out[i, j] = (sum_c a[i, c] b[j, c]) a_scale[i] b_scale[j] + bias[j]: 8-bit operands, exact 32-bit sums.
 //
 // The tensor cores' rows (128 lanes of tensor memory) are output channels (rows of b), their columns tokens (rows of a): a few tokens are a
-// narrow tile, not a nearly empty one, and a warp of the epilogue holds 32 neighbouring channels of one token, so its stores are whole sectors without a
+// narrow tile, not a nearly empty one, and a warp of the epilogue holds 32 neighbouring channels of one token, so its stores are runs of 64 or 128 bytes without a
 // detour through shared memory.  One warp issues tiled copies (128 bytes of the inner size, 128-byte swizzle, zeros beyond the edges) into a ring of
-// stages, one thread of another issues the products, four warps take the sums out of tensor memory.  Where there are fewer tiles than SMs the inner
-// size is split over the CTAs of a cluster, whose partial sums meet in distributed shared memory: integers, so in any order the same.
-// One to four tokens are no tile at all: a warp per pair of channels, four products an instruction, bound by the weights' bytes.
+// stages, another the products, the others take the sums out of tensor memory.  Three forms, by the number of tokens (us, B200):
+//
+// * up to 4: no tile at all, a warp per pair of channels, four products an instruction.  Bound by the weights' bytes: 4096 x 4096 3.3 for one token, 4.7 for four (the
+//   tiles from 5 tokens on: 7.5).
+// * up to 64: tiles of at most 128 channels and all tokens; where there are fewer tiles than SMs the inner size is split over the CTAs of a cluster, whose partial
+//   sums meet in distributed shared memory: integers, so in any order the same.  Bound by the weights' bytes and some 5 us before the first and behind the last of them:
+//   41 tokens, 14336 x 4096: 15.8 (59 MB); 16 tokens, 128256 x 4096: 82 (6.4 TB/s).
+// * more: tiles of two CTAs.  Bound by the tensor cores where the inner size is long: 2048 tokens, 128256 x 4096: 640 to 800 by the state of the power cap (3.4 to 2.7
+//   PFLOP/s, tensor pipe 98.5 % active); 4096^3: 47.5 (2.9); by the stores where it is short, an SM takes some 7 cycles for each 128-byte line that a warp stores to: 768 tokens,
+//   50304 x 768 bf16 36, 777 tokens, 50257 x 767 fp32, where every run of 128 bytes touches two lines, 66.
 #include "rows.cuh"
 #include "tcgen05.cuh"
 
@@ -300,7 +307,7 @@ __global__ void __launch_bounds__(PAIR_THREADS) int8_matmul_pair_kernel(const __
     if (warp == 1) tmem_free_pair(acc, 512);
 }
 
-// M tokens (m of them there): a warp for R channels, its lanes over the inner size.
+// M tokens (m of them there): a warp for R channels, its lanes over the inner size.  (Eight tokens of 14336 x 4096 took 35 us this way, 14.4 as a tile.)
 template <typename T, int M, int R>
 __global__ void __launch_bounds__(256) int8_rows_kernel(const __grid_constant__ Args g) {
     const int lane = lane_id(), channel0 = (blockIdx.x * 8 + warp_id()) * R;
@@ -420,9 +427,8 @@ template <typename T> int launch_pairs(Args g, int sms, cudaStream_t s) {
     return launch_rows(int8_matmul_pair_kernel<T>, "int8_matmul", pairs * 2, PAIR_THREADS, PAIR_BYTES, 2, s, map_a, map_b, g, tokens, (int)tiles);
 }
 
-#ifndef ROWS_MOST
-#define ROWS_MOST 4
-#endif
+constexpr int ROWS_MOST = 4;                       // tokens without a tile
+
 template <typename T> int launch(const Args& g, cudaStream_t s) {
     const int sms = device_sm_count();
     if (sms < 0) return MAB_ERR_CUDA;

@@ -4,7 +4,7 @@
 // the quotient by less than 2^-15, so rint(y) is the code unless y lies that near to a half; a vector in which one does is coded again by exact residuals:
 // where x - c s of the code c = rint(y) (exact in one FMA: c has 7 bits and cancels all but the last bits of x) lies beyond s / 2, or on it with c odd,
 // the neighbour is the code.  The first way takes 5 operations a value (packed products, the rounding by adding 1.5 2^23, whose low byte is the code), the
-// second, for every value, took 43: 14336 x 4096 bf16 72 us.
+// second, for every value, took 43: 14336 x 4096 bf16 42 us against 72, 2047 x 14336 fp32 30 (4.9 TB/s) against 47.
 #include "rows.cuh"
 
 namespace mab {
