@@ -171,6 +171,7 @@ template <typename T, bool FROM_TOP, int PER, class F> __device__ __forceinline_
 // The key of the k-th largest of n >= k keys, or one between that and the (k + slack)-th; all lie in [lo, hi], n <= F::LIST.
 template <typename T, class F> __device__ __noinline__ uint32_t kth_of_list(Shared<F>& sh, int n, int k, int slack, uint32_t lo, uint32_t hi) {
     const int t = threadIdx.x;
+    if (n <= k + slack + 16) return lo;             // (the sample was the whole part, or nearly)
     if (n <= 512) return kth_by_warp<T, false, 16>(sh, sh.list_key, n, lo, hi, k, k + slack);
     if (n <= 1024) return kth_by_warp<T, false, 32>(sh, sh.list_key, n, lo, hi, k, k + slack);
     int reached;
