@@ -57,7 +57,7 @@ struct Shared {
     uint64_t bar;
     double red[MOST_WARPS][3];
     double part[5];                                // this CTA's part, read by the cluster: reference, S_t, m_k, S_k, B
-    double inv, L, P;
+    double inv, q_scale, P;                        // 1 / Sp, exp(Mk - L), P
     float max_t[MOST_WARPS], max_k[MOST_WARPS], ref_w[MOST_WARPS], sum_w[MOST_WARPS];
     float ref, off;
     uint32_t edge[2];                              // the list's positions in the first and the last, partial vector
@@ -170,6 +170,7 @@ __global__ void __launch_bounds__(NT, (PER_THREAD > 1 ? 1024 : MODE == LOSS ? 15
     __shared__ Shared sh;
     const int C = a.cluster, rank = C > 1 ? (int)(blockIdx.x % C) : 0, t = threadIdx.x, k = a.k;
     const int64_t row = blockIdx.x / C;
+    kernel_before_is_done();
     const float w = a.weights ? a.weights[row] : 1.0f;
     if (w == 0.0f) {                                // the row's logits are not looked at
         if (rank == 0 && t == 0) a.loss[row] = 0.0f;
@@ -434,7 +435,9 @@ __global__ void __launch_bounds__(NT, (PER_THREAD > 1 ? 1024 : MODE == LOSS ? 15
         if (l == 0) {
             if (rank == 0) a.loss[row] = (float)(l_ * (double)w);
             if (rank == 0 && MODE == LOSS) a.stats[row] = make_float2(no_rest ? 0.0f : R, (float)off);
-            sh.inv = inv; sh.L = no_rest && no_list ? none : L; sh.P = P;
+            // q_j = exp(y_j - Mk) exp(Mk - L); where A is this CTA's own reference, the second factor is 1 / Sa
+            sh.inv = inv; sh.P = P;
+            sh.q_scale = Mk == A && !above ? 1.0 / Sa : exp(Mk - (no_rest && no_list ? none : L));
             sh.ref = no_rest ? 0.0f : R;
             sh.off = (float)off;
         }
@@ -443,7 +446,7 @@ __global__ void __launch_bounds__(NT, (PER_THREAD > 1 ? 1024 : MODE == LOSS ? 15
     else __syncthreads();
 
     // tau dloss/dz at this CTA's entries; an index that occurs again has the same number at every place
-    const double inv = sh.inv, L = sh.L, P = sh.P;
+    const double inv = sh.inv, q_scale = sh.q_scale, P = sh.P;
     const float back = (float)((double)w * a.inv_tau);
     float d[PER_THREAD];
 #pragma unroll
@@ -457,7 +460,7 @@ __global__ void __launch_bounds__(NT, (PER_THREAD > 1 ? 1024 : MODE == LOSS ? 15
                 p = 0.0;
                 for (int n = 0; n < k; ++n) if (s_idx[n] == idx[i]) p += s_e[n];
             }
-            d[i] = (float)(P * exp(yj[i] - L) - p * inv);
+            d[i] = (float)(P * (ek[i] * q_scale) - p * inv);
             if (MODE == LOSS) a.list_grad[row * k + j] = d[i];
         }
     }
@@ -485,6 +488,7 @@ template <typename T>
 __global__ void __launch_bounds__(GRAD_NT, 3) distill_grad_kernel(Args a) {
     const int parts = a.cluster, part = blockIdx.x % parts, t = threadIdx.x;
     const int64_t row = blockIdx.x / parts;
+    kernel_before_is_done();
     const float w = a.weights ? a.weights[row] : 1.0f;
     if (w == 0.0f) { zero_part<T, GRAD_NT>(a, row, part, parts); return; }
     const float2 st = a.stats[row];

@@ -64,9 +64,11 @@ __global__ void __launch_bounds__(THREADS) int8_matmul_kernel(const __grid_const
         mbar_init_unfenced(&done, 1);
         mbar_init_fence();
         s_lost = 0;
-        for (int i = k0; i < k1 && i < k0 + stages; ++i) load(i, i - k0);         // (only this thread and the copy engine know of the barriers yet)
     }
     if (warp == 1) tmem_alloc(&s_tmem, COLUMNS);
+    kernel_before_is_done();
+    if (t == 0)
+        for (int i = k0; i < k1 && i < k0 + stages; ++i) load(i, i - k0);           // (only this thread and the copy engine know of the barriers yet)
     for (int i = t; i < BN; i += THREADS) s_token[i] = token0 + i < g.m ? g.a_scales[token0 + i] : 0.0f;
     if (t < BM) {
         const int channel = channel0 + t;
@@ -197,6 +199,7 @@ __global__ void __launch_bounds__(PAIR_THREADS) int8_matmul_pair_kernel(const __
     __syncthreads();
     cluster_arrive_wait();                          // the other CTA's barriers are there
     tmem_fence_after();
+    kernel_before_is_done();
     const uint32_t acc = s_tmem;
 
     if (warp < 2) {
@@ -311,6 +314,7 @@ __global__ void __launch_bounds__(PAIR_THREADS) int8_matmul_pair_kernel(const __
 template <typename T, int M, int R>
 __global__ void __launch_bounds__(256) int8_rows_kernel(const __grid_constant__ Args g) {
     const int lane = lane_id(), channel0 = (blockIdx.x * 8 + warp_id()) * R;
+    kernel_before_is_done();
     if (channel0 >= g.n) return;
     int acc[M][R];
 #pragma unroll

@@ -85,6 +85,7 @@ __global__ void __launch_bounds__(NT, HELD == 4 ? 1536 / NT : 1024 / NT) quantiz
     const bool there = row < a.rows;
     const RowGrid<T> g(reinterpret_cast<const T*>(a.x) + (there ? row : 0) * a.pitch, a.cols);
     const int w0 = g.whole_from(0), w1 = g.whole_to(g.count);
+    kernel_before_is_done();
     auto fetch = [&](int v) {                       // any vector; zeros outside the row
         if (v >= w0 && v < w1) return g.load(v);
         float x[N];

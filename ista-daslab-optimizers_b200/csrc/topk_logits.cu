@@ -372,6 +372,7 @@ __global__ void __launch_bounds__(F::NT, F::CTAS) topk_logits_kernel(Args a) {
     const int per = (g.count + C - 1) / C, v0 = min(rank * per, g.count), v1 = min(v0 + per, g.count);
     const int w0 = g.whole_from(v0), w1 = g.whole_to(v1);
     if (t == 0) sh.n = sh.n_list = sh.n_reach = 0;
+    kernel_before_is_done();
     Rest rest = {0.0f, 0.0f, a.scale, false};
     float bound = -INF_F;                           // values above it are candidates
     uint32_t lo_key = 0, top_key = K::MOST;         // no candidate's key lies outside
