@@ -76,7 +76,7 @@ def host_command(source=HOST_SRC, out=None):
     return [os.environ.get('CXX', 'g++'), '-O2', '-std=c++17', '-fPIC', '-shared', '-I', INCLUDE, '-I', os.path.join(base, 'include'),
             '-I', os.path.join(base, 'include', 'torch', 'csrc', 'api', 'include'), '-I', os.path.join(cuda, 'include'),
             '-I', sysconfig.get_paths()['include'], source, '-o', out or host_path(), '-L', os.path.join(base, 'lib'),
-            '-ltorch_python', '-lc10_cuda', '-lc10', '-ltorch_cpu']
+            '-ltorch_python', '-lc10_cuda', '-lc10', '-ltorch_cpu'] + (['-ltorch_cuda'] if source == CALLS_SRC else [])
 
 
 def build(verbose: bool = False, force: bool = False) -> str:

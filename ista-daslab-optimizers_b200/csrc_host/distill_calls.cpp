@@ -7,6 +7,7 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -58,6 +59,9 @@ PyObject* raise_python() {
 
 bool is_float(const at::Tensor& t) { return t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16; }
 int code(const at::Tensor& t) { return t.scalar_type() == at::kFloat ? MAB_F32 : MAB_BF16; }
+
+// A new tensor, straight from the device's allocator.
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& like) { return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt); }
 
 // A matrix on a CUDA device whose rows are contiguous: its address and their distance.
 struct Rows {
@@ -132,11 +136,11 @@ PyObject* quantize_rows(PyObject*, PyObject* const* args, Py_ssize_t n) try {
     const int64_t rows = x.size(0), cols = x.size(1);
     const Target on(x);
     if (!codes.defined()) {
-        codes = at::empty({rows, (cols + 15) / 16 * 16}, x.options().dtype(at::kChar).requires_grad(false));
+        codes = fresh({rows, (cols + 15) / 16 * 16}, at::kChar, x);
         if (cols % 16) codes = codes.narrow(1, 0, cols);
     }
     EXPECT(cr.of(codes) && codes.scalar_type() == at::kChar && codes.sizes() == x.sizes() && codes.device() == x.device());
-    if (!scales.defined()) scales = at::empty({rows}, x.options().dtype(at::kFloat).requires_grad(false));
+    if (!scales.defined()) scales = fresh({rows}, at::kFloat, x);
     EXPECT(is_vector(scales, rows, x));
     int status;
     {
@@ -161,7 +165,7 @@ PyObject* int8_matmul(PyObject*, PyObject* const* args, Py_ssize_t n) try {
     EXPECT(is_vector(a_scales, m, a) && is_vector(b_scales, channels, a) && (!bias.defined() || is_vector(bias, channels, a)));
     EXPECT(!wants_gradient(a_scales) && !wants_gradient(b_scales) && !wants_gradient(bias));
     const Target on(a);
-    if (!out.defined()) out = at::empty({m, channels}, a.options().dtype(args[6] == Py_True ? at::kBFloat16 : at::kFloat));
+    if (!out.defined()) out = fresh({m, channels}, args[6] == Py_True ? at::kBFloat16 : at::kFloat, a);
     EXPECT(outr.of(out) && is_float(out) && out.size(0) == m && out.size(1) == channels && out.device() == a.device() && !wants_gradient(out));
     if (m == 1) ar.pitch = (ar.pitch + 15) / 16 * 16;              // one row: no distance
     if (channels == 1) br.pitch = (br.pitch + 15) / 16 * 16;
@@ -187,8 +191,7 @@ PyObject* topk_logits(PyObject*, PyObject* const* args, Py_ssize_t n) try {
     EXPECT(zr.of(z) && is_float(z) && !wants_gradient(z) && k >= 1 && k <= z.size(1));
     const Target on(z);
     const int64_t rows = z.size(0);
-    const auto options = z.options().requires_grad(false);
-    at::Tensor values = at::empty({rows, k}, options), indices = at::empty({rows, k}, options.dtype(at::kInt)), rest = at::empty({rows}, options.dtype(at::kFloat));
+    at::Tensor values = fresh({rows, k}, z.scalar_type(), z), indices = fresh({rows, k}, at::kInt, z), rest = fresh({rows}, at::kFloat, z);
     const double temperature = PyFloat_AS_DOUBLE(args[2]);
     int status;
     {
@@ -227,10 +230,9 @@ void throw_if(int status, const char* what) {
 
 at::Tensor loss_of(const Lists& l, double temperature, at::Tensor* stats, at::Tensor* list_grad) {
     const Target on(l.logits);
-    const auto options = l.logits.options().dtype(at::kFloat).requires_grad(false);
-    at::Tensor loss = at::empty({l.rows}, options);
-    *stats = at::empty({l.rows, 2}, options);
-    *list_grad = at::empty({l.rows, l.k}, options);
+    at::Tensor loss = fresh({l.rows}, at::kFloat, l.logits);
+    *stats = fresh({l.rows, 2}, at::kFloat, l.logits);
+    *list_grad = fresh({l.rows, l.k}, at::kFloat, l.logits);
     throw_if(g_library.distill_loss(l.rows, l.vocab, l.k, l.z.p, code(l.logits), l.z.pitch, static_cast<const int32_t*>(l.indices.data_ptr()), l.values.data_ptr(), code(l.values),
                                     vector_at(l.rest), vector_at(l.weights), temperature, vector_at(loss), vector_at(*stats), vector_at(*list_grad), on.stream), "distill_loss");
     return loss;
@@ -258,7 +260,7 @@ struct DistillLoss : torch::autograd::Function<DistillLoss> {
             const int64_t rows = logits.size(0), vocab = logits.size(1);
             Rows z;
             z.of(logits);
-            grad = at::empty({rows, vocab}, logits.options().requires_grad(false));
+            grad = fresh({rows, vocab}, logits.scalar_type(), logits);
             throw_if(g_library.distill_grad(rows, vocab, indices.size(1), z.p, code(logits), z.pitch, static_cast<const int32_t*>(indices.data_ptr()), vector_at(weights),
                                             ctx->saved_data["temperature"].toDouble(), vector_at(stats), vector_at(list_grad), vector_at(up), up.stride(0),
                                             grad.data_ptr(), vocab, on.stream), "distill_loss backward");
@@ -294,10 +296,10 @@ PyObject* distill_step(PyObject*, PyObject* const* args, Py_ssize_t n) try {
     at::Tensor grad;
     EXPECT(n == 7 && PyFloat_Check(args[5]) && l.of(args) && tensor(args[6], &grad, true));
     const Target on(l.logits);
-    if (!grad.defined()) grad = at::empty({l.rows, l.vocab}, l.logits.options().requires_grad(false));
+    if (!grad.defined()) grad = fresh({l.rows, l.vocab}, l.logits.scalar_type(), l.logits);
     Rows g;
     EXPECT(g.of(grad) && grad.sizes() == l.logits.sizes() && grad.scalar_type() == l.logits.scalar_type() && grad.device() == l.logits.device() && !grad.requires_grad());
-    at::Tensor loss = at::empty({l.rows}, l.logits.options().dtype(at::kFloat).requires_grad(false));
+    at::Tensor loss = fresh({l.rows}, at::kFloat, l.logits);
     const double temperature = PyFloat_AS_DOUBLE(args[5]);
     int status;
     {
