@@ -338,7 +338,8 @@ __global__ void __launch_bounds__(NT, (PER_THREAD > 1 ? 1024 : MODE == LOSS ? 15
     };
     {
         if (!RESIDENT) {
-            run(h1, w1, [&](int v) { return g.load(v); });
+            // (a step reads them again, from L2 if it can: they are not a stream)
+            run(h1, w1, [&](int v) { return MODE == LOSS ? g.stream(v) : g.load(v); });
             arrived();
         }
         if (RESIDENT || held > 0) run(w0, h1, get);

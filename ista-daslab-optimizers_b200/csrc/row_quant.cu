@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(NT, HELD == 4 ? 1536 / NT : 1024 / NT) quantiz
     const int w0 = g.whole_from(0), w1 = g.whole_to(g.count);
     kernel_before_is_done();
     auto fetch = [&](int v) {                       // any vector; zeros outside the row
-        if (v >= w0 && v < w1) return g.load(v);
+        if (v >= w0 && v < w1) return g.stream(v);
         float x[N];
         g.load_part(v, x, 0.0f);
         return pack(x, (const T*)nullptr);

@@ -24,9 +24,9 @@ constexpr int MAX_K = 1024;
 // Lists of up to 128 by CTAs of 256 threads, six on an SM: their chains of phases overlap the others' streams (2048 rows of 128256 bf16, k = 64: 138 us with the larger form).
 template <bool LARGE> struct Form {
     static constexpr int NT = LARGE ? 512 : 256, WARPS = NT / 32, CTAS = LARGE ? 3 : 6;
-    static constexpr int CAP = LARGE ? 3072 : 1024;             // candidates
-    static constexpr int LIST = LARGE ? 3072 : 1536;            // vectors that hold one by the first bound ...
-    static constexpr int REACH = LARGE ? 1536 : 512;            // ... and by the second
+    static constexpr int CAP = LARGE ? 2560 : 1024;             // candidates
+    static constexpr int LIST = LARGE ? 2560 : 1024;            // vectors that hold one by the first bound ...
+    static constexpr int REACH = LARGE ? 1536 : 512;            // vectors that hold one by the second bound
     static constexpr int MOST_K = LARGE ? MAX_K : 128, ITEMS = CAP / NT;
     static_assert(2 * MOST_K <= CAP, "what is held and what a chunk adds have room");
 };
@@ -92,10 +92,8 @@ struct Rest {
 
 // A candidate's term in the rest, rounded to a multiple of 2^-38: candidates come in any order and to any thread, and doubles on one grid
 // have the same sum in every order (32768 of them, each at most 1 but for a rounding, stay exact).
-__device__ __forceinline__ double grid_term(const Rest& rest, float x) {
-    const double d = (double)ex2(fmaf(x, rest.scale, -rest.ref));
-    return __dadd_rn(__dadd_rn(d, 24576.0), -24576.0);
-}
+__device__ __forceinline__ double on_grid(float term) { return __dadd_rn(__dadd_rn((double)term, 24576.0), -24576.0); }
+__device__ __forceinline__ double grid_term(const Rest& rest, float x) { return on_grid(ex2(fmaf(x, rest.scale, -rest.ref))); }
 // Adds the block's terms to the rest, in the first thread.
 template <class F> __device__ __forceinline__ void add_terms(double* parts, double mine, Rest& rest) {
 #pragma unroll
@@ -396,7 +394,10 @@ __global__ void __launch_bounds__(F::NT, F::CTAS) topk_logits_kernel(Args a) {
             const float m = vector_max(r, (const T*)nullptr);
             if (m > bound) {
                 const int at = atomicAdd(&sh.n_list, 1);
-                if (at < F::LIST) { sh.list[at] = v; sh.list_key[at] = K::of(m); }
+                if (at < F::LIST) {
+                    sh.list[at] = v;
+                    sh.list_key[at] = K::of(m);
+                }
             } else {
                 uint64_t x[N / 2];
                 unpack_pairs(r, x, (const T*)nullptr);
@@ -417,11 +418,11 @@ __global__ void __launch_bounds__(F::NT, F::CTAS) topk_logits_kernel(Args a) {
             for (; v + (UNROLL - 1) * F::NT < w1; v += UNROLL * F::NT) {
                 uint4 r[UNROLL];
 #pragma unroll
-                for (int u = 0; u < UNROLL; ++u) r[u] = g.load(v + u * F::NT);
+                for (int u = 0; u < UNROLL; ++u) r[u] = g.stream(v + u * F::NT);
 #pragma unroll
                 for (int u = 0; u < UNROLL; ++u) see(r[u], v + u * F::NT);
             }
-            for (; v < w1; v += F::NT) see(g.load(v), v);
+            for (; v < w1; v += F::NT) see(g.stream(v), v);
         }
         float lo, hi;
         split(sum, lo, hi);
@@ -439,25 +440,25 @@ __global__ void __launch_bounds__(F::NT, F::CTAS) topk_logits_kernel(Args a) {
         if (all) {
             for (int i = t; i < listed * N; i += F::NT) push(Elem<T>::load(g.p, g.first(w0) + i), g.first(w0) + i);
         } else if (!slow) {
-            // vectors below the new bound go into the sum; of the others, which are some k, a thread has an element at a time
+            // vectors below the new bound go into the sum, each by its own sum in a fixed order; of the others, which are some k, a thread has an element at a time
             for (int j = t; j < listed; j += F::NT) {
-                const int v = sh.list[j];
                 if (sh.list_key[j] >= lo_key) {
                     const int at = atomicAdd(&sh.n_reach, 1);
-                    if (at < F::REACH) sh.reach[at] = v;
+                    if (at < F::REACH) sh.reach[at] = j;
                     continue;
                 }
-                float x[N];
-                unpack(g.load(v), x, (const T*)nullptr);
+                float x[N], part = 0.0f;
+                unpack(g.load(sh.list[j]), x, (const T*)nullptr);
 #pragma unroll
-                for (int i = 0; i < N; ++i) terms += grid_term(rest, x[i]);
+                for (int i = 0; i < N; ++i) part += ex2(fmaf(x[i], rest.scale, -rest.ref));
+                terms += on_grid(part);
             }
             __syncthreads();
             const int reaching = sh.n_reach;
             slow = reaching > F::REACH;
             if (!slow)
                 for (int i = t; i < reaching * N; i += F::NT) {
-                    const int e = g.first(sh.reach[i / N]) + i % N;
+                    const int j = sh.reach[i / N], e = g.first(sh.list[j]) + i % N;
                     const float x = Elem<T>::load(g.p, e);
                     if (x > bound) push(x, e);
                     else terms += grid_term(rest, x);
