@@ -256,47 +256,40 @@ __global__ void __launch_bounds__(PAIR_THREADS) int8_matmul_pair_kernel(const __
         }
         if (!ok) s_lost = 1;
     } else {
-        // 32 channels and every fourth group of 32 tokens a warp
-        constexpr int S = PAIR_SLICES, PER = 8 / S;
+        // 32 channels and every other group of 32 tokens a warp
         const int quarter = warp & 3, slice = (warp - 2) >> 2, groups = tokens / 32;
         int done = 0;
         for (int tile = pair; tile < tiles; tile += pairs, ++done) {
             const int token0 = tile % g.token_tiles * tokens, channel = tile / g.token_tiles * 2 * BM + rank * BM + 32 * quarter + lane;
             const bool there = channel < g.n;
             const float cs = there ? g.b_scales[channel] : 0.0f, bias = g.bias && there ? g.bias[channel] : 0.0f;
-            float scale[PER];                         // of the tokens of this warp's groups, one a lane
-#pragma unroll
-            for (int j = 0; j < PER; ++j) {
-                const int token = token0 + (S * j + slice) * 32 + lane;
-                scale[j] = S * j + slice < groups && token < g.m ? g.a_scales[token] : 0.0f;
-            }
+            auto scale_of = [&](int group) {          // of the group's tokens, one a lane
+                const int token = token0 + 32 * group + lane;
+                return group < groups && token < g.m ? g.a_scales[token] : 0.0f;
+            };
+            float next_scale = scale_of(slice);
             if (!mbar_wait(&ready[done & 1], done / 2 & 1, PAIR_LIMIT)) { if (lane == 0) atomicExch(&s_lost, 1); break; }
             tmem_fence_after();
             const uint32_t from = acc + ((uint32_t)(32 * quarter) << 16) + (done & 1) * 256;
             if (slice >= groups && lane == 0) mbar_arrive_cluster(cluster_addr(&taken[done & 1], 0));
-#pragma unroll
-            for (int j = 0; j < PER; ++j) {
-                const int group = S * j + slice;
-                if (group >= groups) break;
+            // not unrolled: a tile's instructions would not fit the cache (768 tokens, 50304 x 768 bf16 36 us, 777, 50257 x 767 fp32 59; rolled and with one way for whole and partial groups 33 and 50)
+#pragma unroll 1
+            for (int group = slice; group < groups; group += PAIR_SLICES) {
                 int r[32];
                 tmem_load(from + 32 * group, r);
+                const float scale = next_scale;
+                next_scale = scale_of(group + PAIR_SLICES);
                 tmem_wait_load(r);
-                if (group + S >= groups) {          // the warp's sums of the tile are in registers
+                if (group + PAIR_SLICES >= groups) {          // the warp's sums of the tile are in registers
                     tmem_fence_before();
                     if (lane == 0) mbar_arrive_cluster(cluster_addr(&taken[done & 1], 0));
                 }
                 const int first = token0 + 32 * group, there_tokens = g.m - first;
                 T* out = reinterpret_cast<T*>(g.out) + (int64_t)first * g.out_pitch + channel;
-                if (there_tokens >= 32 && __all_sync(0xffffffffu, there)) {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i, out += g.out_pitch)
-                        Elem<T>::store(out, 0, scaled(r[i], __shfl_sync(0xffffffffu, scale[j], i), cs, bias));
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i, out += g.out_pitch) {
-                        const float s = __shfl_sync(0xffffffffu, scale[j], i);
-                        if (there && i < there_tokens) Elem<T>::store(out, 0, scaled(r[i], s, cs, bias));
-                    }
+                for (int i = 0; i < 32; ++i, out += g.out_pitch) {
+                    const float s = __shfl_sync(0xffffffffu, scale, i);
+                    if (there && i < there_tokens) Elem<T>::store(out, 0, scaled(r[i], s, cs, bias));
                 }
             }
         }
@@ -440,8 +433,7 @@ template <typename T> int launch(const Args& g, cudaStream_t s) {
         const int64_t ctas = ceil_div64(g.n, 16);
         if (g.m == 1) return launch_rows(int8_rows_kernel<T, 1, 2>, "int8_matmul", ctas, 256, 0, 1, s, g);
         if (g.m == 2) return launch_rows(int8_rows_kernel<T, 2, 2>, "int8_matmul", ctas, 256, 0, 1, s, g);
-        if (g.m <= 4) return launch_rows(int8_rows_kernel<T, 4, 2>, "int8_matmul", ctas, 256, 0, 1, s, g);
-        return launch_rows(int8_rows_kernel<T, 8, 2>, "int8_matmul", ctas, 256, 0, 1, s, g);
+        return launch_rows(int8_rows_kernel<T, 4, 2>, "int8_matmul", ctas, 256, 0, 1, s, g);
     }
     if (g.m > 64) return launch_pairs<T>(g, sms, s);
     if (g.m <= 16) return launch_tiles<T, 16>(g, sms, s);
