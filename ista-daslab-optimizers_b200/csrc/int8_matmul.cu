@@ -435,6 +435,9 @@ template <typename T> int launch(const Args& g, cudaStream_t s) {
         if (g.m == 2) return launch_rows(int8_rows_kernel<T, 2, 2>, "int8_matmul", ctas, 256, 0, 1, s, g);
         return launch_rows(int8_rows_kernel<T, 4, 2>, "int8_matmul", ctas, 256, 0, 1, s, g);
     }
+    // Few channels and a long inner size leave most SMs without a pair's tile: 65 and 128 tokens, 4096 x 14336, 25 us, in tiles with the inner size split 17.5 and 19 (with an
+    // inner size of 4096 9.3 and 9.8 against 7.5 and 8.9, of 2048 6.3 and 6.7 against 6.6 and 8.0).
+    if (g.m > 64 && g.m <= 128 && g.k > 48 * BK && 8 * ceil_div64(g.n, 2 * BM) <= sms) return launch_tiles<T, 128>(g, sms, s);
     if (g.m > 64) return launch_pairs<T>(g, sms, s);
     if (g.m <= 16) return launch_tiles<T, 16>(g, sms, s);
     if (g.m <= 32) return launch_tiles<T, 32>(g, sms, s);

@@ -89,7 +89,7 @@ def _codes(g, rows, cols, extreme=False):
 @pytest.mark.parametrize('dtype', [F32, BF16])
 @pytest.mark.parametrize('m,n,k,bias', [
     (1, 1, 1, False), (1, 130, 16, True), (2, 77, 767, False), (3, 1000, 129, True), (4, 4096, 4096, False), (5, 128, 128, True), (5, 130, 100, False),
-    (16, 300, 1000, False), (17, 129, 31, True), (31, 1024, 4096, False), (41, 257, 2049, True), (64, 128, 8192, False), (65, 300, 640, True),
+    (16, 300, 1000, False), (17, 129, 31, True), (31, 1024, 4096, False), (41, 257, 2049, True), (64, 128, 8192, False), (65, 300, 640, True), (65, 300, 6400, True), (100, 1001, 8190, False), (128, 513, 6145, True),
     (128, 256, 255, False), (129, 511, 513, True), (256, 384, 1024, False), (257, 1025, 767, True), (300, 2048, 512, False), (777, 515, 129, False),
     (70, 9500, 300, True), (129, 9729, 1025, False), (300, 5000, 1, False), (777, 5003, 767, True), (2048, 1300, 257, False), (1025, 2305, 2048, True)])
 def test_int8_matmul(dtype, m, n, k, bias):
