@@ -82,11 +82,15 @@ struct Rest {
     float s, ref, scale;
     bool far;
     __device__ __forceinline__ void add(float x) { s += ex2(fmaf(x, scale, -ref)); }
+    // The reference only rises: a later bound may be lower than it (of merged lists the k-th to (k + slack)-th is any value in between, far below one's own bound), and
+    // s times a power of two of the difference would overflow.  What is added later lies below some bound before it, and so below the reference.
     __device__ __forceinline__ void move(float to_value) {
-        const float to = to_value == -INF_F ? 0.0f : fminf(fmaxf(to_value * scale, -3e38f), 3e38f);
-        far |= !(fabsf(to) < FAR);
-        if (!(s == 0.0f)) s *= ex2(ref - to);
-        ref = to;
+        const float to = to_value == -INF_F ? -3e38f : fminf(fmaxf(to_value * scale, -3e38f), 3e38f);
+        far |= to_value != -INF_F && !(fabsf(to) < FAR);
+        if (to > ref) {
+            if (!(s == 0.0f)) s *= ex2(ref - to);
+            ref = to;
+        }
     }
 };
 
@@ -278,7 +282,8 @@ template <typename T, class F> __device__ __noinline__ void select_slowly(Shared
     const int t = threadIdx.x;
     __syncthreads();
     if (t == 0) sh.n = 0;
-    rest.s = rest.ref = 0.0f;
+    rest.s = 0.0f;
+    rest.ref = -INF_F;
     uint32_t floor_key = 0;                         // smaller keys cannot be among the k largest any more
     for (int base = v0; base < v1; base += F::NT * SLOW_UNROLL) {
         float x[SLOW_UNROLL][N];
@@ -371,7 +376,7 @@ __global__ void __launch_bounds__(F::NT, F::CTAS) topk_logits_kernel(Args a) {
     const int w0 = g.whole_from(v0), w1 = g.whole_to(v1);
     if (t == 0) sh.n = sh.n_list = sh.n_reach = 0;
     kernel_before_is_done();
-    Rest rest = {0.0f, 0.0f, a.scale, false};
+    Rest rest = {0.0f, -INF_F, a.scale, false};
     float bound = -INF_F;                           // values above it are candidates
     uint32_t lo_key = 0, top_key = K::MOST;         // no candidate's key lies outside
     bool slow = false;
@@ -510,7 +515,7 @@ __global__ void __launch_bounds__(F::NT, F::CTAS) topk_logits_kernel(Args a) {
                 if (!(sh.peer_sum[c] == 0.0)) ref = fmaxf(ref, (float)sh.peer_ref[c]);
             }
             rest.s = 0.0f;
-            rest.ref = ref == -INF_F ? 0.0f : ref;
+            rest.ref = ref;
             if (t < C && !(sh.peer_sum[t] == 0.0)) rest.s = (float)(sh.peer_sum[t] * (double)ex2((float)sh.peer_ref[t] - rest.ref));
         } else {
             int at = 0;

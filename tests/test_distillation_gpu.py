@@ -144,6 +144,16 @@ def test_topk_logits(dtype, rows, vocab, k, tau, skip, gap):
     _check_topk(_placed(z.to(dtype), dtype, skip, gap), k, tau)
 
 
+@pytest.mark.parametrize('rows', [1, 3, 40, 70])
+@pytest.mark.parametrize('step', [0.015625, 1.0, 50.0])
+def test_topk_logits_of_slopes(rows, step):
+    """Few rows are shared by several blocks, whose lists are merged; on a slope they lie far from one another."""
+    for k in (7, 20, 33, 48, 65, 100, 128, 200, 300, 513, 1000):
+        z = (torch.arange(40001, device='cuda').float() * step).expand(rows, 40001).clone()
+        _check_topk(z, k, 1.0)
+        _check_topk(z.flip(1).contiguous(), k, 3.0)
+
+
 @pytest.mark.parametrize('dtype', [F32, BF16])
 @pytest.mark.parametrize('rows', [2, 301])
 @pytest.mark.parametrize('kind', ['equal', 'zeros', 'two', 'ascending', 'descending', 'late', 'masked', 'lowest', 'few', 'none', 'inf', 'many_inf', 'nan',
