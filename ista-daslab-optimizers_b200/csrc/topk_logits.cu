@@ -9,24 +9,26 @@
 // The order is that of 64-bit keys, value above 2^32 - 1 - index: distinct, so "larger" contains the tie rule.  NaN lies below -inf and makes
 // the rest NaN.  A row belongs to a cluster of one to eight CTAs; the first of them merges the candidates of all.
 //
-// Bound by the chains of phases around the stream (some 30 k of a row's 90 k cycles with six rows on an SM) and by the special-function units, which an exponential
-// per logit keeps busy for 75 us of 2048 x 128256 bf16: that takes 133 us with k = 64 (3.9 TB/s; the stream alone 84, plain reading 78), 119 with k = 10; 5 x 50257 fp32
-// with k = 20 11.6.
+// Bound by the chains of phases around the stream (about a quarter of a row's time with six rows on an SM), by the special-function units, which an exponential
+// per logit keeps busy for 75 us of 2048 x 128256 bf16, and by the sample's second reading: that takes 109 us with k = 64 (4.8 TB/s; the stream alone 84, plain reading 78), 93
+// with k = 10; 5 x 50257 fp32 with k = 20 10.1.
 #include "rows.cuh"
 
 namespace mab {
 namespace toplogits {
 
-constexpr int UNROLL = 4;                          // vectors a thread has in flight
+constexpr int UNROLL = 6;                          // vectors a thread has in flight (2048 rows of 128256 bf16, k = 64, with 3 .. 8: 114, 111, 110, 109, 111, 116 us)
 constexpr int SLOW_UNROLL = 2;                     // vectors a thread holds of a chunk that is selected from exactly
 constexpr int MAX_K = 1024;
 
-// Lists of up to 128 by CTAs of 256 threads, six on an SM: their chains of phases overlap the others' streams (2048 rows of 128256 bf16, k = 64: 138 us with the larger form).
+// Lists of up to 128 by CTAs of 256 threads, six on an SM: their chains of phases overlap the others' streams.  They keep the listed vectors themselves (the case above: 122 us
+// when they were read again, from L2 or beyond; 121 with 31 KB a CTA, which leave too little of the SM's memory to the loads under way).
 template <bool LARGE> struct Form {
     static constexpr int NT = LARGE ? 512 : 256, WARPS = NT / 32, CTAS = LARGE ? 3 : 6;
-    static constexpr int CAP = LARGE ? 2560 : 1024;             // candidates
-    static constexpr int LIST = LARGE ? 2560 : 1024;            // vectors that hold one by the first bound ...
+    static constexpr int CAP = LARGE ? 2560 : 768;             // candidates
+    static constexpr int LIST = LARGE ? 2560 : 896;            // vectors that hold one by the first bound
     static constexpr int REACH = LARGE ? 1536 : 512;            // vectors that hold one by the second bound
+    static constexpr bool KEPT = !LARGE;
     static constexpr int MOST_K = LARGE ? MAX_K : 128, ITEMS = CAP / NT;
     static_assert(2 * MOST_K <= CAP, "what is held and what a chunk adds have room");
 };
@@ -44,8 +46,9 @@ struct Args {
 
 template <class F> struct Shared {
     unsigned long long cand[F::CAP];
-    int list[F::LIST];                                 // vectors with a value above the bound ...
-    uint32_t list_key[F::LIST];                        // ... and the keys of their largest
+    uint4 data[F::KEPT ? F::LIST : 1];              // vectors with a value above the bound (LARGE: not kept) ...
+    int list[F::LIST];                              // ... which they are ...
+    uint32_t list_key[F::LIST];                     // ... and the keys of their largest
     int reach[F::REACH];                               // those that reach the second bound
     int n_list, n_reach;
     double red[F::WARPS];
@@ -402,6 +405,7 @@ __global__ void __launch_bounds__(F::NT, F::CTAS) topk_logits_kernel(Args a) {
                 if (at < F::LIST) {
                     sh.list[at] = v;
                     sh.list_key[at] = K::of(m);
+                    if (F::KEPT) sh.data[at] = r;
                 }
             } else {
                 uint64_t x[N / 2];
@@ -453,7 +457,7 @@ __global__ void __launch_bounds__(F::NT, F::CTAS) topk_logits_kernel(Args a) {
                     continue;
                 }
                 float x[N], part = 0.0f;
-                unpack(g.load(sh.list[j]), x, (const T*)nullptr);
+                unpack(F::KEPT ? sh.data[j] : g.load(sh.list[j]), x, (const T*)nullptr);
 #pragma unroll
                 for (int i = 0; i < N; ++i) part += ex2(fmaf(x[i], rest.scale, -rest.ref));
                 terms += on_grid(part);
@@ -464,7 +468,7 @@ __global__ void __launch_bounds__(F::NT, F::CTAS) topk_logits_kernel(Args a) {
             if (!slow)
                 for (int i = t; i < reaching * N; i += F::NT) {
                     const int j = sh.reach[i / N], e = g.first(sh.list[j]) + i % N;
-                    const float x = Elem<T>::load(g.p, e);
+                    const float x = F::KEPT ? Elem<T>::load(reinterpret_cast<const T*>(&sh.data[j]), i % N) : Elem<T>::load(g.p, e);
                     if (x > bound) push(x, e);
                     else terms += grid_term(rest, x);
                 }
@@ -624,10 +628,11 @@ template <typename T, class F> int launch_form(Args a, int64_t rows, int sms, cu
     // CTAs of a row: until every SM has one, no part below 4 KB, and the merged lists fit the candidates' room
     a.cluster = 1;
     while (a.cluster < 8 && rows * a.cluster * 2 <= sms && (int64_t)a.vocab * sizeof(T) / (2 * a.cluster) >= 4096 && 2 * a.cluster * a.k <= F::CAP) a.cluster *= 2;
-    // the sample: an eighth of a row of 128256 bf16 at least (2048 vectors), and so many that some k (part / sample) vectors fit the list, a quarter of it for what the
-    // sample does not show; in four times as many groups as k, as far as the list's room goes
+    // The sample: an eighth of a row of 128256 bf16 at least (2048 vectors), and so many that the list has room.  It holds k (part / sample) vectors, 1.3 to 1.5 times that
+    // with the slack of the bound and groups of several, and for lists of any length varies by less than 1 / sqrt(k): 2 k (part / sample) fit.  In four times as many
+    // groups as k, as far as the list's room goes.
     const int64_t part = ((int64_t)a.vocab / RowGrid<T>::N + a.cluster) / a.cluster;
-    const int each = (int)std::max<int64_t>(2048 / F::NT, std::min<int64_t>(64, ceil_div64(part * a.k, (int64_t)F::NT * F::LIST * 3 / 4)));
+    const int each = (int)std::max<int64_t>(2048 / F::NT, std::min<int64_t>(512, ceil_div64(2 * part * a.k, (int64_t)F::NT * F::LIST)));
     a.groups = std::min({F::LIST / F::NT, each, std::max(1, (4 * a.k + F::NT - 1) / F::NT)});
     a.per = (each + a.groups - 1) / a.groups;
     return launch_rows(topk_logits_kernel<T, F>, "topk_logits", rows * a.cluster, F::NT, sizeof(Shared<F>), a.cluster, s, a);
