@@ -15,7 +15,7 @@
 // results do not depend on timing.
 //
 // Bound by HBM and by the chain of phases around the passes (list, block and cluster sums, three logarithms: some 5 us a row, which the SM's other rows cover in part).
-// bf16, rows of 128256, k = 64 (us): loss of 1536 rows 80 (4.9 TB/s), its gradient 149 (6.2 TB/s), loss and gradient of 4096 rows in one call 443 (4.75 TB/s of the two passes
+// bf16, rows of 128256, k = 64 (us): loss of 1536 rows 75 (5.2 TB/s), its gradient 149 (6.2 TB/s), loss and gradient of 4096 rows in one call 435 (4.8 TB/s of the two passes
 // over HBM that it needs; what it holds and what L2 keeps leave 1.09 of their bytes; 569 before anything was held).
 #include <type_traits>
 #include "rows.cuh"

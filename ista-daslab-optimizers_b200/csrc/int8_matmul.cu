@@ -5,14 +5,14 @@
 // detour through shared memory.  One warp issues tiled copies (128 bytes of the inner size, 128-byte swizzle, zeros beyond the edges) into a ring of
 // stages, another the products, the others take the sums out of tensor memory.  Three forms, by the number of tokens (us, B200):
 //
-// * up to 4: no tile at all, a warp per pair of channels, four products an instruction.  Bound by the weights' bytes: 4096 x 4096 3.3 for one token, 4.7 for four (the
+// * up to 4: no tile at all, a warp per pair of channels, four products an instruction.  Bound by the weights' bytes: 4096 x 4096 3.1 for one token, 4.7 for four (the
 //   tiles from 5 tokens on: 7.5).
 // * up to 64: tiles of at most 128 channels and all tokens; where there are fewer tiles than SMs the inner size is split over the CTAs of a cluster, whose partial
 //   sums meet in distributed shared memory: integers, so in any order the same.  Bound by the weights' bytes and some 5 us before the first and behind the last of them:
-//   41 tokens, 14336 x 4096: 15.8 (59 MB); 16 tokens, 128256 x 4096: 82 (6.4 TB/s).
+//   41 tokens, 14336 x 4096: 14.8 (59 MB); 16 tokens, 128256 x 4096: 82 (6.4 TB/s). (So, too, up to 128 where the channels are few and the inner size long.)
 // * more: tiles of two CTAs.  Bound by the tensor cores where the inner size is long: 2048 tokens, 128256 x 4096: 640 to 800 by the state of the power cap (3.4 to 2.7
-//   PFLOP/s, tensor pipe 98.5 % active); 4096^3: 47.5 (2.9); by the stores where it is short, an SM takes some 7 cycles for each 128-byte line that a warp stores to: 768 tokens,
-//   50304 x 768 bf16 36, 777 tokens, 50257 x 767 fp32, where every run of 128 bytes touches two lines, 66.
+//   PFLOP/s, tensor pipe 98.5 % active); 4096^3: 46.5 (2.96); by the stores where it is short, an SM takes some 7 cycles for each 128-byte line that a warp stores to: 768 tokens,
+//   50304 x 768 bf16 33, 777 tokens, 50257 x 767 fp32, where every run of 128 bytes touches two lines, 51 (the stores alone 46).
 #include "rows.cuh"
 #include "tcgen05.cuh"
 

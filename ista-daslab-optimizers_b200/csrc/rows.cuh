@@ -23,7 +23,7 @@ template <typename T> struct RowGrid {
     __device__ __forceinline__ int whole_to(int v1) const { return v1 == count && (n + lead) % N ? v1 - 1 : v1; }
     __device__ __forceinline__ uint4 load(int v) const { return *reinterpret_cast<const uint4*>(p + first(v)); }
     // The same for a vector of a stream, which nobody reads again soon: what is on its way takes no line of the first cache from the rest (topk_logits of 2048 rows of 128256
-    // bf16 131 us with `load`, 123 so).
+    // bf16 132 us with `load`, 122 so).
     __device__ __forceinline__ uint4 stream(int v) const {
         uint4 r;
         asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p + first(v)) : "memory");
