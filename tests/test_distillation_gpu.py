@@ -233,6 +233,21 @@ def _check_distill(z, idx, val, rest, w, tau, what=''):
     return loss, grad
 
 
+@pytest.mark.parametrize('k', [1, 100])
+def test_distill_around_the_default_shared_memory(k):
+    """Rows that a block holds whole, from 44 to 49 KB with its list."""
+    from ista_daslab_optimizers_b200 import distill_loss, distill_step
+    g = _gen(k)
+    for vocab in range(11200 - 3 * k, 12500 - 3 * k, 50):
+        z = _normal(g, 500, vocab)
+        idx = torch.randint(0, vocab, (500, k), generator=g, device='cuda', dtype=torch.int32)
+        val = _normal(g, 500, k)
+        loss, _ = distill_step(z, idx, val)
+        assert torch.equal(distill_loss(z, idx, val), loss)
+        if vocab % 500 == 0:
+            _check_distill(z, idx, val, None, None, 1.0)
+
+
 @pytest.mark.parametrize('dtype', [F32, BF16])
 @pytest.mark.parametrize('rows,vocab,k,v_dtype,tau,rest,masked,ragged,skip,gap', [
     (1, 1, 1, F32, 1.0, False, False, False, 0, 0), (2, 2, 1, F32, 1.0, True, False, False, 1, 0), (3, 9, 9, BF16, 2.0, False, False, False, 1, 3),
