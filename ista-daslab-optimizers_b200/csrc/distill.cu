@@ -55,8 +55,8 @@ struct Args {
 
 struct Shared {
     uint64_t bar;
-    double red[MOST_WARPS][3];
-    double part[5];                                // this CTA's part, read by the cluster: reference, S_t, m_k, S_k, B
+    double red[MOST_WARPS][4];
+    double part[6];                                // this CTA's part, read by the cluster: reference, S_t, m_k, S_k, its entries' B and e
     double inv, q_scale, P;                        // 1 / Sp, exp(Mk - L), P
     float max_t[MOST_WARPS], max_k[MOST_WARPS], ref_w[MOST_WARPS], sum_w[MOST_WARPS];
     float ref, off;
@@ -68,20 +68,21 @@ __device__ __forceinline__ double list_value(const Args& a, int64_t at) {
     return a.values_bf16 ? (double)bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(a.values)[at]) : (double)reinterpret_cast<const float*>(a.values)[at];
 }
 
-// Sums of three doubles over the first `warps` warps, in every thread.
-__device__ __forceinline__ void block_sum(Shared& sh, int warps, double& x, double& y, double& z) {
+// Sums of four doubles over the first `warps` warps, in every thread.
+__device__ __forceinline__ void block_sum(Shared& sh, int warps, double& x, double& y, double& z, double& u) {
     if (warp_id() < warps) {
 #pragma unroll
         for (int o = 16; o; o >>= 1) {
             x += __shfl_xor_sync(0xffffffffu, x, o);
             y += __shfl_xor_sync(0xffffffffu, y, o);
             z += __shfl_xor_sync(0xffffffffu, z, o);
+            u += __shfl_xor_sync(0xffffffffu, u, o);
         }
-        if (lane_id() == 0) { sh.red[warp_id()][0] = x; sh.red[warp_id()][1] = y; sh.red[warp_id()][2] = z; }
+        if (lane_id() == 0) { sh.red[warp_id()][0] = x; sh.red[warp_id()][1] = y; sh.red[warp_id()][2] = z; sh.red[warp_id()][3] = u; }
     }
     __syncthreads();
-    x = y = z = 0.0;
-    for (int w = 0; w < warps; ++w) { x += sh.red[w][0]; y += sh.red[w][1]; z += sh.red[w][2]; }
+    x = y = z = u = 0.0;
+    for (int w = 0; w < warps; ++w) { x += sh.red[w][0]; y += sh.red[w][1]; z += sh.red[w][2]; u += sh.red[w][3]; }
 }
 
 // factor * exp2((x - ref) scale) of a vector.
@@ -234,7 +235,7 @@ __global__ void __launch_bounds__(NT, (PER_THREAD > 1 ? 1024 : MODE == LOSS ? 15
 #pragma unroll
     for (int i = 0; i < WARPS; ++i) { mt = fmaxf(mt, sh.max_t[i]); mk = fmaxf(mk, sh.max_k[i]); }
     const double M = mt == -INF_F ? 0.0 : (double)mt, Mk = mk == -INF_F ? 0.0 : (double)mk;
-    double sum_p = 0.0, sum_k = 0.0, cross = 0.0, ek[PER_THREAD];
+    double sum_p = 0.0, sum_k = 0.0, cross = 0.0, own_e = 0.0, ek[PER_THREAD];
 #pragma unroll
     for (int i = 0; i < PER_THREAD; ++i) {
         if (i * NT >= k) break;
@@ -246,7 +247,9 @@ __global__ void __launch_bounds__(NT, (PER_THREAD > 1 ? 1024 : MODE == LOSS ? 15
         sum_p += e;
         if (idx[i] >= e0 && idx[i] < e1) {
             ek[i] = exp(yj[i] - Mk);
-            if (!(e == 0.0)) cross += e * (tj[i] - yj[i]);
+            own_e += e;
+            // (each relative to its reference: logits of 10^16, or masked by the type's lowest value on either side, would leave nothing of the other)
+            if (!(e == 0.0)) cross += e * ((tj[i] - M) - (yj[i] - Mk));
         }
     }
     const double e_rest = rest == -(double)INF_F ? 0.0 : exp(rest - M);
@@ -279,7 +282,7 @@ __global__ void __launch_bounds__(NT, (PER_THREAD > 1 ? 1024 : MODE == LOSS ? 15
         if (again) sh.dup = 1;
         else sum_k += ek[i];
     }
-    block_sum(sh, min(WARPS, (k + 31) / 32), sum_p, sum_k, cross);             // (its barrier: the positions are gone)
+    block_sum(sh, min(WARPS, (k + 31) / 32), sum_p, sum_k, cross, own_e);      // (its barrier: the positions are gone)
     const double Sp = sum_p + e_rest;
 
     // everything else: running maximum and sum a thread
@@ -384,7 +387,7 @@ __global__ void __launch_bounds__(NT, (PER_THREAD > 1 ? 1024 : MODE == LOSS ? 15
         St = ws == 0.0f ? 0.0 : (double)(ws * ex2((wr - R) * scale));
 #pragma unroll
         for (int o = WARPS / 2; o; o >>= 1) St += __shfl_xor_sync(0xffffffffu, St, o);
-        if (C > 1 && l == 0) { sh.part[0] = (double)R; sh.part[1] = St; sh.part[2] = Mk; sh.part[3] = sum_k; sh.part[4] = cross; }
+        if (C > 1 && l == 0) { sh.part[0] = (double)R; sh.part[1] = St; sh.part[2] = Mk; sh.part[3] = sum_k; sh.part[4] = cross; sh.part[5] = own_e; }
     }
     if (C > 1) cluster_arrive_wait();
     if (warp_id() == 0) {
@@ -394,6 +397,7 @@ __global__ void __launch_bounds__(NT, (PER_THREAD > 1 ? 1024 : MODE == LOSS ? 15
             const float r = there ? (float)cluster_load_f64(&sh.part[0], l) : -INF_F;
             const double st = there ? cluster_load_f64(&sh.part[1], l) : 0.0, mkk = there ? cluster_load_f64(&sh.part[2], l) : none;
             const double sk = there ? cluster_load_f64(&sh.part[3], l) : 0.0;
+            const double oe = there ? cluster_load_f64(&sh.part[5], l) : 0.0;
             B = there ? cluster_load_f64(&sh.part[4], l) : 0.0;
             R = st == 0.0 ? -INF_F : r;
             K = sk == 0.0 ? none : mkk;
@@ -408,8 +412,11 @@ __global__ void __launch_bounds__(NT, (PER_THREAD > 1 ? 1024 : MODE == LOSS ? 15
             for (int o = 4; o; o >>= 1) {
                 St += __shfl_xor_sync(0xffffffffu, St, o);
                 Sk += __shfl_xor_sync(0xffffffffu, Sk, o);
-                B += __shfl_xor_sync(0xffffffffu, B, o);
             }
+            // B relative to the one reference of all
+            if (!(oe == 0.0)) B -= oe * (mkk - (Sk == 0.0 ? (double)R * a.inv_tau : K));
+#pragma unroll
+            for (int o = 4; o; o >>= 1) B += __shfl_xor_sync(0xffffffffu, B, o);
         } else {
             K = sum_k == 0.0 ? none : Mk;
         }
@@ -426,19 +433,20 @@ __global__ void __launch_bounds__(NT, (PER_THREAD > 1 ? 1024 : MODE == LOSS ? 15
         const double lg = log(l == 0 ? Sa : l == 1 ? (apart ? St : Sr) : Sp);
         const double log_a = __shfl_sync(0xffffffffu, lg, 0), log_t = __shfl_sync(0xffffffffu, lg, 1), log_p = __shfl_sync(0xffffffffu, lg, 2);
         const bool above = apart && y - A > 700.0;                             // the list is nothing against the rest
-        const double Lt = (apart ? y : A) + log_t, L = above ? Lt : A + log_a;
-        const double inv = Sp == 0.0 ? 0.0 : 1.0 / Sp, Lp = Sp == 0.0 ? 0.0 : M + log_p;
+        const double Lt = (apart ? y - A : 0.0) + log_t, L = above ? Lt : log_a;           // relative to A, too
+        const double inv = Sp == 0.0 ? 0.0 : 1.0 / Sp;
         const double pt = e_rest * inv, mass = sum_p * inv, P = Sp == 0.0 ? 0.0 : 1.0;
         double l_ = 0.0, off = 0.0;
-        if (!(Sp == 0.0)) l_ = B * inv - Lp * mass + (no_rest && no_list ? none : L) * P;
-        if (!(pt == 0.0)) l_ += no_rest ? (double)INF_F : pt * (rest - Lp - Lt);
+        if (!(Sp == 0.0)) l_ = B * inv + mass * (L - log_p);
+        if (!(pt == 0.0)) l_ += no_rest ? (double)INF_F : pt * ((rest - M) - log_p + (L - Lt));
         if (!no_rest) off = (P * (above ? 1.0 : Sr / Sa) - pt) / St;
+        else if (no_list && P != 0.0) l_ = off = __longlong_as_double(0x7FF8000000000000ll);        // no distribution at all
         if (l == 0) {
             if (rank == 0) a.loss[row] = (float)(l_ * (double)w);
             if (rank == 0 && MODE == LOSS) a.stats[row] = make_float2(no_rest ? 0.0f : R, (float)off);
             // q_j = exp(y_j - Mk) exp(Mk - L); where A is this CTA's own reference, the second factor is 1 / Sa
             sh.inv = inv; sh.P = P;
-            sh.q_scale = Mk == A && !above ? 1.0 / Sa : exp(Mk - (no_rest && no_list ? none : L));
+            sh.q_scale = !(off == off) ? off : sum_k == 0.0 ? 0.0 : Mk == A && !above ? 1.0 / Sa : exp((Mk - A) - L);
             sh.ref = no_rest ? 0.0f : R;
             sh.off = (float)off;
         }

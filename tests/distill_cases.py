@@ -65,22 +65,28 @@ def distill(z, idx, val, rest, weights, tau):
     to = torch.where(there, idx.long(), vocab)
     t = torch.where(there, val.double() / tau, -math.inf)
     r = torch.full((rows,), -math.inf, dtype=torch.float64, device=z.device) if rest is None else rest.double()
-    lp = torch.logsumexp(torch.cat([t, r[:, None]], 1), 1)
-    none = lp == -math.inf
-    lp = torch.where(none, 0.0, lp)
+    # everything relative to the rows' largest: where those are 1e16, or the type's lowest value, nothing else would be left of 64 bits either
+    m = torch.cat([t, r[:, None]], 1).amax(1)
+    none = m == -math.inf
+    m = torch.where(none, 0.0, m)
+    t, r = t - m[:, None], r - m
+    lp = torch.where(none, 0.0, torch.logsumexp(torch.cat([t, r[:, None]], 1), 1))
     p = torch.zeros(rows, vocab + 1, dtype=torch.float64, device=z.device).scatter_add_(1, to, torch.where(there, (t - lp[:, None]).exp(), 0.0))
     in_list = torch.zeros(rows, vocab + 1, dtype=torch.bool, device=z.device).scatter_(1, to, True)
     p, in_list = p[:, :vocab], in_list[:, :vocab]
     pt = (r - lp).exp()
+    y = y - y.amax(1, keepdim=True)
     total = torch.logsumexp(y, 1)
     outside = y.masked_fill(in_list, -math.inf)
-    mass = torch.logsumexp(outside, 1)
+    o = outside.amax(1)
+    o = torch.where(o == -math.inf, 0.0, o)
+    mass = torch.logsumexp(outside - o[:, None], 1)
     log_q = y - total[:, None]
     lg = torch.cat([log_q, torch.zeros_like(log_q[:, :1])], 1).gather(1, to)
     pj = torch.where(there, (t - lp[:, None]).exp(), 0.0)
     loss = torch.where(pj > 0, pj * (t - lp[:, None] - lg), 0.0).sum(1)
-    loss = loss + torch.where(pt > 0, pt * (r - lp - (mass - total)), 0.0)
-    share = torch.where(in_list | (mass == -math.inf)[:, None], 0.0, pt[:, None] * (outside - mass[:, None]).exp())
+    loss = loss + torch.where(pt > 0, pt * (r - lp - (mass + (o - total))), 0.0)
+    share = torch.where(in_list | (mass == -math.inf)[:, None], 0.0, pt[:, None] * (outside - o[:, None] - mass[:, None]).exp())
     q = log_q.exp()
     grad = torch.where(none[:, None], 0.0, (q - p - share) / tau)
     size = (q + p + share) / tau

@@ -233,6 +233,35 @@ def _check_distill(z, idx, val, rest, w, tau, what=''):
     return loss, grad
 
 
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('rows,vocab', [(2, 40001), (60, 700), (500, 3001)])
+@pytest.mark.parametrize('kind', ['lowest_list', 'huge_list', 'huge_rest', 'lowest_logits', 'lowest_list_and_logits', 'far_below', 'no_logits'])
+def test_distill_far_from_zero(dtype, rows, vocab, kind):
+    """Masks of the type's lowest value that leave a row of the teacher or the student nothing, and logits so large that sums with ordinary ones lose those."""
+    g = _gen(rows + vocab)
+    k, low = 37, torch.finfo(dtype).min
+    z = _normal(g, rows, vocab, scale=3.0)
+    idx = torch.randint(0, vocab, (rows, k), generator=g, device='cuda', dtype=torch.int32)
+    val = _normal(g, rows, k)
+    rest = _normal(g, rows)
+    if kind in ('lowest_list', 'lowest_list_and_logits'):
+        val[:], rest[:] = low, -INF
+    if kind == 'huge_list':
+        val = val * 2.0 ** 55
+    if kind == 'huge_rest':
+        rest = rest.abs() * 2.0 ** 60
+    if kind in ('lowest_logits', 'lowest_list_and_logits'):
+        z[:] = low
+        z[::2, 5] = 0.75 * low
+    if kind == 'far_below':                          # every logit of the list but a few is -inf, the others far below 0
+        z -= 3000.0
+        z.scatter_(1, idx[:, :30].long(), -INF)
+        val[:, :30], rest = -INF, None
+    if kind == 'no_logits':
+        z[::2] = -INF
+    _check_distill(z.to(dtype), idx, val.to(dtype), rest, None, 1.0 if kind != 'huge_list' else 2.0)
+
+
 @pytest.mark.parametrize('k', [1, 100])
 def test_distill_around_the_default_shared_memory(k):
     """Rows that a block holds whole, from 44 to 49 KB with its list."""
