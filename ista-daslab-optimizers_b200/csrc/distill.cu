@@ -432,7 +432,7 @@ __global__ void __launch_bounds__(NT, (PER_THREAD > 1 ? 1024 : MODE == LOSS ? 15
         // three logarithms in three lanes
         const double lg = log(l == 0 ? Sa : l == 1 ? (apart ? St : Sr) : Sp);
         const double log_a = __shfl_sync(0xffffffffu, lg, 0), log_t = __shfl_sync(0xffffffffu, lg, 1), log_p = __shfl_sync(0xffffffffu, lg, 2);
-        const bool above = apart && y - A > 700.0;                             // the list is nothing against the rest
+        const bool above = apart && y - A > 700.0 && Sk == Sk;                 // the list is nothing against the rest
         const double Lt = (apart ? y - A : 0.0) + log_t, L = above ? Lt : log_a;           // relative to A, too
         const double inv = Sp == 0.0 ? 0.0 : 1.0 / Sp;
         const double pt = e_rest * inv, mass = sum_p * inv, P = Sp == 0.0 ? 0.0 : 1.0;
@@ -440,10 +440,11 @@ __global__ void __launch_bounds__(NT, (PER_THREAD > 1 ? 1024 : MODE == LOSS ? 15
         if (!(Sp == 0.0)) l_ = B * inv + mass * (L - log_p);
         if (!(pt == 0.0)) l_ += no_rest ? (double)INF_F : pt * ((rest - M) - log_p + (L - Lt));
         if (!no_rest) off = (P * (above ? 1.0 : Sr / Sa) - pt) / St;
-        else if (no_list && P != 0.0) l_ = off = __longlong_as_double(0x7FF8000000000000ll);        // no distribution at all
+        else if (no_list || !(Sk == Sk)) l_ = off = __longlong_as_double(0x7FF8000000000000ll);     // no distribution at all
+        if (P == 0.0) l_ = off = 0.0;               // nothing to compare with
         if (l == 0) {
             if (rank == 0) a.loss[row] = (float)(l_ * (double)w);
-            if (rank == 0 && MODE == LOSS) a.stats[row] = make_float2(no_rest ? 0.0f : R, (float)off);
+            if (rank == 0 && MODE == LOSS) a.stats[row] = make_float2(P == 0.0 ? INF_F : no_rest ? 0.0f : R, (float)off);
             // q_j = exp(y_j - Mk) exp(Mk - L); where A is this CTA's own reference, the second factor is 1 / Sa
             sh.inv = inv; sh.P = P;
             sh.q_scale = !(off == off) ? off : sum_k == 0.0 ? 0.0 : Mk == A && !above ? 1.0 / Sa : exp((Mk - A) - L);
@@ -469,11 +470,12 @@ __global__ void __launch_bounds__(NT, (PER_THREAD > 1 ? 1024 : MODE == LOSS ? 15
                 p = 0.0;
                 for (int n = 0; n < k; ++n) if (s_idx[n] == idx[i]) p += s_e[n];
             }
-            d[i] = (float)(P * (ek[i] * q_scale) - p * inv);
+            d[i] = P == 0.0 ? 0.0f : (float)(P * (ek[i] * q_scale) - p * inv);
             if (MODE == LOSS) a.list_grad[row * k + j] = d[i];
         }
     }
     if (MODE == STEP) {
+        if (P == 0.0) { zero_part<T, NT>(a, row, rank, C); return; }
         T* out = reinterpret_cast<T*>(a.grad) + row * a.grad_pitch;
         // (the last time that the row is read, and what is written is not read here: neither has to stay in L2, where the rows of the other CTAs wait)
         if (RESIDENT) {
@@ -501,6 +503,7 @@ __global__ void __launch_bounds__(GRAD_NT, 3) distill_grad_kernel(Args a) {
     const float w = a.weights ? a.weights[row] : 1.0f;
     if (w == 0.0f) { zero_part<T, GRAD_NT>(a, row, part, parts); return; }
     const float2 st = a.stats[row];
+    if (st.x == INF_F && st.y == 0.0f) { zero_part<T, GRAD_NT>(a, row, part, parts); return; }      // a row without a teacher
     const float back = (float)((double)w * (double)a.grad_loss[row * a.grad_loss_stride] * a.inv_tau);
     const RowGrid<T> g(reinterpret_cast<const T*>(a.logits) + row * a.pitch, a.vocab);
     int v0, v1;

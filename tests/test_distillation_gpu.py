@@ -235,7 +235,7 @@ def _check_distill(z, idx, val, rest, w, tau, what=''):
 
 @pytest.mark.parametrize('dtype', [F32, BF16])
 @pytest.mark.parametrize('rows,vocab', [(2, 40001), (60, 700), (500, 3001)])
-@pytest.mark.parametrize('kind', ['lowest_list', 'huge_list', 'huge_rest', 'lowest_logits', 'lowest_list_and_logits', 'far_below', 'no_logits'])
+@pytest.mark.parametrize('kind', ['lowest_list', 'huge_list', 'huge_rest', 'lowest_logits', 'lowest_list_and_logits', 'far_below', 'no_logits', 'nan_and_no_teacher', 'nan_in_list', 'nan_in_list_alone'])
 def test_distill_far_from_zero(dtype, rows, vocab, kind):
     """Masks of the type's lowest value that leave a row of the teacher or the student nothing, and logits so large that sums with ordinary ones lose those."""
     g = _gen(rows + vocab)
@@ -257,6 +257,15 @@ def test_distill_far_from_zero(dtype, rows, vocab, kind):
         z -= 3000.0
         z.scatter_(1, idx[:, :30].long(), -INF)
         val[:, :30], rest = -INF, None
+    if kind == 'nan_and_no_teacher':
+        val[:], rest[:] = -INF, -INF
+        z[::2, ::97] = math.nan
+    if kind == 'nan_in_list':
+        z.scatter_(1, idx.long(), -2000.0)
+        z[0, idx[0, 3]] = math.nan
+    if kind == 'nan_in_list_alone':
+        z = torch.full_like(z, -INF).scatter_(1, idx.long(), 1.0)
+        z[0, idx[0, 3]] = math.nan
     if kind == 'no_logits':
         z[::2] = -INF
     _check_distill(z.to(dtype), idx, val.to(dtype), rest, None, 1.0 if kind != 'huge_list' else 2.0)
