@@ -11,11 +11,11 @@
 // the list is worked on): one pass with a running maximum and sum, and for the gradient a second one that reads no global memory.  The list's positions are
 // overwritten by -inf there, so the sum over the others is their own, not a difference of two large ones.  The k terms of the list are in 64 bits: near the
 // optimum the loss is what is left of a difference, and there an error of S_t only enters with the factor q_t - p_t as long as the terms that share it are exact.
-// Rows too long for that are read twice, with a bitmap of the list's positions.  The CTAs exchange five numbers through distributed shared memory, in rank order:
+// Rows too long for that are read twice, with a bitmap of the list's positions.  The CTAs exchange six numbers through distributed shared memory, in rank order:
 // results do not depend on timing.
 //
 // Bound by HBM and by the chain of phases around the passes (list, block and cluster sums, three logarithms: some 5 us a row, which the SM's other rows cover in part).
-// bf16, rows of 128256, k = 64 (us): loss of 1536 rows 75 (5.2 TB/s), its gradient 149 (6.2 TB/s), loss and gradient of 4096 rows in one call 435 (4.8 TB/s of the two passes
+// bf16, rows of 128256, k = 64 (us): loss of 1536 rows 75 (5.2 TB/s), its gradient 149 (6.2 TB/s), loss and gradient of 4096 rows in one call 443 (4.7 TB/s of the two passes
 // over HBM that it needs; what it holds and what L2 keeps leave 1.09 of their bytes; 569 before anything was held).
 #include <type_traits>
 #include "rows.cuh"
