@@ -609,3 +609,26 @@ def test_repeated_calls_give_the_same_bits():
             again = distill_step(z, idx, val, rest, w) + topk_logits(z, 100)
             for a, b in zip(first, again):
                 assert torch.equal(a, b)
+
+
+# ------------------------------------------------------------------------------------------------ kernels that begin while the one before them ends
+
+def test_products_of_both_forms_in_a_row():
+    """Tiles of one CTA (with and without a split inner size) and of two, which take all of an SM's tensor memory, behind one another without a wait: every product is
+    the one that it is alone."""
+    from ista_daslab_optimizers_b200 import int8_matmul, _native as N
+    g = _gen(21)
+    problems = []
+    for m, n, k in ((16, 200, 128), (300, 3000, 128), (41, 4096, 1024), (700, 2000, 256), (5, 19000, 64), (1025, 2305, 300), (128, 400, 6400)):
+        a, b = _codes(g, m, k), _codes(g, n, k)
+        sa, sb = torch.rand(m, generator=g, device='cuda') + 0.01, torch.rand(n, generator=g, device='cuda') * 0.01
+        torch.cuda.synchronize()
+        problems.append((a, b, sa, sb, int8_matmul(a, b, sa, sb, dtype=F32)))
+        torch.cuda.synchronize()
+        want, tol = D.matmul(a, b, sa, sb, None)
+        D.assert_near(problems[-1][4], want, tol, f'{m} x {n} x {k}')
+    for _ in range(20):
+        outs = [(int8_matmul(*p[:4], dtype=F32), p[4]) for p in problems + problems[::-1]]
+        for out, want in outs:
+            assert torch.equal(out, want)
+    assert N.device_error() == 0
