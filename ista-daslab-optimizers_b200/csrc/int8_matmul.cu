@@ -323,14 +323,15 @@ __global__ void __launch_bounds__(256) int8_rows_kernel(const __grid_constant__ 
 #pragma unroll
     for (int i = 0; i < M; ++i) a[i] = g.a + (int64_t)min(i, g.m - 1) * g.a_pitch;
     const int whole = g.k / 16;
+    // (ordinary loads: the kernel before, which may have written the codes, was still running when this one began, and the non-coherent path is for what nobody writes meanwhile)
 #pragma unroll 4
     for (int v = lane; v < whole; v += 32) {
         int4 w[R];
 #pragma unroll
-        for (int r = 0; r < R; ++r) w[r] = __ldg(reinterpret_cast<const int4*>(b[r]) + v);
+        for (int r = 0; r < R; ++r) w[r] = reinterpret_cast<const int4*>(b[r])[v];
 #pragma unroll
         for (int i = 0; i < M; ++i) {
-            const int4 x = __ldg(reinterpret_cast<const int4*>(a[i]) + v);
+            const int4 x = reinterpret_cast<const int4*>(a[i])[v];
 #pragma unroll
             for (int r = 0; r < R; ++r)
                 acc[i][r] = __dp4a(x.x, w[r].x, __dp4a(x.y, w[r].y, __dp4a(x.z, w[r].z, __dp4a(x.w, w[r].w, acc[i][r]))));

@@ -632,3 +632,30 @@ def test_products_of_both_forms_in_a_row():
         for out, want in outs:
             assert torch.equal(out, want)
     assert N.device_error() == 0
+
+
+@pytest.mark.parametrize('m', [1, 2, 3, 4])
+def test_product_reads_what_the_kernel_before_it_wrote(m):
+    """A few tokens quantised into one buffer again and again, each time with the product behind it and no wait between."""
+    from ista_daslab_optimizers_b200 import int8_matmul, quantize_rows
+    g = _gen(31 + m)
+    width, channels, times = 4096, 1500, 40
+    b, sb = quantize_rows(_normal(g, channels, width, scale=0.1))
+    x = _normal(g, times, m, width)
+    codes, scales = torch.empty(m, width, dtype=torch.int8, device='cuda'), torch.empty(m, device='cuda')
+    for _ in range(3):
+        outs = []
+        for i in range(times):
+            quantize_rows(x[i], codes, scales)
+            outs.append(int8_matmul(codes, b, scales, sb, dtype=F32))
+        for i in range(times):
+            c, s = D.quantize(x[i])
+            want, tol = D.matmul(c, b, s, sb, None)
+            D.assert_near(outs[i], want, tol, f'call {i}')
+        # the weights written again, too
+        wide = _normal(g, channels, width, scale=0.1)
+        quantize_rows(wide, b, sb)
+        out = int8_matmul(codes, b, scales, sb, dtype=F32)
+        want_b, want_sb = D.quantize(wide)
+        want, tol = D.matmul(c, want_b, s, want_sb, None)
+        D.assert_near(out, want, tol, 'weights')
