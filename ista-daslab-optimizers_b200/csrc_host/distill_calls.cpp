@@ -248,18 +248,35 @@ struct DistillLoss : torch::autograd::Function<DistillLoss> {
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list upstream) {
         const auto saved = ctx->get_saved_variables();
-        const at::Tensor &logits = saved[0], &indices = saved[1], &weights = saved[2], &stats = saved[3], &list_grad = saved[4];
         at::Tensor up = upstream[0];
         if (!up.defined()) return {at::Tensor(), at::Tensor(), at::Tensor()};
         const bool graph = c10::GradMode::is_enabled();
         at::Tensor grad;
         {
             const c10::AutoGradMode off(false);
-            const Target on(logits);
-            if (up.scalar_type() != at::kFloat) up = up.to(at::kFloat);
-            const int64_t rows = logits.size(0), vocab = logits.size(1);
+            const Target on(up);
+            const int64_t rows = up.size(0);
+            // What hooks for saved tensors give back can be anything: the library only gets what is like what was saved (its distances may be others).  (The messages are literals:
+            // a compiler that links its C++ library statically has streams of its own here, which do not know torch's locale.)
+            auto back = [&](size_t i, at::ScalarType type) {
+                const at::Tensor& t = saved[i];
+                TORCH_CHECK(t.layout() == at::kStrided && t.is_cuda() && t.device() == up.device() && t.scalar_type() == type && t.dim() >= 1 && t.size(0) == rows,
+                            "distill_loss: a saved tensor came back with another device, layout, type or number of rows (hooks for saved tensors have to give back what they got)");
+                return t;
+            };
+            const at::Tensor indices = back(1, at::kInt).contiguous(), stats = back(3, at::kFloat).contiguous(), list_grad = back(4, at::kFloat).contiguous();
+            const at::Tensor weights = saved[2].defined() ? back(2, at::kFloat).contiguous() : at::Tensor();
+            at::Tensor logits = back(0, saved[0].scalar_type() == at::kBFloat16 ? at::kBFloat16 : at::kFloat);
+            TORCH_CHECK(logits.dim() == 2 && indices.dim() == 2 && list_grad.sizes() == indices.sizes() && stats.dim() == 2 && stats.size(1) == 2 &&
+                            (!weights.defined() || weights.dim() == 1),
+                        "distill_loss: a saved tensor came back in another shape (hooks for saved tensors have to give back what they got)");
             Rows z;
-            z.of(logits);
+            if (!z.of(logits)) {
+                logits = logits.contiguous();
+                z.of(logits);
+            }
+            const int64_t vocab = logits.size(1);
+            if (up.scalar_type() != at::kFloat) up = up.to(at::kFloat);
             grad = fresh({rows, vocab}, logits.scalar_type(), logits);
             throw_if(g_library.distill_grad(rows, vocab, indices.size(1), z.p, code(logits), z.pitch, static_cast<const int32_t*>(indices.data_ptr()), vector_at(weights),
                                             ctx->saved_data["temperature"].toDouble(), vector_at(stats), vector_at(list_grad), vector_at(up), up.stride(0),

@@ -659,3 +659,40 @@ def test_product_reads_what_the_kernel_before_it_wrote(m):
         want_b, want_sb = D.quantize(wide)
         want, tol = D.matmul(c, want_b, s, want_sb, None)
         D.assert_near(out, want, tol, 'weights')
+
+
+# ------------------------------------------------------------------------------------------------ hooks for saved tensors
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+def test_saved_tensors_through_hooks(dtype):
+    """What is saved for the backward pass can be moved to the host, copied, or laid out otherwise meanwhile; what comes back as something else is refused."""
+    from ista_daslab_optimizers_b200 import distill_loss, _native as N
+    hooks = torch.autograd.graph.saved_tensors_hooks
+    z, idx, val, rest, w = _problem(5, 3001, 8, dtype, F32, 1.0, True, True, False, 1, 3)
+
+    def gradient(leaf, context=None):
+        if context is None:
+            loss = distill_loss(leaf, idx, val, rest, w)
+        else:
+            with context:
+                loss = distill_loss(leaf, idx, val, rest, w)
+        return torch.autograd.grad(loss.sum(), leaf)[0]
+
+    leaf = z.detach().requires_grad_()
+    want = gradient(leaf)
+    turned = lambda t: t.t().contiguous().t() if t.dim() == 2 else t.clone()      # noqa: E731
+    for context in (torch.autograd.graph.save_on_cpu(), torch.autograd.graph.save_on_cpu(pin_memory=True), hooks(lambda t: t, torch.clone), hooks(lambda t: t, turned)):
+        assert torch.equal(gradient(leaf, context), want)
+    for other in (lambda t: t.cpu(), lambda t: t.double(), lambda t: t.half(), lambda t: t.to_sparse(), lambda t: t[:-1], lambda t: t.flatten(), lambda t: t[..., :1]):
+        before = N.kernel_launch_count()
+        with pytest.raises(RuntimeError, match='came back'):
+            gradient(leaf, hooks(lambda t: t, other))
+        assert N.kernel_launch_count() <= before + 1          # the loss, no gradient
+
+    def broken(t):
+        raise KeyError('a hook of the user')
+
+    for context in (hooks(broken, lambda t: t), hooks(lambda t: t, broken)):
+        with pytest.raises(KeyError, match='a hook of the user'):
+            gradient(leaf, context)
+    assert torch.equal(gradient(leaf), want)
