@@ -2,6 +2,8 @@
 #include <math.h>
 #include <string.h>
 #include <atomic>
+#include <mutex>
+#include <utility>
 #include <vector>
 #include <algorithm>
 #include "common.cuh"
@@ -43,6 +45,26 @@ int device_sm_count() {
         cached_dev = (cached < 0) ? -1 : dev;
     }
     return cached;
+}
+
+// The limit belongs to the kernel on the device, not to a launch, and calls come from several threads at once: set to what one launch needs, it could be lowered by another before that
+// launch.  So it is set once per kernel and device, to all that a block can have beside the kernel's static memory.
+int allow_shared_memory(const void* kernel) {
+    static std::mutex mutex;
+    static std::vector<std::pair<int, const void*>> allowed;         // sorted
+    int dev = 0;
+    MAB_CUDA_TRY(cudaGetDevice(&dev));
+    const std::pair<int, const void*> key(dev, kernel);
+    const std::lock_guard<std::mutex> lock(mutex);
+    const auto at = std::lower_bound(allowed.begin(), allowed.end(), key);
+    if (at != allowed.end() && *at == key) return MAB_OK;
+    const int most = device_max_optin_smem();
+    if (most < 0) return MAB_ERR_CUDA;
+    cudaFuncAttributes attr;
+    MAB_CUDA_TRY(cudaFuncGetAttributes(&attr, kernel));
+    MAB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most - (int)attr.sharedSizeBytes));
+    allowed.insert(at, key);
+    return MAB_OK;
 }
 
 int device_max_optin_smem() { return device_attr(cudaDevAttrMaxSharedMemoryPerBlockOptin, "query shared memory per block"); }

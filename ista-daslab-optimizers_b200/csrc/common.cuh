@@ -15,6 +15,7 @@ void set_error(const char* fmt, ...);
 int  cuda_fail(cudaError_t e, const char* what);   // records and returns MAB_ERR_CUDA
 int  device_sm_count();                            // cached per device, < 0 on failure
 int  device_max_optin_smem();                      // < 0 on failure
+int  allow_shared_memory(const void* kernel);      // lets a kernel have all the dynamic shared memory of the current device
 void count_launch();                               // bumps the process-wide kernel launch counter
 
 #define MAB_CUDA_TRY(expr)                                                     \

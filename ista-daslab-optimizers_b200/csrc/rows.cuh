@@ -180,7 +180,8 @@ __device__ __forceinline__ void kernel_before_is_done() {
 // Launches `kernel` with clusters of `cluster` CTAs (1: without) and counts it.  (Above 48 KB with the kernel's own static memory, a few KB, the size has to be allowed.)
 template <typename... P, typename... A>
 static int launch_rows(void (*kernel)(P...), const char* what, int64_t ctas, int threads, size_t smem, int cluster, cudaStream_t s, A... args) {
-    if (smem > 32 * 1024) MAB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    if (smem > 32 * 1024)
+        if (int rc = allow_shared_memory(reinterpret_cast<const void*>(kernel))) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)ctas);
     cfg.blockDim = dim3((unsigned)threads);

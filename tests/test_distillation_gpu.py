@@ -696,3 +696,78 @@ def test_saved_tensors_through_hooks(dtype):
         with pytest.raises(KeyError, match='a hook of the user'):
             gradient(leaf, context)
     assert torch.equal(gradient(leaf), want)
+
+
+# ------------------------------------------------------------------------------------------------ calls of one kernel with different sizes
+
+def test_threads_with_different_sizes():
+    """Threads whose calls are the same kernels with other amounts of shared memory: rows of other lengths, products with other inner sizes, lists of other lengths."""
+    import threading
+    from ista_daslab_optimizers_b200 import distill_loss, distill_step, int8_matmul, topk_logits
+    g = _gen(41)
+    sizes = ((9000, 640, 20), (15000, 128, 64), (12000, 300, 1000), (10000, 1024, 700))
+    problems = []
+    for vocab, inner, k in sizes:
+        z, val = _normal(g, 500, vocab), _normal(g, 500, 20)
+        idx = torch.randint(0, vocab, (500, 20), generator=g, device='cuda', dtype=torch.int32)
+        a, b = _codes(g, 40, inner), _codes(g, 4000, inner)
+        sa, sb = torch.rand(40, generator=g, device='cuda'), torch.rand(4000, generator=g, device='cuda')
+        few = z[:6].contiguous()
+        problems.append((lambda z=z, idx=idx, val=val: distill_step(z, idx, val), lambda z=z, idx=idx, val=val: (distill_loss(z, idx, val),),
+                         lambda a=a, b=b, sa=sa, sb=sb: (int8_matmul(a, b, sa, sb),), lambda few=few, k=k: topk_logits(few, k)))
+    want = [[call() for call in calls] for calls in problems]
+    torch.cuda.synchronize()
+    errors, start = [], threading.Barrier(len(problems))
+
+    def work(n):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                start.wait()
+                for _ in range(60):
+                    got = [call() for call in problems[n]]
+                for outs, ref in zip(got, want[n]):
+                    for x, y in zip(outs, ref):
+                        assert torch.equal(x, y)
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:                           # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(n,)) for n in range(len(problems))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors, errors[0]
+
+
+def test_one_graph_with_different_sizes_of_one_kernel():
+    """A captured graph holds launches of the same kernels with other amounts of shared memory, and eager calls with others still come between capture and replay."""
+    from ista_daslab_optimizers_b200 import distill_step, int8_matmul
+    g = _gen(43)
+    inputs = []
+    for vocab, inner in ((15000, 1024), (9000, 128), (12000, 640)):
+        idx = torch.randint(0, vocab, (400, 20), generator=g, device='cuda', dtype=torch.int32)
+        inputs.append((_normal(g, 400, vocab), idx, _normal(g, 400, 20), _codes(g, 40, inner), _codes(g, 4000, inner), torch.rand(40, generator=g, device='cuda'),
+                       torch.rand(4000, generator=g, device='cuda')))
+
+    def chain():
+        outs = []
+        for z, idx, val, a, b, sa, sb in inputs:
+            outs += [*distill_step(z, idx, val), int8_matmul(a, b, sa, sb)]
+        return outs
+
+    want = chain()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = chain()
+    small = torch.zeros(300, 8300, device='cuda')
+    distill_step(small, inputs[0][1][:300, :2].contiguous() % 8300, inputs[0][2][:300, :2].contiguous())
+    for _ in range(2):
+        for o in out:
+            o.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        for x, y in zip(out, want):
+            assert torch.equal(x, y)
