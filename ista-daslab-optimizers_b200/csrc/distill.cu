@@ -274,10 +274,15 @@ __global__ void __launch_bounds__(NT, (PER_THREAD > 1 ? 1024 : MODE == LOSS ? 15
         } else if (N == 4) {
             again = atomicExch(reinterpret_cast<uint32_t*>(part) + (idx[i] - f0), 0xFF800000u) == 0xFF800000u;
         } else {
+            // (half a word; another entry can have the other half.  All 16 bits are compared: a NaN with its sign set has those of -inf, too)
             const int shift = (idx[i] - f0 & 1) * 16;
             uint32_t* word = reinterpret_cast<uint32_t*>(part) + (idx[i] - f0 >> 1);
-            again = (atomicOr(word, 0xFF80u << shift) >> shift & 0xFF80u) == 0xFF80u;
-            atomicAnd(word, ~(0x007Fu << shift));
+            uint32_t seen = *reinterpret_cast<volatile uint32_t*>(word), was;
+            do {
+                was = seen;
+                seen = atomicCAS(word, was, (was & ~(0xFFFFu << shift)) | 0xFF80u << shift);
+            } while (seen != was);
+            again = (was >> shift & 0xFFFFu) == 0xFF80u;
         }
         if (again) sh.dup = 1;
         else sum_k += ek[i];

@@ -771,3 +771,29 @@ def test_one_graph_with_different_sizes_of_one_kernel():
         torch.cuda.synchronize()
         for x, y in zip(out, want):
             assert torch.equal(x, y)
+
+
+# ------------------------------------------------------------------------------------------------ NaN of either sign in a list
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('rows,vocab', [(2, 40001), (60, 700), (500, 3001), (3, 9), (300, 200000)])
+@pytest.mark.parametrize('bits', ['sign', 'sign_least', 'sign_all', 'plain'])
+def test_distill_nan_in_list_whatever_its_bits(dtype, rows, vocab, bits):
+    """A listed logit that is NaN, with and without its sign, makes its row NaN throughout, whether the teacher gives the entry mass or not; -inf and repeated entries stay what they are."""
+    g = _gen(vocab)
+    k = 5
+    z = _normal(g, rows, vocab).to(dtype)
+    nan = dict(sign=0xFFC0, sign_least=0xFF81, sign_all=0xFFFF, plain=0x7FC0)[bits]
+    idx = torch.stack([torch.randperm(vocab, generator=g, device='cuda')[:k] for _ in range(rows)]).int()
+    idx[:, 4] = idx[:, 3]
+    z.scatter_(1, idx[:, 2:3].long(), -INF)
+    word, n = (torch.int16, nan) if dtype == BF16 else (torch.int32, nan << 16 | (0xFFFF if bits == 'sign_all' else 0))
+    z.view(word)[0, idx[0, 1].item()] = n - (1 << (16 if dtype == BF16 else 32)) if n >> (15 if dtype == BF16 else 31) else n
+    val = _normal(g, rows, k)
+    val[:, 2] = -INF                                     # nothing where the student has nothing
+    assert z.isnan().sum() == 1
+    loss, grad = _check_distill(z, idx, val, None, None, 1.0, 'with mass')
+    assert loss[0].isnan() and grad[0].isnan().all() and torch.isfinite(loss[1:]).all() and torch.isfinite(grad[1:]).all()
+    val[:, 1] = -INF
+    _, grad = _check_distill(z, idx, val, None, None, 1.0, 'without')
+    assert grad[0].isnan().all() and torch.isfinite(grad[1:]).all()
