@@ -64,9 +64,12 @@ struct Shared {
     int dup;
 };
 
-__device__ __forceinline__ double list_value(const Args& a, int64_t at) {
-    return a.values_bf16 ? (double)bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(a.values)[at]) : (double)reinterpret_cast<const float*>(a.values)[at];
+__device__ __forceinline__ float list_value(const Args& a, int64_t at) {
+    return a.values_bf16 ? bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(a.values)[at]) : reinterpret_cast<const float*>(a.values)[at];
 }
+
+// A logit over the temperature: rounded, so that the difference of two equal ones is 0 however large they are (a fused subtraction would leave the product's rounding, 1 at 10^16).
+__device__ __forceinline__ double at_tau(const Args& a, float logit) { return __dmul_rn((double)logit, a.inv_tau); }
 
 // Sums of four doubles over the first `warps` warps, in every thread.
 __device__ __forceinline__ void block_sum(Shared& sh, int warps, double& x, double& y, double& z, double& u) {
@@ -191,13 +194,13 @@ __global__ void __launch_bounds__(NT, (PER_THREAD > 1 ? 1024 : MODE == LOSS ? 15
     uint32_t* bitmap = reinterpret_cast<uint32_t*>(part + (RESIDENT ? 0 : a.held));              // of the list's positions, where not everything is held
     // the list
     int idx[PER_THREAD];
-    double tj[PER_THREAD], yj[PER_THREAD];
+    float vj[PER_THREAD], zj[PER_THREAD];           // the teacher's logit and the student's
 #pragma unroll
     for (int i = 0; i < PER_THREAD; ++i) {
         if (i * NT >= k) break;
         const bool there = t + i * NT < k;
         idx[i] = there ? a.indices[row * k + t + i * NT] : -1;
-        tj[i] = there ? list_value(a, row * k + t + i * NT) * a.inv_tau : 0.0;
+        vj[i] = there ? list_value(a, row * k + t + i * NT) : 0.0f;
     }
     const double rest = a.rest ? (double)a.rest[row] : -(double)INF_F;
     // (the loads above are on their way)
@@ -211,17 +214,18 @@ __global__ void __launch_bounds__(NT, (PER_THREAD > 1 ? 1024 : MODE == LOSS ? 15
         for (int i = t; i < ((v1 - v0) * N + 31) / 32; i += NT) bitmap[i] = 0;
     if (t == 0) { sh.dup = 0; sh.edge[0] = sh.edge[1] = 0; }
 
-    float mt = -INF_F, mk = -INF_F;                 // largest t, largest y of this CTA's entries: as floats, only references
+    // The largest of the list, and of this CTA's entries the largest of the student's: before the temperature, so that they are exact.  (t and y as floats are infinite where a logit is the
+    // type's lowest and the temperature below 1, and off by more than a double's exponential covers where it is 1e16.)
+    float mt = -INF_F, mk = -INF_F;
 #pragma unroll
     for (int i = 0; i < PER_THREAD; ++i) {
         if (i * NT >= k) break;
         if (idx[i] < 0 || idx[i] >= a.vocab) idx[i] = -1;
         const bool own = idx[i] >= e0 && idx[i] < e1;
-        const float z = own ? Elem<T>::load(g.p, idx[i]) : 0.0f;
+        zj[i] = own ? Elem<T>::load(g.p, idx[i]) : 0.0f;
         if (t + i * NT < k) s_idx[t + i * NT] = idx[i];
-        if (idx[i] >= 0) mt = fmaxf(mt, (float)tj[i]);
-        yj[i] = (double)z * a.inv_tau;
-        if (own) mk = fmaxf(mk, (float)yj[i]);
+        if (idx[i] >= 0) mt = fmaxf(mt, vj[i]);
+        if (own) mk = fmaxf(mk, zj[i]);
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
@@ -230,11 +234,12 @@ __global__ void __launch_bounds__(NT, (PER_THREAD > 1 ? 1024 : MODE == LOSS ? 15
     }
     if (lane_id() == 0) { sh.max_t[warp_id()] = mt; sh.max_k[warp_id()] = mk; }
     __syncthreads();                                // (the barrier of the copy is there, or the bitmap is clear, too)
-    mt = (float)rest;
-    mk = -INF_F;
+    mt = mk = -INF_F;
 #pragma unroll
     for (int i = 0; i < WARPS; ++i) { mt = fmaxf(mt, sh.max_t[i]); mk = fmaxf(mk, sh.max_k[i]); }
-    const double M = mt == -INF_F ? 0.0 : (double)mt, Mk = mk == -INF_F ? 0.0 : (double)mk;
+    double M = fmax(at_tau(a, mt), rest);
+    if (M == -(double)INF_F) M = 0.0;
+    const double Mk = mk == -INF_F ? 0.0 : at_tau(a, mk);
     double sum_p = 0.0, sum_k = 0.0, cross = 0.0, own_e = 0.0, ek[PER_THREAD];
 #pragma unroll
     for (int i = 0; i < PER_THREAD; ++i) {
@@ -242,14 +247,15 @@ __global__ void __launch_bounds__(NT, (PER_THREAD > 1 ? 1024 : MODE == LOSS ? 15
         const int j = t + i * NT;
         ek[i] = 0.0;
         if (j >= k) continue;
-        const double e = idx[i] >= 0 ? exp(tj[i] - M) : 0.0;
+        const double from_M = at_tau(a, vj[i]) - M, e = idx[i] >= 0 ? exp(from_M) : 0.0;
         s_e[j] = e;
         sum_p += e;
         if (idx[i] >= e0 && idx[i] < e1) {
-            ek[i] = exp(yj[i] - Mk);
+            const double from_Mk = at_tau(a, zj[i]) - Mk;
+            ek[i] = exp(from_Mk);
             own_e += e;
             // (each relative to its reference: logits of 10^16, or masked by the type's lowest value on either side, would leave nothing of the other)
-            if (!(e == 0.0)) cross += e * ((tj[i] - M) - (yj[i] - Mk));
+            if (!(e == 0.0)) cross += e * (from_M - from_Mk);
         }
     }
     const double e_rest = rest == -(double)INF_F ? 0.0 : exp(rest - M);
@@ -419,7 +425,7 @@ __global__ void __launch_bounds__(NT, (PER_THREAD > 1 ? 1024 : MODE == LOSS ? 15
                 Sk += __shfl_xor_sync(0xffffffffu, Sk, o);
             }
             // B relative to the one reference of all
-            if (!(oe == 0.0)) B -= oe * (mkk - (Sk == 0.0 ? (double)R * a.inv_tau : K));
+            if (!(oe == 0.0)) B -= oe * (mkk - (Sk == 0.0 ? at_tau(a, R) : K));
 #pragma unroll
             for (int o = 4; o; o >>= 1) B += __shfl_xor_sync(0xffffffffu, B, o);
         } else {
@@ -428,7 +434,7 @@ __global__ void __launch_bounds__(NT, (PER_THREAD > 1 ? 1024 : MODE == LOSS ? 15
         const bool no_rest = St == 0.0, no_list = Sk == 0.0;
         // Everything relative to A.  The factor that brings S_t there is one of fp32 (where it cannot leave its range): L and L_t share it, so its error
         // enters the loss like S_t's own.
-        const double y = (double)R * a.inv_tau, A = no_list ? y : K;
+        const double y = at_tau(a, R), A = no_list ? y : K;
         const double far = (y - A) * 1.4426950408889634;
         double Sr = St;                             // S_t relative to A
         if (!no_rest && !no_list) Sr = fabs(far) < 120.0 ? St * (double)ex2((float)far) : St * exp(fmin(y - A, 700.0));

@@ -797,3 +797,49 @@ def test_distill_nan_in_list_whatever_its_bits(dtype, rows, vocab, bits):
     val[:, 1] = -INF
     _, grad = _check_distill(z, idx, val, None, None, 1.0, 'without')
     assert grad[0].isnan().all() and torch.isfinite(grad[1:]).all()
+
+
+# ------------------------------------------------------------------------------------------------ large logits and lowest masks at other temperatures
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('rows,vocab', [(2, 40001), (60, 700), (500, 3001)])
+@pytest.mark.parametrize('tau', [0.7, 0.3, 1.3, 3.0])
+@pytest.mark.parametrize('kind', ['lowest_list', 'lowest_logits', 'lowest_rows', 'lowest_list_and_logits', 'huge_list', 'huge_logits', 'huge_both', 'huge_below', 'large'])
+def test_distill_far_from_zero_at_other_temperatures(dtype, rows, vocab, tau, kind):
+    """Lowest values divided by a temperature below 1 are beyond fp32, and quotients of 1e16 are further from their nearest float than any exponential reaches.  The plain form is the same
+    as elsewhere; equal logits are equal after the division, others of that size are apart by more than an exponential sees."""
+    g = _gen(rows + vocab)
+    k, low = 37, torch.finfo(dtype).min
+    z = _normal(g, rows, vocab, scale=3.0)
+    idx = torch.stack([torch.randperm(vocab, generator=g, device='cuda')[:k] for _ in range(rows)]).int()
+    val, rest = _normal(g, rows, k), _normal(g, rows)
+    if kind in ('lowest_list', 'lowest_list_and_logits'):
+        val[:], rest[:] = low, -INF
+    if kind in ('lowest_logits', 'lowest_list_and_logits'):
+        z[:] = low
+    if kind == 'lowest_rows':                            # every other row masked, and so is the teacher's
+        z[::2] = low
+        val[::2], rest[::2] = low, -INF
+    if kind in ('huge_list', 'huge_both'):               # two entries share the teacher's mass
+        val[:] = 1.1e16
+        val[:, 2:] = -1.1e16
+        rest[:] = -INF
+    if kind in ('huge_logits', 'huge_both'):
+        z[:] = -1.3e16
+        z.scatter_(1, idx[:, :3].long(), 1.3e16)
+        val[:, 3:], rest[:] = -1.1e16, -INF
+    if kind == 'huge_below':                             # all of the list and the rest at one height far below zero
+        z[:], val[:], rest[:] = -7.7e15, -7.7e15, -INF
+    if kind == 'large':
+        z, val, rest = z * 1e3, val * 1e3, rest * 1e3
+    from ista_daslab_optimizers_b200 import distill_loss, distill_step
+    z, val = z.to(dtype), val.to(dtype)
+    w_loss, w_grad, size = D.distill(z, idx, val, rest, None, tau)
+    loss, grad = distill_step(z, idx, val, rest, None, tau)
+    leaf = z.clone().requires_grad_()
+    loss2 = distill_loss(leaf, idx, val, rest, None, tau)
+    grad2, = torch.autograd.grad(loss2.sum(), leaf)
+    for l, g, what in ((loss, grad, 'step '), (loss2.detach(), grad2, 'loss ')):
+        D.assert_near(l, w_loss, D.sum_error(vocab) + 2 * D.U * w_loss.abs(), what + kind)
+        # as for temperature 1, but an exponential below 2^-126 is 0 before it is multiplied by 1 / tau: off by up to 2^-126 / tau, where tau is below 1 more than 2^-126
+        D.assert_near(g, w_grad, (D.sum_error(vocab) + 72 * D.U) * size + (D.half_step(dtype) * 1.001) * w_grad.abs() + 2.0 ** -126 / min(tau, 1.0), what + kind)
