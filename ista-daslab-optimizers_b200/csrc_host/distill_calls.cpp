@@ -8,6 +8,7 @@
 #include <Python.h>
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -90,7 +91,9 @@ bool tensor(PyObject* o, at::Tensor* out, bool optional = false) {
     *out = THPVariable_Unpack(o);
     return true;
 }
-bool wants_gradient(const at::Tensor& t) { return t.defined() && t.requires_grad() && c10::GradMode::is_enabled(); }
+// A tangent of forward-mode differentiation, which none of the operators carries on.
+bool has_tangent(const at::Tensor& t) { return t.defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(/*level=*/0).defined(); }
+bool wants_gradient(const at::Tensor& t) { return t.defined() && ((t.requires_grad() && c10::GradMode::is_enabled()) || has_tangent(t)); }
 
 // A tensor of the caller's that the library has written to: autograd has to know, where it keeps it (or what shares its memory) for a backward pass.
 void written(const at::Tensor& t, PyObject* given) {
@@ -293,7 +296,7 @@ struct DistillLoss : torch::autograd::Function<DistillLoss> {
 // distill_loss(logits, indices, values, rest or None, weights or None, temperature)
 PyObject* distill_loss(PyObject*, PyObject* const* args, Py_ssize_t n) try {
     Lists l;
-    EXPECT(n == 6 && PyFloat_Check(args[5]) && l.of(args));
+    EXPECT(n == 6 && PyFloat_Check(args[5]) && l.of(args) && !has_tangent(l.logits));
     const double temperature = PyFloat_AS_DOUBLE(args[5]);
     // (what the library refuses is found out here, without an exception)
     EXPECT(l.k >= 1 && l.k <= MAB_MAX_LIST && l.vocab >= 1 && l.vocab <= MAB_MAX_VOCAB && temperature > 1e-6 && temperature < 1e6);
@@ -311,7 +314,7 @@ PyObject* distill_loss(PyObject*, PyObject* const* args, Py_ssize_t n) try {
 PyObject* distill_step(PyObject*, PyObject* const* args, Py_ssize_t n) try {
     Lists l;
     at::Tensor grad;
-    EXPECT(n == 7 && PyFloat_Check(args[5]) && l.of(args) && tensor(args[6], &grad, true));
+    EXPECT(n == 7 && PyFloat_Check(args[5]) && l.of(args) && tensor(args[6], &grad, true) && !has_tangent(l.logits) && !has_tangent(grad));
     const Target on(l.logits);
     if (!grad.defined()) grad = fresh({l.rows, l.vocab}, l.logits.scalar_type(), l.logits);
     Rows g;

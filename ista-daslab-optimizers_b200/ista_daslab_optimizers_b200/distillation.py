@@ -21,6 +21,7 @@ from __future__ import annotations
 import operator
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as N
 
@@ -56,7 +57,14 @@ def _same_device(device, **tensors):
             raise N.NativeError(f'{what} is on {t.device}, not on {device}')
 
 
+def _no_tangent_for(call, **tensors):
+    for what, t in tensors.items():
+        if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            raise N.NativeError(f'{call} has no forward-mode derivative: the tangent of {what} would be lost')
+
+
 def _no_grad_for(call, **tensors):
+    _no_tangent_for(call, **tensors)
     for what, t in tensors.items():
         if t is not None and t.requires_grad and torch.is_grad_enabled():
             raise N.NativeError(f'{call} has no gradient for {what}: what belongs to a frozen teacher is handed over detached, or under torch.no_grad()')
@@ -144,6 +152,7 @@ def _explain_topk(logits, k):
 
 def _explain_lists(what, logits, indices, values, rest, weights, temperature):
     _no_grad_for(what, values=values, rest=rest, weights=weights)
+    _no_tangent_for(what, logits=logits)
     _rows(logits, 'logits')
     rows, vocab = logits.shape
     if indices.dim() != 2 or indices.shape[0] != rows or values.shape != indices.shape:
@@ -172,7 +181,8 @@ def distill_loss(logits, indices, values, rest=None, weights=None, temperature=1
     weights         float32 [rows] or None: a row with weight 0 is not read, whatever it holds, and has loss and gradient 0.  (Multiply by
                     temperature ** 2 here for gradients that do not shrink with the temperature.)
 
-    The gradient comes from a second pass over the logits; `distill_step` gives both in one call.  Differentiable once."""
+    The gradient comes from a second pass over the logits; `distill_step` gives both in one call.  Differentiable once, backward only (a tangent of
+    forward-mode differentiation is refused)."""
     temperature = float(temperature)
     result = (_native_calls or _calls()).distill_loss(logits, indices, values, rest, weights, temperature)
     return result if result is not None else _fail(result, 'distill_loss', _explain_lists, 'distill_loss', logits, indices, values, rest, weights, temperature)
@@ -189,6 +199,7 @@ def distill_step(logits, indices, values, rest=None, weights=None, temperature=1
 
 def _explain_step(logits, indices, values, rest, weights, temperature, grad):
     _explain_lists('distill_step', logits, indices, values, rest, weights, temperature)
+    _no_tangent_for('distill_step', grad=grad)
     if grad is not None:
         if grad.shape != logits.shape or grad.dtype != logits.dtype or grad.requires_grad:
             raise N.NativeError(f'grad must be like the logits, {tuple(logits.shape)} of {logits.dtype}, and require no gradient itself')

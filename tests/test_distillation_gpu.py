@@ -843,3 +843,46 @@ def test_distill_far_from_zero_at_other_temperatures(dtype, rows, vocab, tau, ki
         D.assert_near(l, w_loss, D.sum_error(vocab) + 2 * D.U * w_loss.abs(), what + kind)
         # as for temperature 1, but an exponential below 2^-126 is 0 before it is multiplied by 1 / tau: off by up to 2^-126 / tau, where tau is below 1 more than 2^-126
         D.assert_near(g, w_grad, (D.sum_error(vocab) + 72 * D.U) * size + (D.half_step(dtype) * 1.001) * w_grad.abs() + 2.0 ** -126 / min(tau, 1.0), what + kind)
+
+
+# ------------------------------------------------------------------------------------------------ forward-mode differentiation
+
+@pytest.mark.parametrize('which', ['quantize x', 'matmul a_scales', 'matmul b_scales', 'matmul bias', 'topk logits', 'loss logits', 'loss leaf', 'loss values', 'loss rest', 'loss weights',
+                                   'step logits', 'step values', 'step weights'])
+def test_tangents_are_refused_not_lost(which):
+    import ista_daslab_optimizers_b200 as P
+    from ista_daslab_optimizers_b200 import _native as N
+    from torch.autograd import forward_ad
+    call, name = which.split()
+    g = _gen(51)
+    t = dict(x=_normal(g, 6, 64), a_scales=torch.ones(6, device='cuda'), b_scales=torch.ones(6, device='cuda'), bias=torch.ones(6, device='cuda'), logits=_normal(g, 6, 64),
+             values=_normal(g, 6, 4), rest=_normal(g, 6), weights=torch.ones(6, device='cuda'))
+    idx, codes = torch.zeros(6, 4, dtype=torch.int32, device='cuda'), torch.zeros(6, 64, dtype=torch.int8, device='cuda')
+    calls = dict(quantize=lambda: P.quantize_rows(t['x']), matmul=lambda: P.int8_matmul(codes, codes, t['a_scales'], t['b_scales'], t['bias']),
+                 topk=lambda: P.topk_logits(t['logits'], 3), loss=lambda: P.distill_loss(t['logits'], idx, t['values'], t['rest'], t['weights']),
+                 step=lambda: P.distill_step(t['logits'], idx, t['values'], t['rest'], t['weights']))
+    calls[call]()
+    if name == 'leaf':
+        name = 'logits'
+        t['logits'].requires_grad_()
+    with forward_ad.dual_level():
+        plain = t[name]
+        t[name] = forward_ad.make_dual(plain, torch.ones_like(plain))
+        before = N.kernel_launch_count()
+        for context in (torch.enable_grad(), torch.no_grad()):
+            with context, pytest.raises(N.NativeError, match='no forward-mode derivative'):
+                calls[call]()
+        assert N.kernel_launch_count() == before
+        t[name] = plain
+        calls[call]()
+    calls[call]()
+
+
+def test_gradients_that_a_function_transform_asks_for_are_not_lost():
+    """torch.func's tensors have no memory of their own: the operators refuse them rather than compute beside the transform."""
+    from ista_daslab_optimizers_b200 import distill_loss, topk_logits
+    z, idx, val, rest, _ = _problem(3, 500, 4, F32, F32, 1.0, True, False, False)
+    for call in (lambda: torch.func.grad(lambda y: distill_loss(y, idx, val, rest).sum())(z), lambda: torch.vmap(lambda y: topk_logits(y[None], 3)[0])(z),
+                 lambda: torch.func.jvp(lambda y: distill_loss(y, idx, val, rest), (z,), (z,))):
+        with pytest.raises(RuntimeError):
+            call()
