@@ -138,7 +138,8 @@ int mab_sparse_rows_combine(int64_t d, int64_t rows, int64_t k, int64_t d_block_
 
 /* ---- distillation: a frozen teacher in 8 bits, its top logits, the student's loss ---------------------------
  * No counterpart in the reference.  Rows lie `pitch` elements apart (at least their length) and may start anywhere their
- * element type allows; they are not read or written beyond their length. */
+ * element type allows; they are not read or written beyond their length.  Where a bounded wait inside a kernel runs out, what it should have
+ * written is NaN and mab_device_error() reads 1. */
 
 /* scales[r] = max |x[r, :]| / 127 (0 where that lies below 2^-126), codes[r, c] = the integer nearest x[r, c] / scales[r] (half to
  * even, the exact quotient decides), 0 where the scale is 0.  A row with a NaN or an infinity: scale NaN, codes 0.  The operands of
@@ -152,6 +153,12 @@ int mab_quantize_rows(int64_t rows, int64_t cols, const void* x, int x_dtype, in
 int mab_int8_matmul(int64_t m, int64_t n, int64_t k, const int8_t* a, int64_t a_pitch, const int8_t* b, int64_t b_pitch,
                     const float* a_scales, const float* b_scales, const float* bias, void* out, int out_dtype, int64_t out_pitch,
                     void* stream);
+
+/* The same call without any copy of the operands, as if every wait for one had run out: every element of out is NaN (from five tokens on; fewer wait for
+ * nothing) and mab_device_error() reads 1 afterwards.  Nothing faults; it exists so that the give-up path can be tested. */
+int mab_int8_matmul_selftest(int64_t m, int64_t n, int64_t k, const int8_t* a, int64_t a_pitch, const int8_t* b, int64_t b_pitch,
+                             const float* a_scales, const float* b_scales, const float* bias, void* out, int out_dtype, int64_t out_pitch,
+                             void* stream);
 
 /* Per row the k largest logits in descending order (ties: the lower index first; -0 equals +0; NaN below -inf) into values [rows, k]
  * (the logits' type, unchanged) and indices [rows, k], and rest[r] = log sum exp(logit / temperature) over all others (-inf where

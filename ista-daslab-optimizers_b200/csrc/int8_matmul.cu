@@ -30,7 +30,9 @@ struct Args {
     void* out;
     int m, n, k;
     int token_tiles, split, stages, height;        // tiles of `height` channels (a multiple of 8, at most 128)
+    int give_up;                                   // nothing is copied, as if every wait for it had run out (the selftest)
 };
+constexpr uint32_t NOT_A_NUMBER = 0x7FC00000u;     // the scale of the channels of a tile whose products did not come
 
 __device__ __forceinline__ float scaled(int sum, float token, float channel, float bias) { return fmaf((float)sum * token, channel, bias); }
 
@@ -51,7 +53,7 @@ __global__ void __launch_bounds__(THREADS) int8_matmul_kernel(const __grid_const
     const int warp = warp_id(), lane = lane_id(), t = threadIdx.x;
     const int rank = g.split > 1 ? (int)(blockIdx.x % g.split) : 0;
     const int tile = blockIdx.x / g.split, token0 = tile % g.token_tiles * BN, channel0 = tile / g.token_tiles * g.height;
-    const int steps = (g.k + BK - 1) / BK, k0 = (int)((int64_t)steps * rank / g.split), k1 = (int)((int64_t)steps * (rank + 1) / g.split);
+    const int steps = (g.k + BK - 1) / BK, k0 = (int)((int64_t)steps * rank / g.split), k1 = g.give_up ? k0 : (int)((int64_t)steps * (rank + 1) / g.split);
     const int stages = g.stages;
     auto load = [&](int i, int s) {                 // step i into stage s
         unsigned char* stage = ring + s * STAGE;
@@ -63,7 +65,7 @@ __global__ void __launch_bounds__(THREADS) int8_matmul_kernel(const __grid_const
         for (int i = 0; i < stages; ++i) { mbar_init_unfenced(&full[i], 1); mbar_init_unfenced(&empty[i], 1); }
         mbar_init_unfenced(&done, 1);
         mbar_init_fence();
-        s_lost = 0;
+        s_lost = g.give_up;
     }
     if (warp == 1) tmem_alloc(&s_tmem, COLUMNS);
     wait_for_kernel_before();
@@ -107,8 +109,12 @@ __global__ void __launch_bounds__(THREADS) int8_matmul_kernel(const __grid_const
                 }
                 __syncwarp();
             }
-            for (int n = 0; i < k1 && n < stages; ++i, ++n, next()) mbar_wait(&full[s], parity, 1 << 12);      // lost: copies still on their way must not outlive the CTA
-            if (issuing) mma_commit(&done);
+            const bool issued = i > k0;
+            for (int n = 0; i < k1 && n < stages; ++i, ++n, next()) mbar_wait(&full[s], parity);      // lost: copies still on their way must not outlive the CTA
+            if (issuing) {
+                if (issued) mma_commit(&done);
+                else mbar_arrive(&done);
+            }
         }
     }
     __syncwarp();
@@ -120,10 +126,10 @@ __global__ void __launch_bounds__(THREADS) int8_matmul_kernel(const __grid_const
     T* out = reinterpret_cast<T*>(g.out);
 
     if (g.split == 1) {
-        if (warp >= 2 && !lost) {
+        if (warp >= 2) {
             const int quarter = warp & 3, at = 32 * quarter + lane, channel = channel0 + at;
             const bool there = at < g.height && channel < g.n;
-            const float cs = s_channel[at].x, bias = s_channel[at].y;
+            const float cs = lost ? __uint_as_float(NOT_A_NUMBER) : s_channel[at].x, bias = s_channel[at].y;
             for (int c = 0; c < BN && token0 + c < g.m; c += 16) {
                 int r[16];
                 tmem_load(acc + ((uint32_t)(32 * quarter) << 16) + c, r);
@@ -151,21 +157,25 @@ __global__ void __launch_bounds__(THREADS) int8_matmul_kernel(const __grid_const
         const int there = min(BN, g.m - token0), c0 = there * rank / g.split, c1 = there * (rank + 1) / g.split;      // this CTA's columns
         bool any = false;
         for (int s = 0; s < g.split; ++s) any |= cluster_load_u32(&s_lost, s) != 0;
-        if (!any)
-            for (int i = c0 * (BM / 4) + t; i < c1 * (BM / 4); i += THREADS) {
-                const int column = i / (BM / 4), at = i % (BM / 4) * 4, channel = channel0 + at;
-                int4 p[8], sum = make_int4(0, 0, 0, 0);
+        if (any) {
+            __syncthreads();
+            if (t < BM) s_channel[t].x = __uint_as_float(NOT_A_NUMBER);
+            __syncthreads();
+        }
+        for (int i = c0 * (BM / 4) + t; i < c1 * (BM / 4); i += THREADS) {
+            const int column = i / (BM / 4), at = i % (BM / 4) * 4, channel = channel0 + at;
+            int4 p[8], sum = make_int4(0, 0, 0, 0);
 #pragma unroll
-                for (int s = 0; s < 8; ++s) if (s < g.split) p[s] = cluster_load_int4(&part[4 * i], s);
+            for (int s = 0; s < 8; ++s) if (s < g.split) p[s] = cluster_load_int4(&part[4 * i], s);
 #pragma unroll
-                for (int s = 0; s < 8; ++s) if (s < g.split) { sum.x += p[s].x; sum.y += p[s].y; sum.z += p[s].z; sum.w += p[s].w; }
-                const int sums[4] = {sum.x, sum.y, sum.z, sum.w};
-                T* o = out + (int64_t)(token0 + column) * g.out_pitch + channel;
+            for (int s = 0; s < 8; ++s) if (s < g.split) { sum.x += p[s].x; sum.y += p[s].y; sum.z += p[s].z; sum.w += p[s].w; }
+            const int sums[4] = {sum.x, sum.y, sum.z, sum.w};
+            T* o = out + (int64_t)(token0 + column) * g.out_pitch + channel;
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (at + j < g.height && channel + j < g.n)
-                        Elem<T>::store(o, j, scaled(sums[j], s_token[column], s_channel[at + j].x, s_channel[at + j].y));
-            }
+            for (int j = 0; j < 4; ++j)
+                if (at + j < g.height && channel + j < g.n)
+                    Elem<T>::store(o, j, scaled(sums[j], s_token[column], s_channel[at + j].x, s_channel[at + j].y));
+        }
         cluster_arrive_wait();
     }
     tmem_fence_before();
@@ -173,6 +183,8 @@ __global__ void __launch_bounds__(THREADS) int8_matmul_kernel(const __grid_const
     if (warp == 1) { tmem_fence_after(); tmem_free(acc, COLUMNS); }
 }
 
+// A wait that runs out (a device in trouble) sets the library's flag, and the tiles concerned are NaN.
+//
 // The form for many tokens: two CTAs share a tile of 256 channels and up to 256 tokens, so a stage of the ring is 16 KB of weights and up to 16 KB of tokens
 // a CTA for twice the products, and they stay on their SMs: while other warps take the sums of one tile out of tensor memory, the next tile's go into its other
 // half.  Tiles of the same channels follow one another: the weights come from HBM once.
@@ -185,7 +197,7 @@ __global__ void __launch_bounds__(PAIR_THREADS) int8_matmul_pair_kernel(const __
                                                                         const __grid_constant__ Args g, int tokens, int tiles) {
     extern __shared__ unsigned char dyn[];
     unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~(uintptr_t)1023);
-    __shared__ uint64_t full[PAIR_STAGES], empty[PAIR_STAGES], ready[2], taken[2];
+    __shared__ uint64_t full[PAIR_STAGES], empty[PAIR_STAGES], ready[2], taken[2], drained;
     __shared__ uint32_t s_tmem;
     __shared__ int s_lost;
     const int warp = warp_id(), lane = lane_id(), t = threadIdx.x, rank = (int)(blockIdx.x & 1), pair = (int)(blockIdx.x >> 1), pairs = (int)(gridDim.x >> 1);
@@ -193,6 +205,7 @@ __global__ void __launch_bounds__(PAIR_THREADS) int8_matmul_pair_kernel(const __
     if (t == 0) {
         for (int i = 0; i < PAIR_STAGES; ++i) { mbar_init_unfenced(&full[i], 1); mbar_init_unfenced(&empty[i], 1); }
         for (int i = 0; i < 2; ++i) { mbar_init_unfenced(&ready[i], 1); mbar_init_unfenced(&taken[i], 2 * PAIR_WARPS); }
+        mbar_init_unfenced(&drained, 1);
         mbar_init_fence();
         s_lost = 0;
     }
@@ -209,7 +222,7 @@ __global__ void __launch_bounds__(PAIR_THREADS) int8_matmul_pair_kernel(const __
         int s = 0;
         uint32_t parity = 0;
         auto next = [&] { if (++s == PAIR_STAGES) { s = 0; parity ^= 1; } };
-        bool ok = true;
+        bool ok = !g.give_up;
         if (warp == 0) {
             const uint32_t full0 = cluster_addr(&full[0], 0), bytes = (uint32_t)(2 * BM + tokens) * BK;       // both CTAs' bytes
             int filled = 0;
@@ -234,11 +247,13 @@ __global__ void __launch_bounds__(PAIR_THREADS) int8_matmul_pair_kernel(const __
         } else if (rank == 0) {
             const uint32_t instruction = i8_instruction(2 * BM, tokens), ring0 = smem_addr(ring);
             int done = 0;                           // tiles
+            const int64_t total = ok ? (int64_t)((tiles - pair + pairs - 1) / pairs) * steps : 0;       // stages' fillings
+            int64_t left = total;                   // ... that have not been waited for
             for (int tile = pair; ok && tile < tiles; tile += pairs, ++done) {
                 const uint32_t d = acc + (done & 1) * 256;
                 if (done >= 2 && !mbar_wait(&taken[done & 1], (done / 2 - 1) & 1, PAIR_LIMIT)) { ok = false; break; }
                 tmem_fence_after();
-                for (int i = 0; i < steps; ++i, next()) {
+                for (int i = 0; i < steps; ++i, --left, next()) {
                     if (!mbar_wait(&full[s], parity, PAIR_LIMIT)) { ok = false; break; }
                     tmem_fence_after();
                     const uint32_t stage = ring0 + s * PAIR_STAGE;
@@ -253,24 +268,38 @@ __global__ void __launch_bounds__(PAIR_THREADS) int8_matmul_pair_kernel(const __
                 if (ok && issuing) mma_commit_pair(&ready[done & 1]);
                 __syncwarp();
             }
-            if (!ok)                                // copies that may still be on their way must not outlive the CTAs
-                for (int i = 0; i < PAIR_STAGES; ++i, next()) mbar_wait(&full[s], parity, 1 << 10);
+            if (!ok) {                              // copies and products that may still be on their way must not outlive the CTAs
+                const bool issued = left < total;
+                for (int i = 0; i < PAIR_STAGES && i < left; ++i, next()) mbar_wait(&full[s], parity, PAIR_LIMIT);
+                if (issued) {
+                    if (issuing) mma_commit_pair(&drained, 1);
+                    __syncwarp();
+                    mbar_wait(&drained, 0, PAIR_LIMIT);
+                }
+            }
         }
         if (!ok) s_lost = 1;
     } else {
         // 32 channels and every other group of 32 tokens a warp
         const int quarter = warp & 3, slice = (warp - 2) >> 2, groups = tokens / 32;
         int done = 0;
+        bool lost = g.give_up;                      // (from there on every tile of the pair is NaN)
         for (int tile = pair; tile < tiles; tile += pairs, ++done) {
             const int token0 = tile % g.token_tiles * tokens, channel = tile / g.token_tiles * 2 * BM + rank * BM + 32 * quarter + lane;
             const bool there = channel < g.n;
-            const float cs = there ? g.b_scales[channel] : 0.0f, bias = g.bias && there ? g.bias[channel] : 0.0f;
+            float cs = there ? g.b_scales[channel] : 0.0f;
+            const float bias = g.bias && there ? g.bias[channel] : 0.0f;
             auto scale_of = [&](int group) {          // of the group's tokens, one a lane
                 const int token = token0 + 32 * group + lane;
                 return group < groups && token < g.m ? g.a_scales[token] : 0.0f;
             };
             float next_scale = scale_of(slice);
-            if (!mbar_wait(&ready[done & 1], done / 2 & 1, PAIR_LIMIT)) { if (lane == 0) atomicExch(&s_lost, 1); break; }
+            if (lost || !mbar_wait(&ready[done & 1], done / 2 & 1, PAIR_LIMIT)) {
+                lost = true;
+                s_lost = 1;
+                cs = __uint_as_float(NOT_A_NUMBER);
+            }
+            __syncwarp();
             tmem_fence_after();
             const uint32_t from = acc + ((uint32_t)(32 * quarter) << 16) + (done & 1) * 256;
             if (slice >= groups && lane == 0) mbar_arrive_cluster(cluster_addr(&taken[done & 1], 0));
@@ -459,7 +488,7 @@ int copy_timeout_int8_matmul(int* out, bool clear) {
 
 using namespace mab;
 
-extern "C" int mab_int8_matmul(int64_t m, int64_t n, int64_t k, const int8_t* a, int64_t a_pitch, const int8_t* b, int64_t b_pitch,
+static int int8_matmul(int give_up, int64_t m, int64_t n, int64_t k, const int8_t* a, int64_t a_pitch, const int8_t* b, int64_t b_pitch,
                                const float* a_scales, const float* b_scales, const float* bias, void* out, int out_dtype, int64_t out_pitch,
                                void* stream) {
     MAB_REQUIRE(m >= 0 && n >= 0 && k >= 1, MAB_ERR_BAD_ARG, "mab_int8_matmul: m=%lld, n=%lld, k=%lld", (long long)m, (long long)n, (long long)k);
@@ -474,6 +503,18 @@ extern "C" int mab_int8_matmul(int64_t m, int64_t n, int64_t k, const int8_t* a,
                 "mab_int8_matmul: codes have to start on 16 bytes, their rows a multiple of 16 apart (%lld, %lld)", (long long)a_pitch, (long long)b_pitch);
     MAB_REQUIRE(aligned_to(a_scales, 4) && aligned_to(b_scales, 4) && aligned_to(bias, 4) && aligned_to(out, out_dtype == MAB_F32 ? 4 : 2),
                 MAB_ERR_BAD_ARG, "mab_int8_matmul: misaligned buffer");
-    int8mm::Args g = {a, b, a_pitch, b_pitch, out_pitch, a_scales, b_scales, bias, out, (int)m, (int)n, (int)k, 1, 1, 1, int8mm::BM};
+    int8mm::Args g = {a, b, a_pitch, b_pitch, out_pitch, a_scales, b_scales, bias, out, (int)m, (int)n, (int)k, 1, 1, 1, int8mm::BM, give_up};
     return out_dtype == MAB_F32 ? int8mm::launch<float>(g, (cudaStream_t)stream) : int8mm::launch<uint16_t>(g, (cudaStream_t)stream);
+}
+
+extern "C" int mab_int8_matmul(int64_t m, int64_t n, int64_t k, const int8_t* a, int64_t a_pitch, const int8_t* b, int64_t b_pitch,
+                               const float* a_scales, const float* b_scales, const float* bias, void* out, int out_dtype, int64_t out_pitch,
+                               void* stream) {
+    return int8_matmul(0, m, n, k, a, a_pitch, b, b_pitch, a_scales, b_scales, bias, out, out_dtype, out_pitch, stream);
+}
+
+extern "C" int mab_int8_matmul_selftest(int64_t m, int64_t n, int64_t k, const int8_t* a, int64_t a_pitch, const int8_t* b,
+                                        int64_t b_pitch, const float* a_scales, const float* b_scales, const float* bias, void* out, int out_dtype,
+                                        int64_t out_pitch, void* stream) {
+    return int8_matmul(1, m, n, k, a, a_pitch, b, b_pitch, a_scales, b_scales, bias, out, out_dtype, out_pitch, stream);
 }

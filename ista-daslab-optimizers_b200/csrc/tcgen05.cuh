@@ -82,10 +82,10 @@ __device__ __forceinline__ void mma_i8_pair(uint32_t d, uint64_t a, uint64_t b, 
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
                  ::"r"(d), "l"(a), "l"(b), "r"(instruction), "r"((uint32_t)accumulate) : "memory");
 }
-// An arrival at the barriers at this place of both CTAs.
-__device__ __forceinline__ void mma_commit_pair(uint64_t* bar) {
+// An arrival at the barriers at this place of the CTAs whose bits are set.
+__device__ __forceinline__ void mma_commit_pair(uint64_t* bar, uint16_t ctas = 3) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-                 ::"r"(smem_addr(bar)), "h"((uint16_t)3) : "memory");
+                 ::"r"(smem_addr(bar)), "h"(ctas) : "memory");
 }
 // A box into this CTA's shared memory that reports to the barrier at cluster address `bar`, which can be the other CTA's.
 __device__ __forceinline__ void tile_g2s_pair(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {

@@ -81,6 +81,8 @@ SIGNATURES = {
     'mab_quantize_rows': (c_int, [c_int64, c_int64, c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p, c_void_p]),
     'mab_int8_matmul': (c_int, [c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
                                 c_int64, c_void_p]),
+    'mab_int8_matmul_selftest': (c_int, [c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
+                                         c_int64, c_void_p]),
     'mab_topk_logits': (c_int, [c_int64, c_int64, c_int64, c_void_p, c_int, c_int64, c_double, c_void_p, c_void_p, c_void_p, c_void_p]),
     'mab_distill_loss': (c_int, [c_int64, c_int64, c_int64, c_void_p, c_int, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_double,
                                  c_void_p, c_void_p, c_void_p, c_void_p]),

@@ -886,3 +886,28 @@ def test_gradients_that_a_function_transform_asks_for_are_not_lost():
                  lambda: torch.func.jvp(lambda y: distill_loss(y, idx, val, rest), (z,), (z,))):
         with pytest.raises(RuntimeError):
             call()
+
+
+# ------------------------------------------------------------------------------------------------ waits that run out
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('m,n,k', [(5, 300, 100), (41, 4096, 4096), (64, 200, 8192), (128, 400, 6400), (65, 300, 640), (300, 5000, 64), (777, 3000, 767), (1025, 9729, 1024)])
+def test_product_whose_copies_do_not_come(m, n, k, dtype):
+    """As if every wait had run out: no element keeps what its memory held before, the flag is set, and the next product is right.  Nothing faults: no copy is issued."""
+    from ista_daslab_optimizers_b200 import int8_matmul, _native as N
+    g = _gen(m + n)
+    a, b = _codes(g, m, k), _codes(g, n, k)
+    sa, sb = torch.rand(m, generator=g, device='cuda'), torch.rand(n, generator=g, device='cuda')
+    buf = torch.full((m + 2, n + 3), 7.0, dtype=dtype, device='cuda')
+    out = buf[1:m + 1, 1:n + 1]
+    assert N.device_error() == 0
+    N.check(N.load().mab_int8_matmul_selftest(m, n, k, a.data_ptr(), a.stride(0), b.data_ptr(), b.stride(0), sa.data_ptr(), sb.data_ptr(), None, out.data_ptr(),
+                                              N.MAB_F32 if dtype == F32 else N.MAB_BF16, out.stride(0), torch.cuda.current_stream().cuda_stream), 'selftest')
+    assert N.device_error() == 1
+    assert out.isnan().all()
+    assert (buf[0] == 7).all() and (buf[m + 1] == 7).all() and (buf[:, 0] == 7).all() and (buf[:, n + 1:] == 7).all()
+    N.device_error_clear()
+    int8_matmul(a, b, sa, sb, out=out)
+    want, tol = D.matmul(a, b, sa, sb, None)
+    D.assert_near(out, want, tol + (0 if dtype == F32 else D.half_step(dtype) * want.abs()), 'product')
+    assert N.device_error() == 0
