@@ -138,7 +138,8 @@ int mab_sparse_rows_combine(int64_t d, int64_t rows, int64_t k, int64_t d_block_
 
 /* ---- distillation: a frozen teacher in 8 bits, its top logits, the student's loss ---------------------------
  * No counterpart in the reference.  Rows lie `pitch` elements apart (at least their length) and may start anywhere their
- * element type allows; they are not read or written beyond their length.  Where a bounded wait inside a kernel runs out, what it should have
+ * element type allows; they are not read or written beyond their length.  What a call
+ * writes shares no byte with what it reads (but see grad) or with what else it writes.  Where a bounded wait inside a kernel runs out, what it should have
  * written is NaN and mab_device_error() reads 1. */
 
 /* scales[r] = max |x[r, :]| / 127 (0 where that lies below 2^-126), codes[r, c] = the integer nearest x[r, c] / scales[r] (half to

@@ -17,6 +17,7 @@
 // Bound by HBM and by the chain of phases around the passes (list, block and cluster sums, three logarithms: some 5 us a row, which the SM's other rows cover in part).
 // bf16, rows of 128256, k = 64 (us): loss of 1536 rows 75 (5.2 TB/s), its gradient 149 (6.2 TB/s), loss and gradient of 4096 rows in one call 443 (4.7 TB/s of the two passes
 // over HBM that it needs; what it holds and what L2 keeps leave 1.09 of their bytes; 569 before anything was held).
+#include <initializer_list>
 #include <type_traits>
 #include "rows.cuh"
 #include "async_copy.cuh"
@@ -602,6 +603,17 @@ static int check_grad(const char* who, int64_t rows, int64_t vocab, const void* 
     return MAB_OK;
 }
 
+// ... and one that lies over the lists or the rows' numbers, too.
+static int check_apart(const char* who, int64_t rows, int64_t vocab, int64_t k, int dtype, const void* grad, int64_t grad_pitch, const int32_t* indices,
+                       std::initializer_list<Span> others) {
+    const int64_t e = dtype == MAB_F32 ? 4 : 2;
+    const Span g = {grad, rows, vocab * e, grad_pitch * e};
+    bool ok = apart(g, vector_span(indices, rows * k * 4));
+    for (const Span& o : others) ok = ok && apart(g, o);
+    MAB_REQUIRE(ok, MAB_ERR_BAD_ARG, "%s: the gradient overlaps the lists or the rows' numbers", who);
+    return MAB_OK;
+}
+
 static Args args_of(int64_t vocab, int64_t k, const void* logits, int64_t pitch, const int32_t* indices, const void* values, int v_dtype,
                     const float* rest, const float* weights, double tau) {
     Args a = {};
@@ -645,6 +657,9 @@ extern "C" int mab_distill_grad(int64_t rows, int64_t vocab, int64_t k, const vo
     MAB_REQUIRE(grad_loss_stride >= 0, MAB_ERR_BAD_ARG, "mab_distill_grad: grad_loss_stride=%lld", (long long)grad_loss_stride);
     MAB_REQUIRE(aligned_to(stats, 8) && aligned_to(grad_loss, 4), MAB_ERR_BAD_ARG, "mab_distill_grad: misaligned buffer");
     if (int rc = distill::check_grad("mab_distill_grad", rows, vocab, logits, dtype, pitch, grad, grad_pitch)) return rc;
+    if (int rc = distill::check_apart("mab_distill_grad", rows, vocab, k, dtype, grad, grad_pitch, indices,
+                                      {vector_span(list_grad, rows * k * 4), vector_span(stats, rows * 8), vector_span(weights, rows * 4),
+                                       vector_span(grad_loss, ((rows - 1) * grad_loss_stride + 1) * 4)})) return rc;
     distill::Args a = distill::args_of(vocab, k, logits, pitch, indices, nullptr, MAB_F32, nullptr, weights, temperature);
     a.stats = reinterpret_cast<float2*>(const_cast<float*>(stats)); a.list_grad = const_cast<float*>(list_grad);
     a.grad_loss = grad_loss; a.grad_loss_stride = grad_loss_stride; a.grad = grad; a.grad_pitch = grad_pitch;
@@ -659,6 +674,9 @@ extern "C" int mab_distill_step(int64_t rows, int64_t vocab, int64_t k, const vo
     MAB_REQUIRE(loss && grad, MAB_ERR_BAD_ARG, "mab_distill_step: null pointer");
     MAB_REQUIRE(aligned_to(loss, 4), MAB_ERR_BAD_ARG, "mab_distill_step: misaligned buffer");
     if (int rc = distill::check_grad("mab_distill_step", rows, vocab, logits, dtype, pitch, grad, grad_pitch)) return rc;
+    if (int rc = distill::check_apart("mab_distill_step", rows, vocab, k, dtype, grad, grad_pitch, indices,
+                                      {vector_span(values, rows * k * (v_dtype == MAB_F32 ? 4 : 2)), vector_span(rest, rows * 4), vector_span(weights, rows * 4),
+                                       vector_span(loss, rows * 4)})) return rc;
     distill::Args a = distill::args_of(vocab, k, logits, pitch, indices, values, v_dtype, rest, weights, temperature);
     a.loss = loss; a.grad = grad; a.grad_pitch = grad_pitch;
     return dtype == MAB_F32 ? distill::launch<float, distill::STEP>(a, rows, (cudaStream_t)stream)

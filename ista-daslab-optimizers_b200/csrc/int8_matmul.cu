@@ -503,6 +503,10 @@ static int int8_matmul(int give_up, int64_t m, int64_t n, int64_t k, const int8_
                 "mab_int8_matmul: codes have to start on 16 bytes, their rows a multiple of 16 apart (%lld, %lld)", (long long)a_pitch, (long long)b_pitch);
     MAB_REQUIRE(aligned_to(a_scales, 4) && aligned_to(b_scales, 4) && aligned_to(bias, 4) && aligned_to(out, out_dtype == MAB_F32 ? 4 : 2),
                 MAB_ERR_BAD_ARG, "mab_int8_matmul: misaligned buffer");
+    const int64_t e = out_dtype == MAB_F32 ? 4 : 2;
+    const Span to = {out, m, n * e, out_pitch * e};
+    MAB_REQUIRE(apart(to, {a, m, k, a_pitch}) && apart(to, {b, n, k, b_pitch}) && apart(to, vector_span(a_scales, m * 4)) && apart(to, vector_span(b_scales, n * 4)) &&
+                    apart(to, vector_span(bias, n * 4)), MAB_ERR_BAD_ARG, "mab_int8_matmul: out overlaps an operand, scales or the bias");
     int8mm::Args g = {a, b, a_pitch, b_pitch, out_pitch, a_scales, b_scales, bias, out, (int)m, (int)n, (int)k, 1, 1, 1, int8mm::BM, give_up};
     return out_dtype == MAB_F32 ? int8mm::launch<float>(g, (cudaStream_t)stream) : int8mm::launch<uint16_t>(g, (cudaStream_t)stream);
 }

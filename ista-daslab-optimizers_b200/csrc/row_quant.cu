@@ -163,6 +163,9 @@ extern "C" int mab_quantize_rows(int64_t rows, int64_t cols, const void* x, int 
     MAB_REQUIRE(x_pitch >= cols && codes_pitch >= cols, MAB_ERR_BAD_ARG, "mab_quantize_rows: rows of %lld values lie %lld and %lld apart", (long long)cols,
                 (long long)x_pitch, (long long)codes_pitch);
     MAB_REQUIRE(aligned_to(x, x_dtype == MAB_F32 ? 4 : 2) && aligned_to(scales, 4), MAB_ERR_BAD_ARG, "mab_quantize_rows: misaligned buffer");
+    const int64_t e = x_dtype == MAB_F32 ? 4 : 2;
+    const Span in = {x, rows, cols * e, x_pitch * e}, out = {codes, rows, cols, codes_pitch}, out_scales = vector_span(scales, rows * 4);
+    MAB_REQUIRE(apart(in, out) && apart(in, out_scales) && apart(out, out_scales), MAB_ERR_BAD_ARG, "mab_quantize_rows: the codes or scales overlap one another or x");
     quant8::Args a = {x, x_pitch, codes_pitch, codes, scales, rows, (int)cols};
     return x_dtype == MAB_F32 ? quant8::launch<float>(a, (cudaStream_t)stream) : quant8::launch<uint16_t>(a, (cudaStream_t)stream);
 }

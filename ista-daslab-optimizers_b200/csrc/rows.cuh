@@ -177,6 +177,22 @@ __device__ __forceinline__ void kernel_before_is_done() {
     allow_next_kernel(ANY_GRID);
 }
 
+// Rows in memory, sizes in bytes: what a call writes has to lie apart from what it reads.  Rows of both may lie between one another (a record's fields), at one distance.
+struct Span {
+    const void* p;
+    int64_t rows, width, pitch;
+};
+static inline bool apart(const Span& a, const Span& b) {
+    if (a.p == nullptr || b.p == nullptr || a.rows == 0 || b.rows == 0) return true;
+    const uintptr_t a0 = reinterpret_cast<uintptr_t>(a.p), a1 = a0 + (a.rows - 1) * a.pitch + a.width;
+    const uintptr_t b0 = reinterpret_cast<uintptr_t>(b.p), b1 = b0 + (b.rows - 1) * b.pitch + b.width;
+    if (a1 <= b0 || b1 <= a0) return true;
+    if (a.pitch != b.pitch || a.rows == 1 || b.rows == 1) return false;
+    const int64_t ahead = ((int64_t)(b0 - a0) % a.pitch + a.pitch) % a.pitch;      // where b's rows begin, from the beginnings of a's
+    return ahead >= a.width && ahead + b.width <= a.pitch;
+}
+static inline Span vector_span(const void* p, int64_t bytes) { return {p, 1, bytes, bytes}; }
+
 // Launches `kernel` with clusters of `cluster` CTAs (1: without) and counts it.  (Above 48 KB with the kernel's own static memory, a few KB, the size has to be allowed.)
 template <typename... P, typename... A>
 static int launch_rows(void (*kernel)(P...), const char* what, int64_t ctas, int threads, size_t smem, int cluster, cudaStream_t s, A... args) {

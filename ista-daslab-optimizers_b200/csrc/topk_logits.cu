@@ -662,6 +662,10 @@ extern "C" int mab_topk_logits(int64_t rows, int64_t vocab, int64_t k, const voi
     MAB_REQUIRE(pitch >= vocab, MAB_ERR_BAD_ARG, "mab_topk_logits: rows of %lld logits lie %lld apart", (long long)vocab, (long long)pitch);
     const size_t e = dtype == MAB_F32 ? 4 : 2;
     MAB_REQUIRE(aligned_to(logits, e) && aligned_to(values, e) && aligned_to(indices, 4) && aligned_to(rest, 4), MAB_ERR_BAD_ARG, "mab_topk_logits: misaligned buffer");
+    const Span in = {logits, rows, (int64_t)(vocab * e), (int64_t)(pitch * e)};
+    const Span out[3] = {vector_span(values, rows * k * (int64_t)e), vector_span(indices, rows * k * 4), vector_span(rest, rows * 4)};
+    MAB_REQUIRE(apart(in, out[0]) && apart(in, out[1]) && apart(in, out[2]) && apart(out[0], out[1]) && apart(out[0], out[2]) && apart(out[1], out[2]), MAB_ERR_BAD_ARG,
+                "mab_topk_logits: the outputs overlap one another or the logits");
     toplogits::Args a = {};
     a.logits = logits; a.pitch = pitch; a.values = values; a.indices = indices; a.rest = rest; a.tau = temperature;
     a.scale = (float)(1.4426950408889634 / temperature); a.vocab = (int)vocab; a.k = (int)k;

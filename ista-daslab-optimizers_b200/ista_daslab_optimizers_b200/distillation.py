@@ -14,7 +14,8 @@ autograd, `distill_step` as one call).
 
 Every tensor is a CUDA tensor of one device; the work is enqueued on that device's current stream.  Matrices are two-dimensional, their rows
 contiguous; the rows themselves may lie any distance apart (a slice of columns, every second row).  What the kernels cannot take raises
-NativeError before anything is launched; there is no other implementation behind them.  A wait inside a kernel that runs out (a device in trouble)
+NativeError before anything is launched; there is no other implementation behind them.  Outputs that are given (`codes`, `scales`, `out`, `grad`) share no
+memory with inputs (but `grad` with the logits that it replaces).  A wait inside a kernel that runs out (a device in trouble)
 cannot raise where it happens: what the kernel should have written is NaN, and `_native.device_error()`, which waits for the device, returns 1.
 """
 from __future__ import annotations

@@ -110,3 +110,19 @@ def test_plain_form_of_the_loss_is_the_gradient_it_says():
     loss, grad, _ = D.distill(z.detach(), idx, val, rest, w, tau)
     assert abs(float(loss.sum() - total)) < 1e-12
     assert (grad - want).abs().max() < 1e-12
+
+
+@pytest.mark.parametrize('call,wrong', [
+    (quant, dict(c=P)), (quant, dict(c=P + 4 * 64 * 4 - 1)), (quant, dict(c=P - 255)), (quant, dict(c=P + 4096, s=P + 1020)), (quant, dict(c=P + 4096, s=P + 4096 + 252)),
+    (quant, dict(xp=128, c=P + 255, cp=512)), (quant, dict(xp=128, c=P + 449, cp=512)), (quant, dict(xp=128, c=P + 256, cp=500)),
+    (matmul, dict(a=P, b=P + 4096, sa=P + 8192, sb=P + 8256, out=P + 128)), (matmul, dict(a=P, b=P + 4096, sa=P + 8192, sb=P + 8256, out=P + 4096 - 4)),
+    (matmul, dict(a=P, b=P + 4096, sa=P + 8192, sb=P + 8256, out=P + 8192 + 12)), (matmul, dict(a=P, b=P + 4096, sa=P + 8192, sb=P + 8256, out=P + 8256 - 124)),
+    (matmul, dict(a=P, b=P + 4096, sa=P + 8192, sb=P + 8256, bias=P + 16384, out=P + 16384 + 28)),
+    (topk, dict(v=P + 1020, i=P + 8192, r=P + 12288)), (topk, dict(v=P + 4096, i=P + 4096 + 124, r=P + 12288)), (topk, dict(v=P + 4096, i=P + 8192, r=P + 8192 + 124)),
+    (topk, dict(v=P + 4096, i=P + 8192, r=P)),
+    (grad, dict(z=P, i=P + 4096 + 1020)), (grad, dict(lg=P + 4096 - 124)), (grad, dict(st=P + 4096)), (grad, dict(w=P + 4096 + 1020)), (grad, dict(up=P + 4096 - 48, stride=4)),
+    (step, dict(i=P + 4096 + 1020)), (step, dict(v=P + 4096 - 124)), (step, dict(v=P + 4096 - 60, vd=1)), (step, dict(r=P + 4096)), (step, dict(w=P + 4096 + 1020)), (step, dict(out=P + 4096))])
+def test_overlapping_memory_is_refused(lib, call, wrong):
+    """What a call writes lies over what it reads, or over what else it writes, by as little as a byte."""
+    assert call(lib, **wrong) == BAD
+    assert b'overlap' in lib.mab_last_error()

@@ -911,3 +911,39 @@ def test_product_whose_copies_do_not_come(m, n, k, dtype):
     want, tol = D.matmul(a, b, sa, sb, None)
     D.assert_near(out, want, tol + (0 if dtype == F32 else D.half_step(dtype) * want.abs()), 'product')
     assert N.device_error() == 0
+
+
+# ------------------------------------------------------------------------------------------------ memory that is shared
+
+def test_outputs_between_the_rows_of_inputs():
+    """Records that hold a row of the input and one of the output: no byte is shared, so they are taken.  An output over an input is not, whatever its type."""
+    import ista_daslab_optimizers_b200 as P
+    from ista_daslab_optimizers_b200 import _native as N
+    g = _gen(61)
+    rows, cols = 37, 256
+    record = torch.zeros(rows, cols * 4 + cols, dtype=torch.uint8, device='cuda')      # float32 row, then its codes
+    x = record.view(F32)[:, :cols]
+    x.copy_(_normal(g, rows, cols))
+    codes = record.view(torch.int8)[:, cols * 4:]
+    _, scales = P.quantize_rows(x, codes)
+    want, want_scales = D.quantize(x)
+    assert torch.equal(codes, want) and torch.equal(scales, want_scales)
+    b, sb = P.quantize_rows(_normal(g, 64, cols))
+    wide = torch.zeros(rows, cols + 64 * 4, dtype=torch.uint8, device='cuda')            # codes, then the product's row
+    a, out = wide.view(torch.int8)[:, :cols], wide.view(F32)[:, cols // 4:]
+    a.copy_(codes)
+    P.int8_matmul(a, b, scales, sb, out=out)
+    want, tol = D.matmul(codes, b, scales, sb, None)
+    D.assert_near(out, want, tol, 'product')
+    z, idx, val, rest, w = _problem(6, 64, 4, F32, F32, 1.0, True, True, False)
+    before = N.kernel_launch_count()
+    for call in (lambda: P.quantize_rows(x, x.view(torch.int8)[:, :cols]), lambda: P.quantize_rows(x, scales=record.view(F32).flatten()[:rows]),
+                 lambda: P.int8_matmul(a, b, scales, sb, out=wide.view(F32)[:, :64])):
+        with pytest.raises(N.NativeError, match='overlap'):
+            call()
+    buf = torch.zeros(6 * 64, device='cuda')
+    for shared in (dict(indices=buf.view(torch.int32)[8:32].view(6, 4)), dict(values=buf[100:124].view(6, 4)), dict(rest=buf[378:]), dict(weights=buf[:6])):
+        given = {**dict(indices=idx, values=val, rest=rest, weights=w), **shared}
+        with pytest.raises(N.NativeError, match='overlaps the lists'):
+            P.distill_step(z, **given, grad=buf.view(6, 64))
+    assert N.kernel_launch_count() == before
