@@ -144,7 +144,7 @@ PyObject* quantize_rows(PyObject*, PyObject* const* args, Py_ssize_t n) try {
     }
     EXPECT(cr.of(codes) && codes.scalar_type() == at::kChar && codes.sizes() == x.sizes() && codes.device() == x.device());
     if (!scales.defined()) scales = fresh({rows}, at::kFloat, x);
-    EXPECT(is_vector(scales, rows, x));
+    EXPECT(is_vector(scales, rows, x) && !wants_gradient(scales));
     int status;
     {
         const ReleasedInterpreter other_threads_run;

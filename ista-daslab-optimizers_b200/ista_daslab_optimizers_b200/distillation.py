@@ -45,6 +45,12 @@ def _rows(t, what, dtypes=(torch.float32, torch.bfloat16)):
         raise N.NativeError(f'the rows of {what} overlap')
 
 
+def _tensors(optional=(), **given):
+    for what, t in given.items():
+        if not isinstance(t, torch.Tensor) and not (t is None and what in optional):
+            raise N.NativeError(f'{what} must be a tensor (got {t!r})')
+
+
 def _vector(t, n, what, device, optional=False):
     if optional and t is None:
         return
@@ -61,7 +67,7 @@ def _same_device(device, **tensors):
 
 def _no_tangent_for(call, **tensors):
     for what, t in tensors.items():
-        if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
             raise N.NativeError(f'{call} has no forward-mode derivative: the tangent of {what} would be lost')
 
 
@@ -98,8 +104,9 @@ def quantize_rows(x, codes=None, scales=None):
 
 
 def _explain_quantize(x, codes, scales):
+    _tensors(x=x, codes=codes, scales=scales, optional=('codes', 'scales'))
     _rows(x, 'x')
-    _no_grad_for('quantize_rows', x=x)
+    _no_grad_for('quantize_rows', x=x, scales=scales)
     if codes is not None:
         _rows(codes, 'codes', (torch.int8,))
         if codes.shape != x.shape:
@@ -119,6 +126,7 @@ def int8_matmul(a, b, a_scales, b_scales, bias=None, out=None, dtype=torch.bfloa
 
 
 def _explain_matmul(a, b, a_scales, b_scales, bias, out):
+    _tensors(a=a, b=b, a_scales=a_scales, b_scales=b_scales, bias=bias, out=out, optional=('bias', 'out'))
     _rows(a, 'a', (torch.int8,))
     _rows(b, 'b', (torch.int8,))
     if a.shape[1] != b.shape[1]:
@@ -146,6 +154,7 @@ def topk_logits(logits, k, temperature=1.0):
 
 
 def _explain_topk(logits, k):
+    _tensors(logits=logits)
     _rows(logits, 'logits')
     _no_grad_for('topk_logits', logits=logits)
     if not 1 <= k <= logits.shape[1]:
@@ -153,6 +162,7 @@ def _explain_topk(logits, k):
 
 
 def _explain_lists(what, logits, indices, values, rest, weights, temperature):
+    _tensors(logits=logits, indices=indices, values=values, rest=rest, weights=weights, optional=('rest', 'weights'))
     _no_grad_for(what, values=values, rest=rest, weights=weights)
     _no_tangent_for(what, logits=logits)
     _rows(logits, 'logits')
@@ -201,6 +211,7 @@ def distill_step(logits, indices, values, rest=None, weights=None, temperature=1
 
 def _explain_step(logits, indices, values, rest, weights, temperature, grad):
     _explain_lists('distill_step', logits, indices, values, rest, weights, temperature)
+    _tensors(grad=grad, optional=('grad',))
     _no_tangent_for('distill_step', grad=grad)
     if grad is not None:
         if grad.shape != logits.shape or grad.dtype != logits.dtype or grad.requires_grad:

@@ -126,3 +126,21 @@ def test_overlapping_memory_is_refused(lib, call, wrong):
     """What a call writes lies over what it reads, or over what else it writes, by as little as a byte."""
     assert call(lib, **wrong) == BAD
     assert b'overlap' in lib.mab_last_error()
+
+
+def test_arguments_that_are_no_tensors_are_refused(lib):
+    import ista_daslab_optimizers_b200 as pkg
+    from ista_daslab_optimizers_b200._native import NativeError
+    x, i, v, r, c = torch.zeros(4, 64), torch.zeros(4, 8, dtype=torch.int32), torch.zeros(4, 8), torch.zeros(4), torch.zeros(4, 64, dtype=torch.int8)
+    for other in ([1.0], 3, 'x'):
+        for name, call in (('x', lambda o: pkg.quantize_rows(o)), ('codes', lambda o: pkg.quantize_rows(x, o)), ('scales', lambda o: pkg.quantize_rows(x, None, o)),
+                           ('a', lambda o: pkg.int8_matmul(o, c, r, r)), ('b', lambda o: pkg.int8_matmul(c, o, r, r)), ('a_scales', lambda o: pkg.int8_matmul(c, c, o, r)),
+                           ('b_scales', lambda o: pkg.int8_matmul(c, c, r, o)), ('bias', lambda o: pkg.int8_matmul(c, c, r, r, o)), ('out', lambda o: pkg.int8_matmul(c, c, r, r, None, o)),
+                           ('logits', lambda o: pkg.topk_logits(o, 3)), ('logits', lambda o: pkg.distill_loss(o, i, v)), ('indices', lambda o: pkg.distill_loss(x, o, v)),
+                           ('values', lambda o: pkg.distill_loss(x, i, o)), ('rest', lambda o: pkg.distill_loss(x, i, v, o)), ('weights', lambda o: pkg.distill_loss(x, i, v, r, o)),
+                           ('indices', lambda o: pkg.distill_step(x, o, v)), ('values', lambda o: pkg.distill_step(x, i, o))):
+            with pytest.raises(NativeError, match=name + ' must be a tensor'):
+                call(other)
+    for call in (lambda: pkg.distill_step(x, None, v), lambda: pkg.distill_loss(x, i, None), lambda: pkg.int8_matmul(c, c, None, r)):
+        with pytest.raises(NativeError, match='must be a tensor'):
+            call()

@@ -947,3 +947,23 @@ def test_outputs_between_the_rows_of_inputs():
         with pytest.raises(N.NativeError, match='overlaps the lists'):
             P.distill_step(z, **given, grad=buf.view(6, 64))
     assert N.kernel_launch_count() == before
+
+
+def test_given_outputs_that_ask_for_a_gradient_are_refused():
+    import ista_daslab_optimizers_b200 as P
+    from ista_daslab_optimizers_b200 import _native as N
+    z, idx, val, rest, _ = _problem(6, 64, 4, F32, F32, 1.0, True, False, False)
+    scales, codes = torch.zeros(6, device='cuda', requires_grad=True), torch.zeros(6, 64, dtype=torch.int8, device='cuda')
+    before = N.kernel_launch_count()
+    with pytest.raises(N.NativeError, match='no gradient for scales'):
+        P.quantize_rows(z, codes, scales)
+    with pytest.raises(N.NativeError, match='no gradient for out'):
+        P.int8_matmul(codes, codes, rest, rest, out=torch.zeros(6, 6, device='cuda', requires_grad=True))
+    with pytest.raises(N.NativeError, match='require no gradient itself'):
+        P.distill_step(z, idx, val, rest, grad=z.clone().requires_grad_())
+    with pytest.raises(N.NativeError, match='grad must be a tensor'):
+        P.distill_step(z, idx, val, rest, grad=3.0)
+    assert N.kernel_launch_count() == before
+    with torch.no_grad():
+        P.quantize_rows(z, codes, scales)
+    assert torch.equal(scales, D.quantize(z)[1])
