@@ -170,8 +170,9 @@ int mab_topk_logits(int64_t rows, int64_t vocab, int64_t k, const void* logits, 
 /* loss[r] = weights[r] * KL(teacher || student) over the list's tokens and one class for all others, both distributions at
  * `temperature`: the teacher's from its logits `values` [rows, k] at `indices` [rows, k] and rest[r], the logarithm of the mass of everything
  * else as mab_topk_logits gives it (NULL: none; the teacher's distribution is that over its list), the student's from
- * logits [rows, vocab].  An index outside [0, vocab) is an entry that is not there; an index that occurs again counts with the sum of its
- * entries.  weights [rows] or NULL (all 1): a row with weight 0 is not read, its loss is 0.  A row without a teacher (no entry, no
+ * logits [rows, vocab].  An index outside [0, vocab) is an entry that is not there; an index that occurs again is a
+ * term p log(p / q) for each of its entries: the gradient is that of their sum, the loss lies below KL of the merged entries by the entropy of the split
+ * among them times their share (it can be negative).  weights [rows] or NULL (all 1): a row with weight 0 is not read, its loss is 0.  A row without a teacher (no entry, no
  * rest) has loss 0.  stats [rows, 2] and list_grad [rows, k] are what mab_distill_grad needs. */
 int mab_distill_loss(int64_t rows, int64_t vocab, int64_t k, const void* logits, int dtype, int64_t pitch, const int32_t* indices,
                      const void* values, int v_dtype, const float* rest, const float* weights, double temperature, float* loss,

@@ -7,6 +7,8 @@
 //   tau dloss/dz_v = P q_v - sum_{j: index_j = v} p_j              for v in the list
 //                  = exp(y_v - L_t) (P q_t - p_t)                  elsewhere
 //
+// An index that occurs again has a term of its own for each of its entries: with p = sum p_j over them, sum p_j log(p_j / q) = p log(p / q) - p H(p_j / p), H the entropy of the split.
+//
 // A row belongs to a cluster of one to eight CTAs, each of which has its part of the row in shared memory from the beginning to the end (a bulk copy, on its way while
 // the list is worked on): one pass with a running maximum and sum, and for the gradient a second one that reads no global memory.  The list's positions are
 // overwritten by -inf there, so the sum over the others is their own, not a difference of two large ones.  The k terms of the list are in 64 bits: near the

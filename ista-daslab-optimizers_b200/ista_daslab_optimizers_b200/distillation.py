@@ -187,7 +187,10 @@ def distill_loss(logits, indices, values, rest=None, weights=None, temperature=1
 
     logits          the student's, float32 or bfloat16 [rows, vocab]; the only input with a gradient
     indices, values the teacher's list, int32 and float32 or bfloat16 [rows, k], as `topk_logits` gives it (k at most 1024).  An index outside
-                    [0, vocab) is an entry that is not there (lists of different lengths); one that occurs again counts with the sum of its entries
+                    [0, vocab) is an entry that is not there (lists of different lengths); one that occurs again is a term p log(p / q) for
+                    each of its entries: the gradient is that of the sum of their shares, and the loss lies below the divergence of the merged entries by the
+                    entropy of the split among them times their share, which does not depend on the student (two equal entries with all of the mass: by log 2, so
+                    it can be negative)
     rest            float32 [rows]: the logarithm of the teacher's mass outside its list at this temperature, as `topk_logits` gives it; None: the
                     teacher's distribution is the one over its list
     weights         float32 [rows] or None: a row with weight 0 is not read, whatever it holds, and has loss and gradient 0.  (Multiply by

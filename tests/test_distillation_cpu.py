@@ -144,3 +144,31 @@ def test_arguments_that_are_no_tensors_are_refused(lib):
     for call in (lambda: pkg.distill_step(x, None, v), lambda: pkg.distill_loss(x, i, None), lambda: pkg.int8_matmul(c, c, None, r)):
         with pytest.raises(NativeError, match='must be a tensor'):
             call()
+
+
+def split_entropy(p, idx):
+    """Sum over the indices of a list of p H(p_j / p), p the sum of their entries' p_j: by how much terms of their own lie below those of merged entries."""
+    h = 0.0
+    for i in set(idx):
+        parts = [x for x, j in zip(p, idx) if j == i]
+        h -= sum(x * math.log(x / sum(parts)) for x in parts)
+    return h
+
+
+def test_repeated_indices_against_merged_entries():
+    """A list with repeated indices has the gradient of the list in which they are one entry each, and its loss less the entropy of the split."""
+    g = torch.Generator().manual_seed(1)
+    z = torch.randn(1, 30, generator=g, dtype=torch.float64) * 2
+    idx, val, rest = [4, 9, 4, 7, 9, 4], torch.randn(1, 6, generator=g).double(), torch.randn(1, generator=g).double()
+    merged = sorted(set(idx))
+    sums = torch.stack([torch.logsumexp(val[0, [n for n, j in enumerate(idx) if j == i]], 0) for i in merged])[None]
+    one = D.distill(z, torch.tensor([idx], dtype=torch.int32), val, rest, None, 1.0)
+    two = D.distill(z, torch.tensor([merged], dtype=torch.int32), sums, rest, None, 1.0)
+    p = torch.softmax(torch.cat([val, rest[:, None]], 1), 1)[0, :6].tolist()
+    assert abs(float(two[0] - one[0]) - split_entropy(p, idx)) < 1e-12
+    assert (one[1] - two[1]).abs().max() < 1e-12
+    # two equal entries on a token that the student is sure of
+    z = torch.full((1, 5), -100.0, dtype=torch.float64)
+    z[0, 2] = 100.0
+    loss = D.distill(z, torch.tensor([[2, 2]], dtype=torch.int32), torch.zeros(1, 2), None, None, 1.0)[0]
+    assert abs(float(loss) + math.log(2)) < 1e-12

@@ -967,3 +967,24 @@ def test_given_outputs_that_ask_for_a_gradient_are_refused():
     with torch.no_grad():
         P.quantize_rows(z, codes, scales)
     assert torch.equal(scales, D.quantize(z)[1])
+
+
+@pytest.mark.parametrize('rows', [3, 320])
+def test_repeated_indices_against_merged_entries(rows):
+    """The kernels' loss and gradient with repeated indices, from those of the list in which they are one entry each: the same gradient, and the loss less the entropy of the split."""
+    from ista_daslab_optimizers_b200 import distill_step
+    from test_distillation_cpu import split_entropy
+    vocab, k = 20011, 12
+    z, idx, val, rest, _ = _problem(rows, vocab, k, F32, F32, 1.0, True, False, False)
+    idx[:, 5:8] = idx[:, 1:2]
+    idx[:, 11] = idx[:, 0]
+    loss, grad = distill_step(z, idx, val, rest)
+    v = val.double()
+    v[:, 1] = torch.logsumexp(v[:, [1, 5, 6, 7]], 1)
+    v[:, 0] = torch.logsumexp(v[:, [0, 11]], 1)
+    keep = idx.clone()
+    keep[:, 5:8], keep[:, 11] = -1, -1
+    w_loss, w_grad, size = D.distill(z, keep, v, rest, None, 1.0)
+    p = torch.softmax(torch.cat([val.double(), rest.double()[:, None]], 1), 1)[:, :k].tolist()
+    below = torch.tensor([split_entropy(a, b) for a, b in zip(p, idx.tolist())], dtype=torch.float64, device='cuda')
+    D.assert_distill(loss, grad, (w_loss - below, w_grad, size), vocab, 'repeated')
