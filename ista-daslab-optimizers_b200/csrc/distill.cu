@@ -565,9 +565,12 @@ template <typename T, int MODE> int launch(Args a, int64_t rows, cudaStream_t s)
         return launch_rows(kernel, "distill", rows * a.cluster, NT, list + smem, a.cluster, s, a);
     };
     if (vectors * 16 <= PART) return go(std::true_type(), std::integral_constant<int, 256>(), vectors * 16);
-    if (MODE == LOSS || vectors * 16 <= 140 * 1024) return go(std::false_type(), std::integral_constant<int, 256>(), bits);
-    a.held = (int)std::min<int64_t>((int64_t)vectors, std::max<int64_t>(0, STEP_SHARED - (int64_t)(list + bits)) / 16);
-    return go(std::false_type(), std::integral_constant<int, 512>(), bits + (size_t)a.held * 16);
+    if constexpr (MODE == STEP)
+        if (vectors * 16 > 140 * 1024) {
+            a.held = (int)std::min<int64_t>((int64_t)vectors, std::max<int64_t>(0, STEP_SHARED - (int64_t)(list + bits)) / 16);
+            return go(std::false_type(), std::integral_constant<int, 512>(), bits + (size_t)a.held * 16);
+        }
+    return go(std::false_type(), std::integral_constant<int, 256>(), bits);
 }
 
 template <typename T> int launch_grad(Args a, int64_t rows, cudaStream_t s) {

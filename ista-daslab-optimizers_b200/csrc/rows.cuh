@@ -107,9 +107,6 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-// The value next below that of an order key (ord_key); the two zeros have one key, that of +0.
-__device__ __forceinline__ float below_key(uint32_t key) { return ord_value(key == 0x80000000u ? 0x7FFFFFFEu : key - 1u); }
-
 constexpr float INF_F = __builtin_huge_valf();
 constexpr uint32_t KEY_NEG_INF = 0x007FFFFFu;       // ord_key(-inf); every number lies above it
 // Order key of a value with NaN (0) below -inf and one key for the two zeros.
@@ -135,11 +132,6 @@ __device__ __forceinline__ double cluster_load_f64(const double* p, int rank) {
     asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(cluster_addr(p, rank)) : "memory");
     return v;
 }
-__device__ __forceinline__ float cluster_load_f32(const float* p, int rank) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr(p, rank)) : "memory");
-    return v;
-}
 __device__ __forceinline__ uint32_t cluster_load_u32(const void* p, int rank) {
     uint32_t v;
     asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(cluster_addr(p, rank)) : "memory");
@@ -150,12 +142,6 @@ __device__ __forceinline__ int4 cluster_load_int4(const void* p, int rank) {
     asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(cluster_addr(p, rank)) : "memory");
     return v;
 }
-__device__ __forceinline__ unsigned long long cluster_load_u64(const void* p, int rank) {
-    unsigned long long v;
-    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(cluster_addr(p, rank)) : "memory");
-    return v;
-}
-
 __device__ __forceinline__ void cluster_store_u32(void* p, int rank, uint32_t v) {
     asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr(p, rank)), "r"(v) : "memory");
 }

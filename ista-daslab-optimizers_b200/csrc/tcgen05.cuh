@@ -13,15 +13,6 @@ __device__ __forceinline__ bool elect_one() {
     return p != 0;
 }
 
-// Barriers of some warps of a CTA; the second one also tells whether any thread said so.
-__device__ __forceinline__ void named_barrier(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
-__device__ __forceinline__ bool named_barrier_or(int id, int threads, bool said) {
-    uint32_t any;
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-                 : "=r"(any) : "r"((uint32_t)said), "r"(id), "r"(threads) : "memory");
-    return any != 0;
-}
-
 __device__ __forceinline__ void tmem_alloc(uint32_t* to_smem, uint32_t columns) {       // a whole warp; columns: a power of two, at least 32
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(to_smem)), "r"(columns) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");

@@ -59,7 +59,7 @@ template <class F> struct Shared {
     uint32_t warp_max[F::WARPS], found;
     int scan[40];
     double terms[F::WARPS];                            // of candidates that go into the rest
-};                                                  //   a sum of integers does not depend on it
+};
 
 // Order keys of as many bits as the type has; NaN (0) below -inf, one key for the two zeros.
 template <typename T> struct Key {
