@@ -494,7 +494,7 @@ int launch_ef_topk_quant(const mab_tensor* dev_tensors, int n_tensors, int total
     auto run = [&](auto kern, int stage_bytes_full) -> int {
         const int stage_elems = stage_bytes_full > limit ? 0 : max_dbs;
         const int smem = (stage_elems ? stage_bytes_full : 0) + scratch;
-        MAB_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        if (int rc = allow_shared_memory(reinterpret_cast<const void*>(kern))) return rc;
         kern<<<grid, SEL_THREADS, smem, s>>>(dev_tensors, n_tensors, total_units, qshift, stage_elems, la);
         return MAB_OK;
     };

@@ -930,7 +930,7 @@ int launch_ef_topk_quant_bf16(const mab_tensor* dev_tensors, int n_tensors, int 
     const int per_sm = std::min(S_CTAS, (device_max_optin_smem() + 1024) / (smem + 3 * 1024 + 128));
     if (per_sm < 2) return 1;                                // not even two CTAs per SM: the caller uses the other kernel
     const int grid = (int)std::min<int64_t>(total_units, (int64_t)device_sm_count() * per_sm);
-    MAB_CUDA_TRY(cudaFuncSetAttribute(ef_topk_quant_bf16_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    if (int rc = allow_shared_memory(reinterpret_cast<const void*>(ef_topk_quant_bf16_kernel))) return rc;
     ef_topk_quant_bf16_kernel<<<grid, S_NT, smem, s>>>(dev_tensors, n_tensors, total_units, max_dbs, allowing);
     count_launch();
     cudaError_t e = cudaGetLastError();

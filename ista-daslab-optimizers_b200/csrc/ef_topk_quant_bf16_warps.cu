@@ -1098,7 +1098,7 @@ int launch_ef_topk_quant_bf16_warps(const mab_tensor* dev_tensors, int n_tensors
     LooseArgs la = {0, nullptr, nullptr, nullptr};
     if (loose) la = *loose;
     auto run = [&](auto kern) -> int {
-        MAB_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        if (int rc = allow_shared_memory(reinterpret_cast<const void*>(kern))) return rc;
         kern<<<grid, S_NT, smem, s>>>(dev_tensors, n_tensors, total_units, max_dbs, allowing, la);
         return MAB_OK;
     };

@@ -844,7 +844,7 @@ int launch_ef_topk_quant_f32(const mab_tensor* dev_tensors, int n_tensors, int t
     const int fixed = (int)sizeof(int) * (WIN_MAX_TENSORS + 1) + 128 + 1024;     // static arrays and the per-CTA reservation
     if (max_k > F_MAX_K || F_CTAS * (smem + fixed) > device_max_optin_smem() + 1024) return 1;
     const int grid = (int)std::min<int64_t>(total_units, (int64_t)device_sm_count() * F_CTAS);
-    MAB_CUDA_TRY(cudaFuncSetAttribute(ef_topk_quant_f32_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    if (int rc = allow_shared_memory(reinterpret_cast<const void*>(ef_topk_quant_f32_kernel))) return rc;
     ef_topk_quant_f32_kernel<<<grid, F_NT, smem, s>>>(dev_tensors, n_tensors, total_units, qshift, tile_bytes, allowing);
     count_launch();
     cudaError_t e = cudaGetLastError();

@@ -1166,7 +1166,7 @@ static int launch_window_impl(const mab_tensor* dev_tensors, const mab_tensor* s
     if (L.smem > 0) {
         const int nt = L.threads;
         auto run = [&](auto kern, int threads) -> int {
-            MAB_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L.smem));
+            if (int rc = allow_shared_memory(reinterpret_cast<const void*>(kern))) return rc;
             if constexpr (MODE == MODE_WRITE_UPDATE) kern<<<L.grid, threads, L.smem, s>>>(*single, units_tile, max_k, write == 2, a);
             else MAB_CUDA_TRY(launch_behind_kernel(kern, L.grid, threads, L.smem, s, dev_tensors, n_tensors, units_tile, max_k, L.dense_at, a));
             return MAB_OK;
@@ -1258,7 +1258,7 @@ int launch_window_step(const mab_tensor* dev_tensors, int n_tensors, int units_t
     if (smem > 0) {
         const int sms = device_sm_count(), grid = std::min(units_tile, sms * 2);
         auto kern = behind_a && early_form(units_tile, grid, sms) ? window_resident_kernel<true> : window_resident_kernel<false>;
-        MAB_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        if (int rc = allow_shared_memory(reinterpret_cast<const void*>(kern))) return rc;
         MAB_CUDA_TRY(launch_behind_kernel(kern, grid, WR_THREADS, smem, s, dev_tensors, n_tensors, units_tile, max_k, tile_bytes, a));
         count_launch();
         cudaError_t e = cudaGetLastError();
