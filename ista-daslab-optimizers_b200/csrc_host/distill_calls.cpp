@@ -64,12 +64,12 @@ int code(const at::Tensor& t) { return t.scalar_type() == at::kFloat ? MAB_F32 :
 // A new tensor, straight from the device's allocator.
 at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& like) { return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt); }
 
-// A matrix on a CUDA device whose rows are contiguous: its address and their distance.
+// A matrix on a CUDA device whose rows are contiguous: its address and their distance.  (A tensor whose negation torch has put off, the imaginary part of a conjugate, holds other numbers than its memory.)
 struct Rows {
     void* p = nullptr;
     int64_t pitch = 0;
     bool of(const at::Tensor& t) {
-        if (t.layout() != at::kStrided || t.dim() != 2 || !t.is_cuda()) return false;
+        if (t.layout() != at::kStrided || t.dim() != 2 || !t.is_cuda() || t.is_neg()) return false;
         const int64_t rows = t.size(0), cols = t.size(1);
         if (cols > 1 && t.stride(1) != 1) return false;
         pitch = rows > 1 ? t.stride(0) : std::max<int64_t>(cols, 1);
@@ -80,7 +80,7 @@ struct Rows {
 
 // n contiguous float32 values on the device of `like`.
 bool is_vector(const at::Tensor& t, int64_t n, const at::Tensor& like) {
-    return t.scalar_type() == at::kFloat && t.dim() == 1 && t.size(0) == n && t.device() == like.device() && t.is_contiguous();
+    return t.scalar_type() == at::kFloat && t.dim() == 1 && t.size(0) == n && t.device() == like.device() && t.is_contiguous() && !t.is_neg();
 }
 float* vector_at(const at::Tensor& t) { return t.defined() ? static_cast<float*>(t.data_ptr()) : nullptr; }
 
@@ -220,7 +220,7 @@ struct Lists {
         vocab = logits.size(1);
         if (indices.scalar_type() != at::kInt || indices.dim() != 2 || indices.size(0) != rows || indices.device() != logits.device() || !indices.is_contiguous()) return false;
         k = indices.size(1);
-        if (!is_float(values) || values.sizes() != indices.sizes() || values.device() != logits.device() || !values.is_contiguous()) return false;
+        if (!is_float(values) || values.sizes() != indices.sizes() || values.device() != logits.device() || !values.is_contiguous() || values.is_neg()) return false;
         if ((rest.defined() && !is_vector(rest, rows, logits)) || (weights.defined() && !is_vector(weights, rows, logits))) return false;
         return !wants_gradient(values) && !wants_gradient(rest) && !wants_gradient(weights);
     }
@@ -265,7 +265,7 @@ struct DistillLoss : torch::autograd::Function<DistillLoss> {
                 const at::Tensor& t = saved[i];
                 TORCH_CHECK(t.layout() == at::kStrided && t.is_cuda() && t.device() == up.device() && t.scalar_type() == type && t.dim() >= 1 && t.size(0) == rows,
                             "distill_loss: a saved tensor came back with another device, layout, type or number of rows (hooks for saved tensors have to give back what they got)");
-                return t;
+                return t.resolve_neg();
             };
             const at::Tensor indices = back(1, at::kInt).contiguous(), stats = back(3, at::kFloat).contiguous(), list_grad = back(4, at::kFloat).contiguous();
             const at::Tensor weights = saved[2].defined() ? back(2, at::kFloat).contiguous() : at::Tensor();
@@ -280,6 +280,7 @@ struct DistillLoss : torch::autograd::Function<DistillLoss> {
             }
             const int64_t vocab = logits.size(1);
             if (up.scalar_type() != at::kFloat) up = up.to(at::kFloat);
+            up = up.resolve_neg();
             grad = fresh({rows, vocab}, logits.scalar_type(), logits);
             throw_if(g_library.distill_grad(rows, vocab, indices.size(1), z.p, code(logits), z.pitch, static_cast<const int32_t*>(indices.data_ptr()), vector_at(weights),
                                             ctx->saved_data["temperature"].toDouble(), vector_at(stats), vector_at(list_grad), vector_at(up), up.stride(0),

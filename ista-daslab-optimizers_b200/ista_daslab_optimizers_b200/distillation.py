@@ -49,6 +49,8 @@ def _tensors(optional=(), **given):
     for what, t in given.items():
         if not isinstance(t, torch.Tensor) and not (t is None and what in optional):
             raise N.NativeError(f'{what} must be a tensor (got {t!r})')
+        if t is not None and t.is_neg():
+            raise N.NativeError(f'{what} has a negation that is not resolved yet: hand over {what}.resolve_neg()')
 
 
 def _vector(t, n, what, device, optional=False):

@@ -988,3 +988,83 @@ def test_repeated_indices_against_merged_entries(rows):
     p = torch.softmax(torch.cat([val.double(), rest.double()[:, None]], 1), 1)[:, :k].tolist()
     below = torch.tensor([split_entropy(a, b) for a, b in zip(p, idx.tolist())], dtype=torch.float64, device='cuda')
     D.assert_distill(loss, grad, (w_loss - below, w_grad, size), vocab, 'repeated')
+
+
+# ------------------------------------------------------------------------------------------------ what memory holds, and how far it reaches
+
+def test_tensors_with_a_negation_put_off():
+    """The imaginary part of a conjugate is a view whose memory holds the opposite numbers: it is refused, or resolved where it is the gradient from above."""
+    import ista_daslab_optimizers_b200 as P
+    from ista_daslab_optimizers_b200 import _native as N
+    g = _gen(71)
+    column = torch.complex(_normal(g, 5, 1), _normal(g, 5, 1)).conj().imag
+    one = torch.complex(_normal(g, 1), _normal(g, 1)).conj().imag
+    assert column.is_neg() and one.is_neg()
+    idx, val = torch.zeros(5, 1, dtype=torch.int32, device='cuda'), torch.ones(5, 1, device='cuda')
+    codes = torch.ones(1, 16, dtype=torch.int8, device='cuda')
+    for call in (lambda: P.quantize_rows(column), lambda: P.topk_logits(column, 1), lambda: P.distill_step(column, idx, val), lambda: P.distill_loss(column, idx, val),
+                 lambda: P.int8_matmul(codes, codes, one, one.resolve_neg()), lambda: P.int8_matmul(codes, codes, one.resolve_neg(), one.resolve_neg(), one),
+                 lambda: P.distill_step(val[:1], idx[:1], val[:1], one), lambda: P.distill_step(val[:1], idx[:1], val[:1], None, one)):
+        with pytest.raises(N.NativeError, match='negation'):
+            call()
+    z, idx, val, rest, _ = _problem(5, 500, 4, F32, F32, 1.0, True, False, False)
+    leaf = z.clone().requires_grad_()
+    up = torch.complex(_normal(g, 5), _normal(g, 5)).conj().imag
+    got, = torch.autograd.grad(P.distill_loss(leaf, idx, val, rest), leaf, up)
+    want, = torch.autograd.grad(P.distill_loss(leaf, idx, val, rest), leaf, up.resolve_neg().clone())
+    assert torch.equal(got, want)
+
+
+def test_offsets_beyond_32_bits():
+    """Matrices of more than 2^31 elements, by many rows and by few that lie far apart: their last rows are what they are alone."""
+    from ista_daslab_optimizers_b200 import distill_loss, distill_step, int8_matmul, quantize_rows, topk_logits
+    g = _gen(73)
+    rows, vocab, k = 17000, 128256, 8
+    last = _normal(g, 5, vocab).to(BF16)
+    z = torch.zeros(rows, vocab, dtype=BF16, device='cuda')
+    z[-5:] = last
+    idx = torch.randint(0, vocab, (rows, k), generator=g, device='cuda', dtype=torch.int32)
+    val = _normal(g, rows, k)
+    for whole, alone in zip(topk_logits(z, k), topk_logits(last, k)):
+        assert torch.equal(whole[-5:], alone) or whole.dtype == F32
+        D.assert_near(whole[-5:], alone, 2 * D.sum_error(vocab) + 4 * D.U * alone.abs().float(), 'top')          # (other numbers of blocks a row)
+    want = D.distill(last, idx[-5:], val[-5:], None, None, 1.0)
+    leaf = z.requires_grad_()
+    loss = distill_loss(leaf, idx, val)
+    grad, = torch.autograd.grad(loss.sum(), leaf)
+    D.assert_distill(loss[-5:].detach(), grad[-5:], want, vocab, 'loss')
+    z = z.detach()
+    loss, _ = distill_step(z, idx, val, grad=z)
+    D.assert_distill(loss[-5:], z[-5:], want, vocab, 'step')
+    del grad, leaf
+    # products: 17000 x 128256 outputs
+    a, b = _codes(g, rows, 64), _codes(g, vocab, 64)
+    sa, sb = torch.rand(rows, generator=g, device='cuda'), torch.rand(vocab, generator=g, device='cuda')
+    out = int8_matmul(a, b, sa, sb, out=z)
+    p, tol = D.matmul(a[-300:], b, sa[-300:], sb, None)
+    D.assert_near(out[-300:], p, tol + D.half_step(BF16) * p.abs(), 'product')
+    codes, scales = quantize_rows(z)
+    want_codes, want_scales = D.quantize(z[-300:])
+    assert torch.equal(codes[-300:], want_codes) and torch.equal(scales[-300:], want_scales)
+    # three rows 2^30 + 8 elements apart
+    buf = z.flatten()
+    del z, out, codes
+    far = torch.empty(2 * (2 ** 30 + 8) + 70000, dtype=BF16, device='cuda')
+    del buf
+    x = far.as_strided((3, 70000), (2 ** 30 + 8, 1))
+    x.copy_(_normal(g, 3, 70000))
+    near = x.clone()
+    for p, q in zip(topk_logits(x, 100) + quantize_rows(x) + distill_step(x, idx[:3] % 70000, val[:3]),
+                    topk_logits(near, 100) + quantize_rows(near) + distill_step(near, idx[:3] % 70000, val[:3])):
+        assert torch.equal(p, q)
+    want = distill_step(near, idx[:3] % 70000, val[:3])[1]
+    assert torch.equal(distill_step(x, idx[:3] % 70000, val[:3], grad=x)[1], want)
+    # ... and codes and products as far apart
+    wide = torch.empty(2 * (2 ** 30 + 16) + 4096, dtype=torch.int8, device='cuda')
+    c = wide.as_strided((3, 4096), (2 ** 30 + 16, 1))
+    quantize_rows(x[:, :4096].float(), c)
+    o = far.as_strided((3, 3), (2 ** 30 + 8, 1))
+    s = torch.ones(3, device='cuda')
+    for pad in (c, torch.cat([c, torch.zeros(6, 4096, dtype=torch.int8, device='cuda')])):
+        assert torch.equal(int8_matmul(pad, c, torch.ones(len(pad), device='cuda'), s, dtype=F32)[:3], int8_matmul(pad.contiguous(), c.contiguous(), torch.ones(len(pad), device='cuda'), s, dtype=F32)[:3])
+    assert torch.equal(int8_matmul(c, c, s, s, out=o), int8_matmul(c.contiguous(), c.contiguous(), s, s))
