@@ -68,20 +68,19 @@ __global__ void __launch_bounds__(THREADS) int8_matmul_kernel(const __grid_const
         s_lost = g.give_up;
     }
     if (warp == 1) tmem_alloc(&s_tmem, COLUMNS);
-    wait_for_kernel_before();
+    tmem_fence_before();
+    __syncthreads();
+    tmem_fence_after();
+    // The next kernel begins not before this CTA has its tensor memory: a CTA of it that came first could hold all of it (the pairs take 512 columns) while it waits for this kernel.
+    kernel_before_is_done();
+    const uint32_t acc = s_tmem;
     if (t == 0)
-        for (int i = k0; i < k1 && i < k0 + stages; ++i) load(i, i - k0);           // (only this thread and the copy engine know of the barriers yet)
+        for (int i = k0; i < k1 && i < k0 + stages; ++i) load(i, i - k0);
     for (int i = t; i < BN; i += THREADS) s_token[i] = token0 + i < g.m ? g.a_scales[token0 + i] : 0.0f;
     if (t < BM) {
         const int channel = channel0 + t;
         s_channel[t] = t < g.height && channel < g.n ? make_float2(g.b_scales[channel], g.bias ? g.bias[channel] : 0.0f) : make_float2(0.0f, 0.0f);
     }
-    tmem_fence_before();
-    __syncthreads();
-    tmem_fence_after();
-    // Not before this CTA has its tensor memory: a CTA of the next kernel that came first could hold all of it (the pairs take 512 columns) while it waits for this kernel.
-    allow_next_kernel(ANY_GRID);
-    const uint32_t acc = s_tmem;
 
     if (warp < 2) {
         const bool issuing = elect_one();
