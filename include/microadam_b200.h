@@ -155,8 +155,8 @@ int mab_int8_matmul(int64_t m, int64_t n, int64_t k, const int8_t* a, int64_t a_
                     const float* a_scales, const float* b_scales, const float* bias, void* out, int out_dtype, int64_t out_pitch,
                     void* stream);
 
-/* The same call without any copy of the operands, as if every wait for one had run out: every element of out is NaN (from five tokens on; fewer wait for
- * nothing) and mab_device_error() reads 1 afterwards.  Nothing faults; it exists so that the give-up path can be tested. */
+/* The same call without any copy of the operands, as if every wait for one had run out: every element of out is NaN (but where few tokens
+ * take no tile and wait for nothing) and mab_device_error() reads 1 afterwards.  Nothing faults; it exists so that the give-up path can be tested. */
 int mab_int8_matmul_selftest(int64_t m, int64_t n, int64_t k, const int8_t* a, int64_t a_pitch, const int8_t* b, int64_t b_pitch,
                              const float* a_scales, const float* b_scales, const float* bias, void* out, int out_dtype, int64_t out_pitch,
                              void* stream);

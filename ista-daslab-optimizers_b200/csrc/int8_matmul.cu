@@ -5,11 +5,11 @@
 // detour through shared memory.  One warp issues tiled copies (128 bytes of the inner size, 128-byte swizzle, zeros beyond the edges) into a ring of
 // stages, another the products, the others take the sums out of tensor memory.  Three forms, by the number of tokens (us, B200):
 //
-// * up to 4: no tile at all, a warp per pair of channels, four products an instruction.  Bound by the weights' bytes: 4096 x 4096 3.1 for one token, 4.7 for four (the
-//   tiles from 5 tokens on: 7.5).
+// * up to 2 (4 where the weights are few): no tile at all, a warp per pair of channels, four products an instruction.  Bound by the weights' bytes: 4096 x 4096 3.4 for one token, 5.2 for
+//   four (the tiles from 5 tokens on: 5.5).
 // * up to 64: tiles of at most 128 channels and all tokens; where there are fewer tiles than SMs the inner size is split over the CTAs of a cluster, whose partial
 //   sums meet in distributed shared memory: integers, so in any order the same.  Bound by the weights' bytes and some 5 us before the first and behind the last of them:
-//   41 tokens, 14336 x 4096: 14.8 (59 MB); 16 tokens, 128256 x 4096: 82 (6.4 TB/s). (So, too, up to 128 where the channels are few and the inner size long.)
+//   41 tokens, 14336 x 4096: 14.4 (59 MB); 16 tokens, 128256 x 4096: 80.5 (6.5 TB/s). (So, too, up to 128 where the channels are few and the inner size long.)
 // * more: tiles of two CTAs.  Bound by the tensor cores where the inner size is long: 2048 tokens, 128256 x 4096: 640 to 800 by the state of the power cap (3.4 to 2.7
 //   PFLOP/s, tensor pipe 98.5 % active); 4096^3: 46.5 (2.96); by the stores where it is short, an SM takes some 7 cycles for each 128-byte line that a warp stores to: 768 tokens,
 //   50304 x 768 bf16 33, 777 tokens, 50257 x 767 fp32, where every run of 128 bytes touches two lines, 51 (the stores alone 46).
@@ -333,7 +333,15 @@ __global__ void __launch_bounds__(PAIR_THREADS) int8_matmul_pair_kernel(const __
     if (warp == 1) tmem_free_pair(acc, 512);
 }
 
-// M tokens (m of them there): a warp for R channels, its lanes over the inner size.  (Eight tokens of 14336 x 4096 took 35 us this way, 14.4 as a tile.)
+// 16 codes, by a load that the compiler leaves where it is: the kernel before, which may have written them, was still running when this one began, so they are neither the non-coherent
+// path's (for what nobody writes meanwhile) nor to be asked for before the wait; and all of a round's are on their way together (4 tokens, 4096 x 14336: 24.2 us by plain C++ loads, 19.5).
+__device__ __forceinline__ int4 load_codes(const int8_t* p) {
+    int4 r;
+    asm volatile("ld.global.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p) : "memory");
+    return r;
+}
+
+// M tokens (m of them there): a warp for R channels, its lanes over the inner size.
 template <typename T, int M, int R>
 __global__ void __launch_bounds__(256) int8_rows_kernel(const __grid_constant__ Args g) {
     const int lane = lane_id(), channel0 = (blockIdx.x * 8 + warp_id()) * R;
@@ -351,15 +359,14 @@ __global__ void __launch_bounds__(256) int8_rows_kernel(const __grid_constant__ 
 #pragma unroll
     for (int i = 0; i < M; ++i) a[i] = g.a + (int64_t)min(i, g.m - 1) * g.a_pitch;
     const int whole = g.k / 16;
-    // (ordinary loads: the kernel before, which may have written the codes, was still running when this one began, and the non-coherent path is for what nobody writes meanwhile)
 #pragma unroll 4
     for (int v = lane; v < whole; v += 32) {
         int4 w[R];
 #pragma unroll
-        for (int r = 0; r < R; ++r) w[r] = reinterpret_cast<const int4*>(b[r])[v];
+        for (int r = 0; r < R; ++r) w[r] = load_codes(b[r] + 16 * v);
 #pragma unroll
         for (int i = 0; i < M; ++i) {
-            const int4 x = reinterpret_cast<const int4*>(a[i])[v];
+            const int4 x = load_codes(a[i] + 16 * v);
 #pragma unroll
             for (int r = 0; r < R; ++r)
                 acc[i][r] = __dp4a(x.x, w[r].x, __dp4a(x.y, w[r].y, __dp4a(x.z, w[r].z, __dp4a(x.w, w[r].w, acc[i][r]))));
@@ -455,12 +462,14 @@ template <typename T> int launch_pairs(Args g, int sms, cudaStream_t s) {
     return launch_rows(int8_matmul_pair_kernel<T>, "int8_matmul", pairs * 2, PAIR_THREADS, PAIR_BYTES, 2, s, map_a, map_b, g, tokens, (int)tiles);
 }
 
-constexpr int ROWS_MOST = 4;                       // tokens without a tile
+// Tokens without a tile: one and two, and up to four where the weights are no more than 16 MB.  us, without and with: 4 x 1000 x 512 2.25 and 3.75, 4 x 4096 x 4096 5.2 and 5.45,
+// 4 x 20000 x 1000 7.95 and 7.3, 3 x 14336 x 4096 19.3 and 12.8, 4 x 128256 x 4096 120 and 78; one token of 128256 x 4096 takes 79 without.
+static bool without_tile(int64_t m, int64_t n, int64_t k) { return m <= 2 || (m <= 4 && n * k <= 1 << 24); }
 
 template <typename T> int launch(const Args& g, cudaStream_t s) {
     const int sms = device_sm_count();
     if (sms < 0) return MAB_ERR_CUDA;
-    if (g.m <= ROWS_MOST) {
+    if (without_tile(g.m, g.n, g.k)) {
         const int64_t ctas = ceil_div64(g.n, 16);
         if (g.m == 1) return launch_rows(int8_rows_kernel<T, 1, 2>, "int8_matmul", ctas, 256, 0, 1, s, g);
         if (g.m == 2) return launch_rows(int8_rows_kernel<T, 2, 2>, "int8_matmul", ctas, 256, 0, 1, s, g);

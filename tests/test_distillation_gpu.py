@@ -1068,3 +1068,15 @@ def test_offsets_beyond_32_bits():
     for pad in (c, torch.cat([c, torch.zeros(6, 4096, dtype=torch.int8, device='cuda')])):
         assert torch.equal(int8_matmul(pad, c, torch.ones(len(pad), device='cuda'), s, dtype=F32)[:3], int8_matmul(pad.contiguous(), c.contiguous(), torch.ones(len(pad), device='cuda'), s, dtype=F32)[:3])
     assert torch.equal(int8_matmul(c, c, s, s, out=o), int8_matmul(c.contiguous(), c.contiguous(), s, s))
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('m', [1, 2, 3, 4, 5])
+@pytest.mark.parametrize('n,k', [(4097, 4095), (4097, 4097), (33000, 515), (1200, 16001)])
+def test_int8_matmul_of_few_tokens_on_both_sides_of_the_border(m, n, k, dtype):
+    from ista_daslab_optimizers_b200 import int8_matmul
+    g = _gen(m * 7 + n * 3 + k)
+    a, b = _codes(g, m, k), _codes(g, n, k)
+    sa, sb, bias = torch.rand(m, generator=g, device='cuda') + 0.01, torch.rand(n, generator=g, device='cuda') * 0.01, _normal(g, n, scale=50.0)
+    want, tol = D.matmul(a, b, sa, sb, bias)
+    D.assert_near(int8_matmul(a, b, sa, sb, bias, dtype=dtype), want, tol + (0 if dtype == F32 else D.half_step(dtype) * want.abs()), 'product')
