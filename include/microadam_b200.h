@@ -144,7 +144,7 @@ int mab_sparse_rows_combine(int64_t d, int64_t rows, int64_t k, int64_t d_block_
 
 /* scales[r] = max |x[r, :]| / 127 (0 where that lies below 2^-126), codes[r, c] = the integer nearest x[r, c] / scales[r] (half to
  * even, the exact quotient decides), 0 where the scale is 0.  A row with a NaN or an infinity: scale NaN, codes 0.  The operands of
- * mab_int8_matmul: rows are tokens of activations or output channels of weights.  x is read once. */
+ * mab_int8_matmul: rows are tokens of activations or output channels of weights.  Rows of up to 16384 floats (32768 bf16) are read once. */
 int mab_quantize_rows(int64_t rows, int64_t cols, const void* x, int x_dtype, int64_t x_pitch, int8_t* codes,
                       int64_t codes_pitch, float* scales, void* stream);
 
@@ -184,7 +184,8 @@ int mab_distill_grad(int64_t rows, int64_t vocab, int64_t k, const void* logits,
                      const float* weights, double temperature, const float* stats, const float* list_grad, const float* grad_loss,
                      int64_t grad_loss_stride, void* grad, int64_t grad_pitch, void* stream);
 
-/* Both in one call, with grad_loss = 1: a row is read from HBM once.  grad may be logits itself. */
+/* Both in one call, with grad_loss = 1.  A row is read once where a block, or few rows' four, hold it in shared memory (66 KB each); of a longer one the rest is read
+ * twice, from L2 as far as it is still there.  grad may be logits itself. */
 int mab_distill_step(int64_t rows, int64_t vocab, int64_t k, const void* logits, int dtype, int64_t pitch, const int32_t* indices,
                      const void* values, int v_dtype, const float* rest, const float* weights, double temperature, float* loss,
                      void* grad, int64_t grad_pitch, void* stream);

@@ -17,7 +17,7 @@
 // results do not depend on timing.
 //
 // Bound by HBM and by the chain of phases around the passes (list, block and cluster sums, three logarithms: some 5 us a row, which the SM's other rows cover in part).
-// bf16, rows of 128256, k = 64 (us): loss of 1536 rows 75 (5.2 TB/s), its gradient 149 (6.2 TB/s), loss and gradient of 4096 rows in one call 443 (4.7 TB/s of the two passes
+// bf16, rows of 128256, k = 64 (us): loss of 1536 rows 75 (5.2 TB/s), its gradient 149 (6.2 TB/s), loss and gradient of 4096 rows in one call 442 (4.7 TB/s of the two passes
 // over HBM that it needs; what it holds and what L2 keeps leave 1.09 of their bytes; 569 before anything was held).
 #include <initializer_list>
 #include <type_traits>
@@ -539,9 +539,9 @@ static int cluster_of(int64_t rows, int64_t bytes, int sms) {
     return c;
 }
 
-// Parts of up to 66 KB are held as a whole, by clusters of four where a step has few rows (us, one CTA a row and four: 300 rows of 128256 bf16 53 and 47, 600 rows 84
-// and 85: a cluster's exchange costs some 2 us a row).  Longer rows: the loss reads its row once anyway; a step reads what it does not hold a second time, from L2 if the
-// rows under way fit there.  Up to 140 KB they do with four CTAs of 256 threads an SM (2048 rows of 50257 bf16: 97, with two of 512 threads that hold 100 KB each 114; of
+// Parts of up to 66 KB are held as a whole, by clusters of four where a step has few rows (us, one CTA a row and four: 300 rows of 128256 bf16 52 and 47, 600 rows 83
+// and 85: a cluster's exchange costs some 2 us a row; the border of 296 rows lies below both, what is best between them goes by how the waves fall and is not measured).  Longer rows: the loss reads its row once anyway; a step reads what it does not hold a second time, from L2 if the
+// rows under way fit there.  Up to 140 KB they do with four CTAs of 256 threads an SM (2048 rows of 50257 bf16: 93 to 97, with two of 512 threads that hold 100 KB each 114; of
 // 80000: 153 and 147), beyond 400 KB a part only with more CTAs a row (1000 rows of 151936 fp32: 325, with two 266, with four 262).
 template <typename T, int MODE> int launch(Args a, int64_t rows, cudaStream_t s) {
     const int sms = device_sm_count();

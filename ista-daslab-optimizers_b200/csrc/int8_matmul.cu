@@ -3,7 +3,8 @@
 // The tensor cores' rows (128 lanes of tensor memory) are output channels (rows of b), their columns tokens (rows of a): a few tokens are a
 // narrow tile, not a nearly empty one, and a warp of the epilogue holds 32 neighbouring channels of one token, so its stores are runs of 64 or 128 bytes without a
 // detour through shared memory.  One warp issues tiled copies (128 bytes of the inner size, 128-byte swizzle, zeros beyond the edges) into a ring of
-// stages, another the products, the others take the sums out of tensor memory.  Three forms, by the number of tokens (us, B200):
+// stages, another the products, the others take the sums out of tensor memory.  Three forms, by the number of tokens (us, B200; here and in the other kernels of rows: a call in a row of calls
+// from a graph, several sets of inputs in turn, so without the host):
 //
 // * up to 2 (4 where the weights are few): no tile at all, a warp per pair of channels, four products an instruction.  Bound by the weights' bytes: 4096 x 4096 3.4 for one token, 5.2 for
 //   four (the tiles from 5 tokens on: 5.5).
@@ -11,8 +12,9 @@
 //   sums meet in distributed shared memory: integers, so in any order the same.  Bound by the weights' bytes and some 5 us before the first and behind the last of them:
 //   41 tokens, 14336 x 4096: 14.4 (59 MB); 16 tokens, 128256 x 4096: 80.5 (6.5 TB/s). (So, too, up to 128 where the channels are few and the inner size long.)
 // * more: tiles of two CTAs.  Bound by the tensor cores where the inner size is long: 2048 tokens, 128256 x 4096: 640 to 800 by the state of the power cap (3.4 to 2.7
-//   PFLOP/s, tensor pipe 98.5 % active); 4096^3: 46.5 (2.96); by the stores where it is short, an SM takes some 7 cycles for each 128-byte line that a warp stores to: 768 tokens,
-//   50304 x 768 bf16 33, 777 tokens, 50257 x 767 fp32, where every run of 128 bytes touches two lines, 51 (the stores alone 46).
+//   PFLOP/s, tensor pipe 98.4 % active); 4096^3: 46.3 (2.97); by the stores where it is short, an SM takes some 7 cycles for each 128-byte line that a warp stores to: 768 tokens,
+//   50304 x 768 bf16 33, 777 tokens, 50257 x 767 fp32, where every run of 128 bytes touches two lines, 51 (the stores alone 46; 57 to 59 with outputs that were not in L2), 2048 tokens,
+//   50257 x 768 fp32 152.  Rows through shared memory and bulk copies, from tiles that overlap by 16 bytes, took 53, and 114 for the 2048: not in the code, and the border between them not measured.
 #include "rows.cuh"
 #include "tcgen05.cuh"
 

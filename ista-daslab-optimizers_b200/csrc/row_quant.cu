@@ -1,10 +1,12 @@
 // Rows into 8-bit integers with one scale each: s = max |x| / 127, code = the integer nearest x / s (half to even).
 //
-// A row is held in the registers of its threads between the maximum and the codes, so it is read once: bound by HBM (2 or 4 bytes in, one out).  y = x RN(1/s) is off
+// A row is held in the registers of its threads between the maximum and the codes, so it is read once (beyond 4096 vectors of 16 bytes, 16384 fp32 or 32768 bf16 values, what is beyond is
+// fetched again): bound by HBM (2 or 4 bytes in, one out).  y = x RN(1/s) is off
 // the quotient by less than 2^-15, so rint(y) is the code unless y lies that near to a half; a vector in which one does is coded again by exact residuals:
 // where x - c s of the code c = rint(y) (exact in one FMA: c has 7 bits and cancels all but the last bits of x) lies beyond s / 2, or on it with c odd,
 // the neighbour is the code.  The first way takes 5 operations a value (packed products, the rounding by adding 1.5 2^23, whose low byte is the code), the
-// second, for every value, took 43: 14336 x 4096 bf16 42 us against 72, 2047 x 14336 fp32 30 (4.9 TB/s) against 47.
+// second, for every value, took 43: 14336 x 4096 bf16 42 us (4.2 TB/s) against 72, 2047 x 14336 fp32 30 (4.9 TB/s) against 47.  What keeps bf16 from HBM's rate: a CTA's loads stop while
+// it reduces and codes its row.
 #include "rows.cuh"
 
 namespace mab {

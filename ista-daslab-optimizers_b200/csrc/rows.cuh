@@ -154,7 +154,7 @@ __device__ __forceinline__ void cluster_store_f64(void* p, int rank, double v) {
 
 // Kernels that are launched by `launch_rows` begin while the one before them in the stream ends (programmatic launches): what a kernel does before this call
 // touches no global memory but its parameters, and every thread of every CTA makes it, since the completion of one is what the next relies on.  Its own successor may be
-// launched from here on.  What is saved is the gap between two kernels: us a call in a row of calls, without and so: topk_logits of 59 rows of 1363 8.2 / 6.7, int8_matmul of
+// launched from here on.  What is saved is the gap between two kernels: us a call in a row of calls, without and so, when it was brought in: topk_logits of 59 rows of 1363 8.2 / 6.7, int8_matmul of
 // 41 x 1000 x 512 8.2 / 6.2, distill_step of 8 rows of 8000 8.2 / 6.5, 16 x 4096 x 4096 10.2 / 6.9.  A kernel that takes tensor memory makes this call behind the barrier
 // that follows the allocation.
 __device__ __forceinline__ void kernel_before_is_done() {

@@ -11,7 +11,8 @@
 //
 // Bound by the chains of phases around the stream (about a quarter of a row's time with six rows on an SM), by the special-function units, which an exponential
 // per logit keeps busy for 75 us of 2048 x 128256 bf16, and by the sample's second reading: that takes 109 us with k = 64 (4.8 TB/s; the stream alone 84, plain reading 78), 93
-// with k = 10; 5 x 50257 fp32 with k = 20 10.1.
+// with k = 10; 5 x 50257 fp32 with k = 20 10.1.  Further from the bytes are lists above 128, whose bounds are found a bit a step and which a network sorts (4096 x 128256, k = 256: 429, 2.4 TB/s;
+// 2048 x 20000, k = 130: 98), and short rows, which the sample reads whole before the stream does (2048 x 8000, k = 64: 33).
 #include "rows.cuh"
 
 namespace mab {

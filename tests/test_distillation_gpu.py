@@ -1080,3 +1080,22 @@ def test_int8_matmul_of_few_tokens_on_both_sides_of_the_border(m, n, k, dtype):
     sa, sb, bias = torch.rand(m, generator=g, device='cuda') + 0.01, torch.rand(n, generator=g, device='cuda') * 0.01, _normal(g, n, scale=50.0)
     want, tol = D.matmul(a, b, sa, sb, bias)
     D.assert_near(int8_matmul(a, b, sa, sb, bias, dtype=dtype), want, tol + (0 if dtype == F32 else D.half_step(dtype) * want.abs()), 'product')
+
+
+@pytest.mark.parametrize('use_reentrant', [False, True])
+def test_loss_inside_a_checkpoint(use_reentrant):
+    """The student's head and its loss computed again in the backward pass instead of being kept: the gradients are the same."""
+    from ista_daslab_optimizers_b200 import distill_loss
+    from torch.utils.checkpoint import checkpoint
+    _, idx, val, rest, w = _problem(20, 3001, 8, F32, F32, 1.0, True, True, True)
+    g = _gen(81)
+    hidden, weight = _normal(g, 20, 64).requires_grad_(), _normal(g, 3001, 64, scale=0.2).requires_grad_()
+
+    def loss(h, u):
+        return distill_loss(h @ u.t(), idx, val, rest, w).sum()
+
+    want = torch.autograd.grad(loss(hidden, weight), (hidden, weight))
+    for _ in range(2):
+        hidden.grad = weight.grad = None
+        checkpoint(loss, hidden, weight, use_reentrant=use_reentrant).backward()
+        assert torch.equal(hidden.grad, want[0]) and torch.equal(weight.grad, want[1])
