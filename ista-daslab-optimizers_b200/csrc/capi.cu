@@ -2,8 +2,8 @@
 #include <math.h>
 #include <string.h>
 #include <atomic>
+#include <exception>
 #include <mutex>
-#include <utility>
 #include <vector>
 #include <algorithm>
 #include "common.cuh"
@@ -47,24 +47,33 @@ int device_sm_count() {
     return cached;
 }
 
-// The limit belongs to the kernel on the device, not to a launch, and calls come from several threads at once: set to what one launch needs, it could be lowered by another before that
-// launch.  So it is set once per kernel and device, to all that a block can have beside the kernel's static memory.
-int allow_shared_memory(const void* kernel) {
+// The limit belongs to the kernel in the device's context, not to a launch, and calls come from several threads at once: set to what one launch needs, it could be lowered by another
+// before that launch.  So every call sets it to the same number, all that a block can have beside the kernel's static memory.  (That number is kept; that it was set is not, a context can be
+// reset.)
+int allow_shared_memory(const void* kernel) try {
+    struct Known { int dev; const void* kernel; int most; };
     static std::mutex mutex;
-    static std::vector<std::pair<int, const void*>> allowed;         // sorted
-    int dev = 0;
+    static std::vector<Known> known;
+    int dev = 0, most = -1;
     MAB_CUDA_TRY(cudaGetDevice(&dev));
-    const std::pair<int, const void*> key(dev, kernel);
-    const std::lock_guard<std::mutex> lock(mutex);
-    const auto at = std::lower_bound(allowed.begin(), allowed.end(), key);
-    if (at != allowed.end() && *at == key) return MAB_OK;
-    const int most = device_max_optin_smem();
-    if (most < 0) return MAB_ERR_CUDA;
-    cudaFuncAttributes attr;
-    MAB_CUDA_TRY(cudaFuncGetAttributes(&attr, kernel));
-    MAB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most - (int)attr.sharedSizeBytes));
-    allowed.insert(at, key);
+    {
+        const std::lock_guard<std::mutex> lock(mutex);
+        for (const Known& k : known) if (k.kernel == kernel && k.dev == dev) { most = k.most; break; }
+    }
+    if (most < 0) {
+        const int all = device_max_optin_smem();
+        if (all < 0) return MAB_ERR_CUDA;
+        cudaFuncAttributes attr;
+        MAB_CUDA_TRY(cudaFuncGetAttributes(&attr, kernel));
+        most = all - (int)attr.sharedSizeBytes;
+        const std::lock_guard<std::mutex> lock(mutex);
+        known.push_back({dev, kernel, most});
+    }
+    MAB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
     return MAB_OK;
+} catch (const std::exception& e) {
+    set_error("shared memory of a kernel: %s", e.what());
+    return MAB_ERR_CUDA;
 }
 
 int device_max_optin_smem() { return device_attr(cudaDevAttrMaxSharedMemoryPerBlockOptin, "query shared memory per block"); }
