@@ -172,9 +172,10 @@ static inline bool apart(const Span& a, const Span& b) {
     const uintptr_t a0 = reinterpret_cast<uintptr_t>(a.p), a1 = a0 + (a.rows - 1) * a.pitch + a.width;
     const uintptr_t b0 = reinterpret_cast<uintptr_t>(b.p), b1 = b0 + (b.rows - 1) * b.pitch + b.width;
     if (a1 <= b0 || b1 <= a0) return true;
-    if (a.pitch != b.pitch || a.rows == 1 || b.rows == 1) return false;
-    const int64_t ahead = ((int64_t)(b0 - a0) % a.pitch + a.pitch) % a.pitch;      // where b's rows begin, from the beginnings of a's
-    return ahead >= a.width && ahead + b.width <= a.pitch;
+    if ((a.rows == 1 && b.rows == 1) || (a.rows > 1 && b.rows > 1 && a.pitch != b.pitch)) return false;
+    const int64_t pitch = a.rows > 1 ? a.pitch : b.pitch;
+    const int64_t ahead = ((int64_t)(b0 - a0) % pitch + pitch) % pitch;            // where b's rows begin, from the beginnings of a's
+    return ahead >= a.width && ahead + b.width <= pitch;
 }
 static inline Span vector_span(const void* p, int64_t bytes) { return {p, 1, bytes, bytes}; }
 

@@ -1099,3 +1099,18 @@ def test_loss_inside_a_checkpoint(use_reentrant):
         hidden.grad = weight.grad = None
         checkpoint(loss, hidden, weight, use_reentrant=use_reentrant).backward()
         assert torch.equal(hidden.grad, want[0]) and torch.equal(weight.grad, want[1])
+
+
+def test_scales_behind_a_row():
+    """A vector in the gap behind a row of the output shares no byte with it; one that reaches the next row does."""
+    import ista_daslab_optimizers_b200 as P
+    from ista_daslab_optimizers_b200 import _native as N
+    g = _gen(91)
+    x = _normal(g, 5, 256)
+    record = torch.zeros(5, 256 + 32, dtype=torch.uint8, device='cuda')
+    codes, scales = record.view(torch.int8)[:, :256], record.view(F32)[1, 64:69]
+    P.quantize_rows(x, codes, scales)
+    want, want_scales = D.quantize(x)
+    assert torch.equal(codes, want) and torch.equal(scales, want_scales)
+    with pytest.raises(N.NativeError, match='overlap'):
+        P.quantize_rows(x, codes, record.view(F32).flatten()[72 + 68:72 + 73])
